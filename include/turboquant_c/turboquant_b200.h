@@ -531,6 +531,63 @@ int tq_decode_buffer_values(tq_decode_buffer_t buf, int start, int end, void* ou
 int tq_hybrid_attention(tq_kv_cache_t cache, tq_decode_buffer_t buf, int layer, const void* queries, int q_dtype,
                         int q_heads, void* out_fp16, void* stream);
 
+/* ---- the paged 8-bit KV cache -------------------------------------------------------------
+ * One cache for the requests of a server, in pages of 16, 32, 64 or 128 tokens (the reference's holds one sequence,
+ * include/turboquant/kv_cache.h:42-133).  Lengths, tables and the free pages live on the device: a loop in which the device decides
+ * how many tokens a request gets (drafts that are accepted or not) never waits for the host, and a step can be captured in a graph.
+ *
+ * Keys and values are held as whole numbers -127 .. 127 times a power of two for each page and KV head, keys and values apart: the
+ * smallest 2^e, e >= -100, with which the largest magnitude does not round to more than 127 (to the nearest, ties to even).  Tokens
+ * that join a page which holds older ones make its scale larger where they need to, never smaller, and the older numbers are then
+ * rounded once more (truncation leaves scales as they are).  A NaN or an infinity makes the scale of its page and head NaN, and with it every row of the attention that
+ * sees a token of that page and head, until the page is begun anew.
+ *
+ * A step is a plan, then an append and an attention per layer, in stream order.  All calls on a cache must be ordered (one stream, or
+ * events between streams); they work on the cache's device whichever is current.  Data pointers are device pointers, except for rows, counts and
+ * lengths, which may be host memory where the stream is not being captured.  A captured graph that appends or attends holds
+ * its plan too. */
+typedef struct tq_paged_cache_s* tq_paged_cache_t;
+
+/** head_dim 64 or 128; max_requests (rows of the block tables) up to 4096; max_tokens: new tokens of a plan at most.  All
+ *  memory is allocated here: num_layers * num_pages * num_heads * (2 * page_tokens * head_dim + 32) bytes, and tables. */
+tq_paged_cache_t tq_paged_cache_create(int num_layers, int num_heads, int head_dim, int num_pages, int page_tokens, int max_requests,
+                                       int max_pages_per_request, int max_tokens);
+void tq_paged_cache_free(tq_paged_cache_t cache);
+
+/** counts[i] more tokens for the request in row rows[i] (NULL: row i), each row at most once, 0 <= counts[i] <= max_count, `tokens` in
+ *  all or fewer.  Takes the pages that they need off the free ones, in the requests' order.  Outputs, each NULL or a device array:
+ *    starts    [n + 1]   first of each request's rows in the step's tensors; starts[n] = their number
+ *    lengths   [n]       tokens that the request holds, the new ones included
+ *    slots     [tokens]  page * page_tokens + place in the page of each new token, -1 behind the last
+ *    positions [tokens]  its position in the request (as tq_rope_f16 takes them), 0 behind the last
+ *    tables    [n, tables_width]  the requests' pages, -1 behind the last (and cut to the width)
+ *  A batch that does not fit (a bad row or count, a row of the tables or the free pages used up) changes nothing: its starts are 0,
+ *  its slots -1, the step's appends and attentions do nothing, and tq_paged_status tells. */
+int tq_paged_plan(tq_paged_cache_t cache, const int* rows, const int* counts, int n, int tokens, int max_count, int* starts, int* lengths,
+                  int* slots, int* positions, int* tables, int tables_width, void* stream);
+/** The request in row rows[i] keeps its first lengths[i] tokens (0: it is gone); its other pages become free, to be taken in the same order
+ *  again.  All or nothing, as above.  Ends the plan in force. */
+int tq_paged_truncate(tq_paged_cache_t cache, const int* rows, const int* lengths, int n, void* stream);
+/** Keys and values [tokens, heads, head_dim] of the planned tokens (TQ_F32 or TQ_F16), token t at t * stride elements (heads * head_dim
+ *  or more: a slice of a fused projection's result), into a layer.  `tokens` is the plan's; rows behind the last request's are not read.
+ *  Fastest where pointers and strides are multiples of 16 bytes. */
+int tq_paged_append(tq_paged_cache_t cache, int layer, const void* keys, const void* values, int dtype, int tokens, long key_stride,
+                    long value_stride, void* stream);
+/** The values that whole pages hold: [n, page_tokens, heads, head_dim] each, TQ_F32 or TQ_F16, 16-byte aligned, either of them NULL.  Pages are
+ *  device memory; one outside the cache leaves its rows as they are (tq_paged_status). */
+int tq_paged_read(tq_paged_cache_t cache, int layer, const int* pages, int n, void* keys, void* values, int dtype, void* stream);
+/** Attention of the planned tokens' queries, fp16 [tokens, q_heads, head_dim], over their requests' tokens: the one at position p sees
+ *  max(0, p - window + 1) .. p, all up to p with window 0.  q_heads is a multiple of the KV heads, whose groups are
+ *  contiguous.  scale 0: 1 / sqrt(head_dim).  out fp16 of the queries' shape, strides in elements from token to token; lse
+ *  (may be NULL): fp32 [tokens, q_heads], the log of each softmax denominator, with which parts merge
+ *  (tq_exchange_merge_attention).  Rows behind the last request's are left as they are.  Results do not depend on the order in which CTAs run. */
+int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window,
+                       float scale, void* out_fp16, long out_stride, float* lse, void* stream);
+/** Non-zero, once, when a call that has finished found its batch impossible or a wait on the device ran out. */
+int tq_paged_status(tq_paged_cache_t cache);
+/** Free pages, once all work on the device is done (waits for it); -1 on error. */
+int tq_paged_free_pages(tq_paged_cache_t cache);
+
 #ifdef __cplusplus
 }
 #endif

@@ -162,6 +162,16 @@ def load() -> C.CDLL:
     sig("tq_decode_buffer_values", i, [vp, i, i, vp, vp])
     sig("tq_hybrid_attention", i, [vp, vp, i, vp, i, i, vp, vp])
 
+    sig("tq_paged_cache_create", vp, [i, i, i, i, i, i, i, i])
+    sig("tq_paged_cache_free", None, [vp])
+    sig("tq_paged_plan", i, [vp, vp, vp, i, i, i, vp, vp, vp, vp, vp, i, vp])
+    sig("tq_paged_truncate", i, [vp, vp, vp, i, vp])
+    sig("tq_paged_append", i, [vp, i, vp, vp, i, i, C.c_long, C.c_long, vp])
+    sig("tq_paged_read", i, [vp, i, vp, i, vp, vp, i, vp])
+    sig("tq_paged_attention", i, [vp, i, vp, i, i, C.c_long, i, C.c_float, vp, C.c_long, vp, vp])
+    sig("tq_paged_status", i, [vp])
+    sig("tq_paged_free_pages", i, [vp])
+
     sig("tq_distributed_init", vp, [C.c_char_p, C.c_char_p])
     sig("tq_distributed_init_local", vp, [])
     sig("tq_distributed_rank", i, [vp])

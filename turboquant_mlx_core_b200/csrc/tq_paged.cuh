@@ -1,0 +1,142 @@
+// The paged 8-bit KV cache: how it lies in memory, and what its kernels share.
+//
+// A page holds P tokens of every KV head.  The piece of a page that belongs to one head is one block of memory:
+//
+//   [keys P x D bytes][values P x D bytes][key scale, value scale, 24 bytes unused]
+//
+// so that a copy engine fetches a head's tokens of a page in three contiguous pieces and neither the number of heads nor the
+// order of the pages matters.  A byte is code + 128, code -127 .. 127; the value is code * scale, the scale a power of two
+// (or NaN: the block received a value that was not finite).  Powers of two make every product with a scale exact, a code that
+// is rounded again when its block's scale grows loses half a step at most, and scales of different pages are taken together
+// inside a matrix product without a rounding.
+//
+// The 16-byte chunks of a token's row stand in an order that depends on the token (key_chunk, value_chunk): the attention
+// kernel's warps read the rows of eight tokens at once from shared memory, which lie a multiple of 64 bytes apart, and would meet
+// in the same banks otherwise.
+#pragma once
+
+#include <cstdint>
+
+#include "tq_common.cuh"
+
+namespace tq {
+
+constexpr int kPagedMaxRequests = 4096;
+constexpr int kPagedMinExponent = -100;
+constexpr int kPagedTail = 32;   // bytes behind a block's codes
+
+__host__ __device__ __forceinline__ size_t paged_block_bytes(int page_tokens, int dim) {
+    return 2 * static_cast<size_t>(page_tokens) * dim + kPagedTail;
+}
+// Where chunk c (16 dims) of a token's keys or values stands in its row.
+template <int D>
+__device__ __forceinline__ int key_chunk(int token, int c) {
+    if constexpr (D == 128) return c ^ ((token & 1) << 2);
+    else return c;
+}
+template <int D>
+__device__ __forceinline__ int value_chunk(int token, int c) {
+    if constexpr (D == 128) return c ^ (((token >> 1) & 3) << 1);
+    else return c ^ ((token >> 1) & 3);
+}
+
+// What the device keeps of the last plan, beside the arrays of PagedBatch.
+struct PagedHeader {
+    int free_pages;      // pages on the stack
+    int requests, tokens, pieces;   // of the plan (all 0 where it was refused)
+};
+// A run of new tokens in one page.
+struct PagedPiece {
+    int token, count, page, offset;
+};
+// Device arrays of a cache that its kernels read (and the plan writes).
+struct PagedBatch {
+    PagedHeader* header;
+    int* lengths;          // [max_requests] tokens that each row of the tables holds
+    int* tables;           // [max_requests][max_pages]
+    int* stack;            // [num_pages] free pages, the next ones last
+    int* rows;             // [max_requests] of the plan: row of the tables, first token, tokens held with the new ones
+    int* starts;           // (+ 1)
+    int* held;
+    PagedPiece* pieces;
+    int max_requests, max_pages, num_pages, page_tokens, max_pieces;
+};
+
+// Status codes of the paged cache's kernels.
+enum PagedStatus : unsigned int {
+    kPagedOk = 0,
+    kPagedBadRow = 1,      // a row outside the tables, or twice
+    kPagedBadCount = 2,    // a negative count, one above max_count, or more tokens in all than announced
+    kPagedLongRequest = 3, // a request would need more pages than a table's row holds
+    kPagedNoPages = 4,     // not enough free pages
+    kPagedBadLength = 5,   // truncation to a length that the request does not have
+    kPagedBadPage = 6,     // a page number outside the cache
+    kPagedWait = 7         // a bounded wait ran out
+};
+
+// ---- launches (tq_paged_plan.cu) ---------------------------------------------------------------
+struct PagedPlanArgs {
+    PagedBatch b;
+    const int* rows;      // or null: 0, 1, ...
+    const int* counts;
+    int n, tokens, max_count;
+    int* starts;          // outputs, any of them null
+    int* lengths;
+    int* slots;
+    int* positions;
+    int* tables;
+    int tables_width;
+    unsigned int* status;
+};
+void launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st);
+// counts: the lengths to keep
+void launch_paged_truncate(const PagedPlanArgs& a, cudaStream_t st);
+void launch_paged_init(uint8_t* layer, size_t blocks, size_t block_bytes, cudaStream_t st);
+
+struct PagedAppendArgs {
+    const PagedHeader* header;
+    const PagedPiece* pieces;
+    uint8_t* layer;
+    const void* keys;
+    const void* values;
+    long key_stride, value_stride;   // elements from token to token
+    int heads, page_tokens, tokens, num_pages;
+};
+void launch_paged_append(const PagedAppendArgs& a, int dim, bool half, int n, int max_count, cudaStream_t st);
+
+struct PagedReadArgs {
+    const uint8_t* layer;
+    const int* pages;
+    void* keys;
+    void* values;
+    int n, heads, page_tokens, num_pages;
+    unsigned int* status;
+};
+void launch_paged_read(const PagedReadArgs& a, int dim, bool half, cudaStream_t st);
+
+// ---- attention (tq_paged_attention.cu) -----------------------------------------------------------
+// An item that several CTAs share, as the CTA in which it begins leaves it for the kernel that adds the parts up.
+struct PagedJoin {
+    int last;        // the CTA in which it ends; 0: nothing to join (CTA 0 is never a last one)
+    int token;       // first token of its request
+    int first_row;   // rows (token-major: row = token * group + head of the group) first_row ..
+    int rows;        // ... and how many
+    int head;        // KV head
+};
+struct PagedAttnArgs {
+    PagedBatch b;
+    const uint8_t* layer;
+    const __half* q;
+    __half* out;
+    float* lse;          // or null
+    long q_stride, out_stride;
+    int n, tokens, heads, group, window;
+    float scale_log2;    // softmax scale times log2(e)
+    float* partial;
+    PagedJoin* joins;
+    unsigned int* status;
+};
+size_t paged_attn_scratch_bytes(int dim, int sms);
+void launch_paged_attention(const PagedAttnArgs& a, int dim, int max_count, void* scratch, int sms, cudaStream_t st);
+
+}  // namespace tq

@@ -1,0 +1,598 @@
+// Attention over the paged 8-bit KV cache: the new tokens' queries against all tokens of their request up to their own.
+//
+//   s = q . k scale,  o = sum softmax(s) v          q [tokens, heads * group, D] fp16, k and v code * 2^e of a page and head
+//
+// The query rows of a request and KV head are its new tokens times the heads of the group, token-major.  paged_attn_kernel takes them 16 at a time:
+// the decode step's kernel, bound by the bytes of the cache.  Every CTA streams an equal share of all (request, KV head, 16
+// rows, 64 tokens) units, whatever the requests' lengths, which only the device knows: it sums them up first and finds its share by
+// itself.  An item (request, KV head, 16 rows) that ends in another CTA than it begins in is added up by paged_join_kernel, in order.
+//
+// One warp copies (bulk copies into a ring, an mbarrier per stage); four multiply, 16 tokens of a tile each, with a softmax of
+// their own, so that they meet only at an item's end.  Products are mma.sync.m16n8k16 on halves, into which the codes go exactly:
+// a byte b = code + 128 becomes the half 1024 + b by a byte permutation, and 1152 is taken off.  The order of the dims inside a
+// product is free as long as both operands share it: a lane takes the 16 dims of one 16-byte chunk.  (tcgen05 would need the operands
+// in shared or tensor memory, behind a barrier for every tile; 16 rows leave 7/8 of its 128 idle.)
+//
+// Rounding: products of halves are exact and summed in fp32; the softmax is fp32; the weights are rounded to halves for the second product
+// (times 2^15, so that they are normal numbers down to 2^-29 of the largest), their sum is taken before that.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "tq_common.cuh"
+#include "tq_paged.cuh"
+
+namespace tq {
+
+namespace {
+
+constexpr int kRowTile = 16;          // query rows of an item
+constexpr int kTileTokens = 64;       // tokens of a unit
+constexpr int kMulWarps = 4;
+constexpr int kAttnThreads = 32 * (kMulWarps + 1);
+constexpr int kAttnStages = 4;
+constexpr int kAttnCtas = 2;          // to an SM
+constexpr float kWeightOffset = 15.f; // weights are held times 2^15
+constexpr unsigned long long kPagedWaitLimitNs = 200ull * 1000 * 1000;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ unsigned long long timer_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Bounded wait; gives up at once when another thread has.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile unsigned int* abort_flag) {
+    unsigned long long t0 = 0;
+    for (uint32_t spin = 0;; ++spin) {
+        uint32_t done;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+        if ((spin & 15) == 15 && *abort_flag) return false;
+        if (spin == 64) t0 = timer_ns();
+        if (spin > 64 && (spin & 63) == 0 && timer_ns() - t0 > kPagedWaitLimitNs) return false;
+    }
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two of the bytes of w (`which`: their places, with the 0x64 of a half behind each) as halves of code.
+__device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t which) {
+    const uint32_t raw = __byte_perm(w, 0x64646464u, which);
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), off);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A request's part of the work, in units: its tiles times its row tiles (times the KV heads).
+struct RequestWork {
+    int row, start, count, held, lo, hi;   // tiles lo .. hi - 1
+    int row_tiles;
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, int i) {
+        row = a.b.rows[i];
+        start = a.b.starts[i];
+        count = a.b.starts[i + 1] - start;
+        held = a.b.held[i];
+        const int first = held - count;   // position of the first new token
+        lo = a.window > 0 ? max(0, first - a.window + 1) / kTileTokens : 0;
+        hi = (held + kTileTokens - 1) / kTileTokens;
+        row_tiles = start + count <= a.tokens ? (count * a.group + kRowTile - 1) / kRowTile : 0;
+    }
+    __device__ __forceinline__ long long units(int heads) const { return static_cast<long long>(row_tiles) * heads * (hi - lo); }
+};
+
+// A CTA's share [u, end) of the units and where it stands in them: (request, KV head, row tile, tile), the tile running fastest.
+struct Walker {
+    RequestWork w;
+    int i, n, head, row_tile, tile;
+    long long left;      // units of the share that are still to do, this item's included
+    __device__ __forceinline__ void place(const PagedAttnArgs& a, int request, long long skip, long long units) {
+        i = request;
+        left = units;
+        w.load(a, i);
+        while (skip >= w.units(a.heads)) {   // (the share begins inside a request that has units)
+            skip -= w.units(a.heads);
+            w.load(a, ++i);
+        }
+        const int tiles = w.hi - w.lo;
+        tile = w.lo + static_cast<int>(skip % tiles);
+        skip /= tiles;
+        row_tile = static_cast<int>(skip % w.row_tiles);
+        head = static_cast<int>(skip / w.row_tiles);
+    }
+    // Tiles of the present item that belong to the share.
+    __device__ __forceinline__ int run() const { return static_cast<int>(min(static_cast<long long>(w.hi - tile), left)); }
+    // Behind that run; false at the share's end.
+    __device__ __forceinline__ bool next(const PagedAttnArgs& a) {
+        left -= run();
+        if (left <= 0) return false;
+        if (++row_tile == w.row_tiles) {
+            row_tile = 0;
+            if (++head == a.heads) {
+                head = 0;
+                do w.load(a, ++i);
+                while (w.units(a.heads) == 0);
+            }
+        }
+        tile = w.lo;
+        return true;
+    }
+};
+
+template <int D>
+struct AttnShape {
+    static constexpr int kTileBytes = kTileTokens * D;
+    static constexpr int kScales = 4;   // pages in a tile at most
+    static constexpr int kStageBytes = 2 * kTileBytes + 16 * kScales;
+    static constexpr int kRowFloats = D + 4;
+    static constexpr int kMergeBytes = kMulWarps * kRowTile * kRowFloats * 4;
+    static constexpr int kSmem = kAttnStages * kStageBytes + kMergeBytes;
+    static constexpr int kPart = kRowTile * (D + 2);   // floats of a part: rows, then (maximum, sum) of each
+};
+
+template <int D>
+__global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+    using S = AttnShape<D>;
+    extern __shared__ __align__(128) uint8_t s_mem[];
+    __shared__ __align__(8) unsigned long long s_full[kAttnStages], s_empty[kAttnStages];
+    __shared__ long long s_sum[kAttnThreads + 1];
+    __shared__ float s_ml[kMulWarps][kRowTile][2], s_vref[kMulWarps];
+    __shared__ unsigned int s_abort;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int s = 0; s < kAttnStages; ++s) {
+            bar_init(smem_addr(&s_full[s]), 1);
+            bar_init(smem_addr(&s_empty[s]), kMulWarps);
+        }
+        s_abort = 0;
+        s_sum[0] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait_release();
+    const int n = min(a.n, a.b.header->requests);
+
+    // units in front of each thread's requests
+    const int per = (n + kAttnThreads - 1) / kAttnThreads;
+    {
+        long long mine = 0;
+        for (int i = tid * per; i < min(n, (tid + 1) * per); ++i) {
+            RequestWork w;
+            w.load(a, i);
+            mine += w.units(a.heads);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, mine, o);
+            if (lane >= o) mine += t;
+        }
+        s_sum[tid + 1] = mine;
+    }
+    __syncthreads();
+    long long total = 0, before[kMulWarps + 1];
+#pragma unroll
+    for (int k = 0; k < kMulWarps + 1; ++k) {
+        before[k] = total;
+        total += s_sum[32 * (k + 1)];
+    }
+    const long long ctas = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
+    if (tid == 0) a.joins[c].last = 0;
+    if (c >= ctas) return;
+    const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
+    Walker at;
+    {
+        // the thread's range of requests in which the share begins: the last whose sum in front is at most u0
+        int lo = 0, hi = kAttnThreads;
+        auto front = [&](int t) {
+            long long b = 0;
+#pragma unroll
+            for (int k = 0; k < kMulWarps + 1; ++k)
+                if (k == t >> 5) b = before[k];
+            return (t & 31) == 0 ? b : b + s_sum[t];
+        };
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (front(mid) <= u0) lo = mid;
+            else hi = mid;
+        }
+        at.place(a, lo * per, u0 - front(lo), u1 - u0);
+    }
+
+    if (warp == kMulWarps) {
+        // ---- copies ----
+        const int P = a.b.page_tokens, span = min(P, kTileTokens);   // tokens of a page in a tile
+        const size_t block = paged_block_bytes(P, D);
+        int known_row = -1, known_first = -1, known = 0;   // 32 entries of a row of the tables, one per lane
+        uint32_t s = 0, phase = 0;
+        bool ok = true, more = true;
+        int issued = 0;
+        while (ok && more) {
+            const int tiles = at.run();
+            for (int t = at.tile; ok && t < at.tile + tiles; ++t) {
+                const int token = t * kTileTokens, here = min(kTileTokens, at.w.held - token), pages = (here + span - 1) / span;
+                const int first = token / P;
+                if (at.w.row != known_row || (first & ~31) != known_first) {
+                    known_row = at.w.row;
+                    known_first = first & ~31;
+                    known = known_first + lane < a.b.max_pages ? a.b.tables[static_cast<size_t>(known_row) * a.b.max_pages + known_first + lane] : 0;
+                }
+                ok = bar_wait(smem_addr(&s_empty[s]), phase ^ 1, &s_abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t full = smem_addr(&s_full[s]);
+                if (lane == 0) bar_expect(full, static_cast<uint32_t>(here * D * 2 + pages * 16));
+                __syncwarp();
+                // lanes 0 .. 3: keys of the pages, 4 .. 7: values, 8 .. 11: scales
+                const int j = lane & 3, part = lane >> 2;
+                const int page = __shfl_sync(0xffffffffu, known, (first + j) & 31);
+                if (part < 3 && j < pages) {
+                    const uint32_t bytes = static_cast<uint32_t>(min(span, here - j * span)) * D;
+                    const uint8_t* const src = a.layer + (static_cast<size_t>(page) * a.heads + at.head) * block;
+                    const uint32_t stage = smem_addr(s_mem) + s * S::kStageBytes;
+                    const size_t in_page = static_cast<size_t>(P > kTileTokens ? token % P : 0) * D;
+                    if (part == 0) bulk_copy(stage + j * span * D, src + in_page, bytes, full);
+                    else if (part == 1) bulk_copy(stage + S::kTileBytes + j * span * D, src + static_cast<size_t>(P) * D + in_page, bytes, full);
+                    else bulk_copy(stage + 2 * S::kTileBytes + 16 * j, src + 2 * static_cast<size_t>(P) * D, 16, full);
+                }
+                issued = min(issued + 1, kAttnStages);
+                if (++s == kAttnStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+            more = ok && at.next(a);
+        }
+        if (!ok) {
+            if (lane == 0) {
+                s_abort = 1;
+                raise_status(a.status, kPagedWait);
+            }
+            // copies on their way land before the CTA's memory is another's (the flag does not cut this short)
+            unsigned int never = 0;
+            for (int k = 0; k < issued; ++k) {
+                if (s == 0) phase ^= 1;
+                s = s == 0 ? kAttnStages - 1 : s - 1;
+                bar_wait(smem_addr(&s_full[s]), phase, &never);
+            }
+        }
+        return;
+    }
+
+    // ---- products ----
+    const int g = lane >> 2, qd = lane & 3;
+    const int P = a.b.page_tokens, span_shift = P >= kTileTokens ? 6 : P == 32 ? 5 : 4;
+    const bool q_wide = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stride * 2)) & 7) == 0;
+    const bool out_wide = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * 2)) & 15) == 0;
+    uint32_t s = 0, phase = 0;
+    bool more = true, alive = true;
+    while (more) {
+        const int rows = at.w.count * a.group, row0 = at.row_tile * kRowTile;
+        const int live_rows = min(kRowTile, rows - row0);
+        const int first_pos = at.w.held - at.w.count;
+        // queries: lane (g, qd) holds rows g and g + 8, of each 16-byte chunk c = qd + 4 j of dims the products 4 j .. 4 j + 3
+        uint32_t qf[D / 16][4];
+        int pos[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = row0 + min(g + 8 * r, live_rows - 1), token = row / a.group, hq = at.head * a.group + row - token * a.group;
+            const bool live = g + 8 * r < live_rows;
+            pos[r] = first_pos + token;
+            const __half* const src = a.q + (at.w.start + token) * a.q_stride + static_cast<long>(hq) * D + 16 * qd;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint2 v = make_uint2(0u, 0u);
+                    const __half* const p = src + 64 * j + 4 * k;
+                    if (live) {
+                        if (q_wide) v = *reinterpret_cast<const uint2*>(p);
+                        else {
+                            const __half2 x = __halves2half2(p[0], p[1]), y = __halves2half2(p[2], p[3]);
+                            v = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+                        }
+                    }
+                    qf[4 * j + k][r] = v.x;
+                    qf[4 * j + k][2 + r] = v.y;
+                }
+        }
+        const int pos_min = first_pos + row0 / a.group, pos_max = first_pos + (row0 + live_rows - 1) / a.group;
+
+        float o[D / 8][4];
+#pragma unroll
+        for (int u = 0; u < D / 8; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[u][k] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
+
+        const int tiles = at.run();
+        const bool begins = at.tile == at.w.lo, ends = at.tile + tiles == at.w.hi;
+        for (int t = at.tile; t < at.tile + tiles; ++t) {
+            alive = alive && __all_sync(0xffffffffu, bar_wait(smem_addr(&s_full[s]), phase, &s_abort));
+            if (!alive) {   // (it still goes through the barriers with the others)
+                if (lane == 0) {
+                    s_abort = 1;
+                    raise_status(a.status, kPagedWait);
+                }
+                break;
+            }
+            const uint8_t* const stage = s_mem + s * S::kStageBytes;
+            const int w0 = t * kTileTokens + 16 * warp;   // this warp's first token
+            if (w0 <= pos_max && (a.window <= 0 || w0 + 15 > pos_min - a.window)) {
+                float2 scales = *reinterpret_cast<const float2*>(stage + 2 * S::kTileBytes + 16 * ((16 * warp) >> span_shift));
+                if (!(scales.y < INFINITY)) scales = make_float2(__uint_as_float(0x7fc00000u), 0.f);   // values that are not numbers: the rows that see them
+                // scores: columns 2 qd, 2 qd + 1 of the tokens 0 .. 7 and 8 .. 15
+                float sc[2][4] = {};
+                const uint8_t* const keys = stage + 16 * warp * D;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        const int token = 8 * nt + g;
+                        const uint4 raw = *reinterpret_cast<const uint4*>(keys + token * D + 16 * key_chunk<D>(token, qd + 4 * j));
+                        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma_f16(sc[nt], qf[4 * j + k], code_halves(w[k], 0x4140), code_halves(w[k], 0x4342));
+                    }
+                const float f = scales.x * a.scale_log2;
+                const bool masks = w0 + 15 > pos_min || (a.window > 0 && w0 <= pos_max - a.window);
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float x = sc[nt][k] * f;
+                        if (masks) {
+                            const int token = w0 + 8 * nt + 2 * qd + (k & 1), p = pos[k >> 1];
+                            if (token > p || (a.window > 0 && token <= p - a.window)) x = -INFINITY;
+                        }
+                        sc[nt][k] = x;
+                        top[k >> 1] = fmaxf(top[k >> 1], x);
+                    }
+                bool moved = false;
+                float shift[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                    shift[r] = fmaxf(m[r], top[r]);
+                    moved = moved || shift[r] > m[r];
+                }
+                const float vnew = fmaxf(vref, scales.y);
+                if (__any_sync(0xffffffffu, moved || vnew > vref)) {
+                    const float vs = vnew > 0.f ? vref / vnew : 0.f;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float x = shift[r] > m[r] ? exp2_approx(m[r] - shift[r]) : 1.f;
+                        l[r] *= x;
+#pragma unroll
+                        for (int u = 0; u < D / 8; ++u) {
+                            o[u][2 * r] *= x * vs;
+                            o[u][2 * r + 1] *= x * vs;
+                        }
+                        m[r] = shift[r];
+                    }
+                    vref = vnew;
+                }
+                const float ratio = scales.y / fmaxf(vref, 1e-37f);
+                uint32_t pf[4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kWeightOffset;
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const float p0 = exp2_approx(sc[nt][2 * r] - base), p1 = exp2_approx(sc[nt][2 * r + 1] - base);
+                        l[r] += p0 + p1;
+                        pf[2 * nt + r] = pack_half2(p0 * ratio, p1 * ratio);
+                    }
+                }
+                // values: lane (g, qd) takes the chunk of dims of column g, of the tokens 2 qd, 2 qd + 1 and those 8 further on
+                const uint8_t* const values = stage + S::kTileBytes + 16 * warp * D;
+                constexpr int kWords = D / 32;   // 4 dims each of a lane's D / 8
+                uint32_t v[4][kWords];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int token = 2 * qd + (k & 1) + 8 * (k >> 1);
+                    if constexpr (D == 128) {
+                        const uint4 raw = *reinterpret_cast<const uint4*>(values + token * D + 16 * value_chunk<D>(token, g));
+                        v[k][0] = raw.x; v[k][1] = raw.y; v[k][2] = raw.z; v[k][3] = raw.w;
+                    } else {
+                        const uint2 raw = *reinterpret_cast<const uint2*>(values + token * D + 16 * value_chunk<D>(token, g >> 1) + 8 * (g & 1));
+                        v[k][0] = raw.x; v[k][1] = raw.y;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    uint32_t pair[4];   // bytes of two tokens side by side: dims 0, 1 and 2, 3 of the first two tokens, then of the others
+                    pair[0] = __byte_perm(v[0][w], v[1][w], 0x5140);
+                    pair[1] = __byte_perm(v[0][w], v[1][w], 0x7362);
+                    pair[2] = __byte_perm(v[2][w], v[3][w], 0x5140);
+                    pair[3] = __byte_perm(v[2][w], v[3][w], 0x7362);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const uint32_t which = (d & 1) ? 0x4342 : 0x4140;
+                        mma_f16(o[4 * w + d], pf, code_halves(pair[d >> 1], which), code_halves(pair[2 + (d >> 1)], which));
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_addr(&s_empty[s]));
+            if (++s == kAttnStages) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+
+        // ---- the four warps' sums together ----
+        float* const s_o = reinterpret_cast<float*>(s_mem + kAttnStages * S::kStageBytes);
+        constexpr int kDims = D / 8;   // dims of a lane's column
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            float* const to = s_o + (warp * kRowTile + g + 8 * r) * S::kRowFloats;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int u = 0; u < kDims; u += 4)
+                    *reinterpret_cast<float4*>(to + (2 * qd + e) * kDims + u) = make_float4(o[u][2 * r + e], o[u + 1][2 * r + e], o[u + 2][2 * r + e], o[u + 3][2 * r + e]);
+            if (qd == 0) {
+                s_ml[warp][g + 8 * r][0] = m[r];
+                s_ml[warp][g + 8 * r][1] = l[r];
+            }
+        }
+        if (lane == 0) s_vref[warp] = vref;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kMulWarps) : "memory");
+        {
+            constexpr int kEach = kRowTile * D / (32 * kMulWarps);   // dims of a thread
+            const int r = tid / (D / kEach), d0 = tid % (D / kEach) * kEach;
+            float top = -INFINITY, sum = 0.f, acc[kEach];
+#pragma unroll
+            for (int w = 0; w < kMulWarps; ++w) top = fmaxf(top, s_ml[w][r][0]);
+#pragma unroll
+            for (int d = 0; d < kEach; ++d) acc[d] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kMulWarps; ++w) {
+                // (a warp that saw nothing has zeros; one that met a NaN has no maximum, and its sum says so)
+                const float mw = s_ml[w][r][0], x = mw == top || mw == -INFINITY ? 1.f : exp2_approx(mw - top), y = x * s_vref[w];
+                sum = fmaf(s_ml[w][r][1], x, sum);
+                const float* const from = s_o + (w * kRowTile + r) * S::kRowFloats + d0;
+#pragma unroll
+                for (int d = 0; d < kEach; d += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(from + d);
+                    acc[d] = fmaf(v.x, y, acc[d]);
+                    acc[d + 1] = fmaf(v.y, y, acc[d + 1]);
+                    acc[d + 2] = fmaf(v.z, y, acc[d + 2]);
+                    acc[d + 3] = fmaf(v.w, y, acc[d + 3]);
+                }
+            }
+            if (begins && ends) {
+                if (r < live_rows) {
+                    const int row = row0 + r, token = row / a.group, hq = at.head * a.group + row - token * a.group;
+                    __half* const to = a.out + (at.w.start + token) * a.out_stride + static_cast<long>(hq) * D + d0;
+                    const float inv = 1.f / sum;
+#pragma unroll
+                    for (int d = 0; d < kEach; ++d) acc[d] *= inv;
+                    if (out_wide) {
+#pragma unroll
+                        for (int d = 0; d < kEach; d += 8) {
+                            const float v[8] = {acc[d], acc[d + 1], acc[d + 2], acc[d + 3], acc[d + 4], acc[d + 5], acc[d + 6], acc[d + 7]};
+                            *reinterpret_cast<uint4*>(to + d) = pack_halves(v);
+                        }
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < kEach; ++d) to[d] = __float2half_rn(acc[d]);
+                    }
+                    if (a.lse && d0 == 0)
+                        a.lse[(at.w.start + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kWeightOffset + log2f(sum)) * 0.6931471805599453f;
+                }
+            } else {
+                float* const part = a.partial + (2 * c + (begins ? 1 : 0)) * static_cast<long>(S::kPart);
+#pragma unroll
+                for (int d = 0; d < kEach; d += 4) *reinterpret_cast<float4*>(part + r * D + d0 + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+                if (d0 == 0) *reinterpret_cast<float2*>(part + kRowTile * D + 2 * r) = make_float2(top, sum);
+                if (begins && tid == 0) {
+                    // the CTA that holds the item's last unit: the largest c' with total * c' / ctas <= that unit
+                    const long long last_unit = u1 - at.left + (at.w.hi - at.tile) - 1;
+                    a.joins[c] = {static_cast<int>(((last_unit + 1) * ctas - 1) / total), at.w.start, row0, live_rows, at.head};
+                }
+            }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kMulWarps) : "memory");
+        more = at.next(a);
+    }
+}
+
+// Parts of an item that several CTAs share, in the CTAs' order, a CTA per row: its four warps take a quarter of the parts each.
+template <int D>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int kPart = AttnShape<D>::kPart, kEach = D / 32;
+    __shared__ float s_acc[4][D], s_sum[4];
+    pdl_wait_release();
+    const PagedJoin join = a.joins[blockIdx.x];
+    const int r = blockIdx.y, c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (join.last == 0 || r >= join.rows) return;
+    const int parts = join.last - c + 1;
+    auto part_of = [&](int k) { return a.partial + (2 * (c + k) + (k == 0 ? 1 : 0)) * static_cast<long>(kPart); };
+    float top = -INFINITY;
+    for (int k = lane; k < parts; k += 32) top = fmaxf(top, part_of(k)[kRowTile * D + 2 * r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int k0 = parts * warp / 4, k1 = parts * (warp + 1) / 4;
+    float acc[kEach] = {}, sum = 0.f;
+    for (int base = k0; base < k1; base += 8) {
+        float2 ml[8];
+        float v[8][kEach];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float* const p = part_of(min(base + k, k1 - 1));
+            ml[k] = *reinterpret_cast<const float2*>(p + kRowTile * D + 2 * r);
+#pragma unroll
+            for (int d = 0; d < kEach; ++d) v[k][d] = p[r * D + 32 * d + lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (base + k >= k1) continue;
+            const float x = ml[k].x == top || ml[k].x == -INFINITY ? 1.f : exp2_approx(ml[k].x - top);
+            sum = fmaf(ml[k].y, x, sum);
+#pragma unroll
+            for (int d = 0; d < kEach; ++d) acc[d] = fmaf(v[k][d], x, acc[d]);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < kEach; ++d) s_acc[warp][32 * d + lane] = acc[d];
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    const float all = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], inv = 1.f / all;
+    const int row = join.first_row + r, token = row / a.group, hq = join.head * a.group + row - token * a.group;
+    for (int d = threadIdx.x; d < D; d += 128)
+        a.out[(join.token + token) * a.out_stride + static_cast<long>(hq) * D + d] = __float2half_rn((s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d]) * inv);
+    if (a.lse && threadIdx.x == 0)
+        a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kWeightOffset + log2f(all)) * 0.6931471805599453f;
+}
+
+template <int D>
+void launch_typed(PagedAttnArgs a, int max_count, void* scratch, int sms, cudaStream_t st) {
+    const int ctas = sms * kAttnCtas;
+    a.joins = static_cast<PagedJoin*>(scratch);
+    a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
+    TQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnShape<D>::kSmem));
+    launch_pdl(paged_attn_kernel<D>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), AttnShape<D>::kSmem, st, a);
+    const long rows = std::min<long>(kRowTile, static_cast<long>(max_count) * a.group);
+    launch_pdl(paged_join_kernel<D>, dim3(static_cast<unsigned int>(ctas), static_cast<unsigned int>(rows)), dim3(128), 0, st, a);
+}
+
+}  // namespace
+
+size_t paged_attn_scratch_bytes(int dim, int sms) {
+    const size_t ctas = static_cast<size_t>(sms) * kAttnCtas;
+    return (ctas * sizeof(PagedJoin) + 255) / 256 * 256 + ctas * 2 * kRowTile * (static_cast<size_t>(dim) + 2) * sizeof(float);
+}
+void launch_paged_attention(const PagedAttnArgs& a, int dim, int max_count, void* scratch, int sms, cudaStream_t st) {
+    if (dim == 64) launch_typed<64>(a, max_count, scratch, sms, st);
+    else launch_typed<128>(a, max_count, scratch, sms, st);
+}
+
+}  // namespace tq
