@@ -66,7 +66,8 @@ public:
         TQ_CUDA(cudaMemcpy(b_.stack, stack.data(), 4ul * pages, cudaMemcpyHostToDevice));
         TQ_CUDA(cudaMemcpy(&b_.header->free_pages, &pages, 4, cudaMemcpyHostToDevice));
         scratch_.owned_by(&use_);
-        scratch_.resize(tq::paged_attn_scratch_bytes(dim, sms_));
+        prompt_scratch_ = (tq::paged_attn_scratch_bytes(dim, sms_) + 255) / 256 * 256;   // (behind the other kernel's)
+        scratch_.resize(prompt_scratch_ + tq::paged_prompt_scratch_bytes(dim, sms_));
         TQ_CUDA(cudaDeviceSynchronize());   // the first call may come on any stream
         h_status_ = tq::status_word_take(device_);
         d_status_ = static_cast<unsigned int*>(tq::pinned_host_device_alias(h_status_));
@@ -173,9 +174,15 @@ public:
         a.heads = heads_;
         a.group = q_heads / heads_;
         a.window = window;
+        a.page_shift = b_.page_tokens == 16 ? 4 : b_.page_tokens == 32 ? 5 : b_.page_tokens == 64 ? 6 : 7;
         a.scale_log2 = static_cast<float>((scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(dim_))) * 1.4426950408889634);
         a.status = d_status_;
-        tq::launch_paged_attention(a, dim_, max_count_, scratch_.as<void>(), sms_, st);
+        // The device finds the requests of each kernel; a batch of one has one.
+        const long max_rows = static_cast<long>(max_count_) * a.group;
+        const bool many = max_rows > kFewRows;
+        a.few_rows = many && n_ == 1 ? 0 : kFewRows;
+        if (many) tq::launch_paged_prompt(a, dim_, scratch_.as<char>() + prompt_scratch_, sms_, st);
+        if (a.few_rows) tq::launch_paged_attention(a, dim_, static_cast<int>(std::min<long>(max_rows, kFewRows)), scratch_.as<void>(), sms_, st);
     }
     void check_status() {
         const unsigned int code = *static_cast<volatile unsigned int*>(h_status_);
@@ -197,6 +204,9 @@ public:
     }
 
 private:
+    // Query rows of a request (new tokens times query heads to a KV head) that the kernel for few rows takes.
+    static constexpr int kFewRows = 16;
+
     void check_layer(int layer) const { TQ_REQUIRE(layer >= 0 && layer < static_cast<int>(layers_.size()), "Layer index out of range"); }
     void begin(cudaStream_t st) {
         tq::ensure_device(device_);
@@ -212,6 +222,7 @@ private:
 
     int heads_, dim_, max_tokens_, device_ = 0, sms_ = 0;
     int n_ = -1, tokens_ = 0, max_count_ = 0;   // of the plan in force (n_ < 0: none)
+    size_t prompt_scratch_ = 0;
     tq::StreamUse use_;
     std::vector<DeviceBuffer> layers_;
     DeviceBuffer state_, scratch_;

@@ -130,13 +130,77 @@ struct PagedAttnArgs {
     __half* out;
     float* lse;          // or null
     long q_stride, out_stride;
-    int n, tokens, heads, group, window;
+    int n, tokens, heads, group, window, page_shift;
+    int few_rows;        // requests of more query rows (new tokens times the group) go through tq_paged_prompt.cu
     float scale_log2;    // softmax scale times log2(e)
     float* partial;
     PagedJoin* joins;
     unsigned int* status;
 };
 size_t paged_attn_scratch_bytes(int dim, int sms);
-void launch_paged_attention(const PagedAttnArgs& a, int dim, int max_count, void* scratch, int sms, cudaStream_t st);
+// The requests of at most a.few_rows rows.
+void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratch, int sms, cudaStream_t st);
+// The others (tq_paged_prompt.cu).
+size_t paged_prompt_scratch_bytes(int dim, int sms);
+void launch_paged_prompt(PagedAttnArgs a, int dim, void* scratch, int sms, cudaStream_t st);
+
+// ---- what the attention kernels share -------------------------------------------------------------
+namespace paged_device {
+
+constexpr uint32_t kPagedWaitLimit = 400u * 1000 * 1000;   // cycles: 0.2 s at 2 GHz
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Bounded wait; gives up when another thread has.  (Few instructions: there is one behind every step of the kernels.  The limit is in clock cycles: reading
+// the global timer takes longer than most waits, and a waiting warp does not see its barrier meanwhile.)
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile unsigned int* abort_flag) {
+    uint32_t begin = 0;
+    for (uint32_t spin = 0;; ++spin) {
+        uint32_t done;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+        if ((spin & 255) == 255) {
+            uint32_t now;
+            asm volatile("mov.u32 %0, %%clock;" : "=r"(now));
+            if (spin == 255) begin = now;
+            if (*abort_flag || now - begin > kPagedWaitLimit) return false;
+        }
+    }
+}
+// Eight halves at any even address, out of the way of the code that runs all the time.
+__device__ __noinline__ inline void store_halves_anywhere(__half* p, uint4 v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        p[2 * k] = __ushort_as_half(static_cast<unsigned short>(w[k]));
+        p[2 * k + 1] = __ushort_as_half(static_cast<unsigned short>(w[k] >> 16));
+    }
+}
+__device__ __noinline__ inline uint4 load_halves_anywhere(const __half* p) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __half_as_ushort(p[2 * k]) | static_cast<uint32_t>(__half_as_ushort(p[2 * k + 1])) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+}  // namespace paged_device
 
 }  // namespace tq

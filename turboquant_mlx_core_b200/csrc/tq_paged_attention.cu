@@ -1,4 +1,5 @@
-// Attention over the paged 8-bit KV cache: the new tokens' queries against all tokens of their request up to their own.
+// Attention over the paged 8-bit KV cache: the new tokens' queries against all tokens of their request up to their own; here
+// requests of few query rows (tq_paged_prompt.cu: many).
 //
 //   s = q . k scale,  o = sum softmax(s) v          q [tokens, heads * group, D] fp16, k and v code * 2^e of a page and head
 //
@@ -26,6 +27,8 @@ namespace tq {
 
 namespace {
 
+using namespace paged_device;
+
 constexpr int kRowTile = 16;          // query rows of an item
 constexpr int kTileTokens = 64;       // tokens of a unit
 constexpr int kMulWarps = 4;
@@ -33,36 +36,7 @@ constexpr int kAttnThreads = 32 * (kMulWarps + 1);
 constexpr int kAttnStages = 4;
 constexpr int kAttnCtas = 2;          // to an SM
 constexpr float kWeightOffset = 15.f; // weights are held times 2^15
-constexpr unsigned long long kPagedWaitLimitNs = 200ull * 1000 * 1000;
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ unsigned long long timer_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// Bounded wait; gives up at once when another thread has.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile unsigned int* abort_flag) {
-    unsigned long long t0 = 0;
-    for (uint32_t spin = 0;; ++spin) {
-        uint32_t done;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
-        if ((spin & 15) == 15 && *abort_flag) return false;
-        if (spin == 64) t0 = timer_ns();
-        if (spin > 64 && (spin & 63) == 0 && timer_ns() - t0 > kPagedWaitLimitNs) return false;
-    }
-}
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
@@ -78,16 +52,6 @@ __device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t which) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), off);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // A request's part of the work, in units: its tiles times its row tiles (times the KV heads).
 struct RequestWork {
     int row, start, count, held, lo, hi;   // tiles lo .. hi - 1
@@ -100,7 +64,7 @@ struct RequestWork {
         const int first = held - count;   // position of the first new token
         lo = a.window > 0 ? max(0, first - a.window + 1) / kTileTokens : 0;
         hi = (held + kTileTokens - 1) / kTileTokens;
-        row_tiles = start + count <= a.tokens ? (count * a.group + kRowTile - 1) / kRowTile : 0;
+        row_tiles = start + count <= a.tokens && count * a.group <= a.few_rows ? (count * a.group + kRowTile - 1) / kRowTile : 0;
     }
     __device__ __forceinline__ long long units(int heads) const { return static_cast<long long>(row_tiles) * heads * (hi - lo); }
 };
@@ -574,13 +538,13 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 }
 
 template <int D>
-void launch_typed(PagedAttnArgs a, int max_count, void* scratch, int sms, cudaStream_t st) {
+void launch_typed(PagedAttnArgs a, int max_rows, void* scratch, int sms, cudaStream_t st) {
     const int ctas = sms * kAttnCtas;
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
     TQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnShape<D>::kSmem));
     launch_pdl(paged_attn_kernel<D>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), AttnShape<D>::kSmem, st, a);
-    const long rows = std::min<long>(kRowTile, static_cast<long>(max_count) * a.group);
+    const int rows = std::min(kRowTile, max_rows);
     launch_pdl(paged_join_kernel<D>, dim3(static_cast<unsigned int>(ctas), static_cast<unsigned int>(rows)), dim3(128), 0, st, a);
 }
 
@@ -590,9 +554,9 @@ size_t paged_attn_scratch_bytes(int dim, int sms) {
     const size_t ctas = static_cast<size_t>(sms) * kAttnCtas;
     return (ctas * sizeof(PagedJoin) + 255) / 256 * 256 + ctas * 2 * kRowTile * (static_cast<size_t>(dim) + 2) * sizeof(float);
 }
-void launch_paged_attention(const PagedAttnArgs& a, int dim, int max_count, void* scratch, int sms, cudaStream_t st) {
-    if (dim == 64) launch_typed<64>(a, max_count, scratch, sms, st);
-    else launch_typed<128>(a, max_count, scratch, sms, st);
+void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratch, int sms, cudaStream_t st) {
+    if (dim == 64) launch_typed<64>(a, max_rows, scratch, sms, st);
+    else launch_typed<128>(a, max_rows, scratch, sms, st);
 }
 
 }  // namespace tq
