@@ -29,13 +29,12 @@ namespace {
 
 using namespace paged_device;
 
-constexpr int kRowTile = 16;          // query rows of an item
 constexpr int kTileTokens = 64;       // tokens of a unit
 constexpr int kMulWarps = 4;
 constexpr int kAttnThreads = 32 * (kMulWarps + 1);
-constexpr int kAttnStages = 4;
-constexpr int kAttnCtas = 2;          // to an SM
-constexpr float kWeightOffset = 15.f; // weights are held times 2^15
+// The reference maximum of a row moves only when a score exceeds it by 2^kSlack: a vote instead of a reduction for most tiles.  Weights are held times 2^kOffset and at most
+// 2^15: halves that are normal numbers down to 2^-25 of the reference.
+constexpr float kOffset = 11.f, kSlack = 4.f;
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -44,6 +43,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The 8 x 8 halves that a warp holds, two to a lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 // Two of the bytes of w (`which`: their places, with the 0x64 of a half behind each) as halves of code.
 __device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t which) {
@@ -56,7 +61,7 @@ __device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t which) {
 struct RequestWork {
     int row, start, count, held, lo, hi;   // tiles lo .. hi - 1
     int row_tiles;
-    __device__ __forceinline__ void load(const PagedAttnArgs& a, int i) {
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, int i, int tile_rows) {
         row = a.b.rows[i];
         start = a.b.starts[i];
         count = a.b.starts[i + 1] - start;
@@ -64,12 +69,13 @@ struct RequestWork {
         const int first = held - count;   // position of the first new token
         lo = a.window > 0 ? max(0, first - a.window + 1) / kTileTokens : 0;
         hi = (held + kTileTokens - 1) / kTileTokens;
-        row_tiles = start + count <= a.tokens && count * a.group <= a.few_rows ? (count * a.group + kRowTile - 1) / kRowTile : 0;
+        row_tiles = start + count <= a.tokens && count * a.group <= a.few_rows ? (count * a.group + tile_rows - 1) / tile_rows : 0;
     }
     __device__ __forceinline__ long long units(int heads) const { return static_cast<long long>(row_tiles) * heads * (hi - lo); }
 };
 
 // A CTA's share [u, end) of the units and where it stands in them: (request, KV head, row tile, tile), the tile running fastest.
+template <int ROWS>
 struct Walker {
     RequestWork w;
     int i, n, head, row_tile, tile;
@@ -77,10 +83,10 @@ struct Walker {
     __device__ __forceinline__ void place(const PagedAttnArgs& a, int request, long long skip, long long units) {
         i = request;
         left = units;
-        w.load(a, i);
+        w.load(a, i, ROWS);
         while (skip >= w.units(a.heads)) {   // (the share begins inside a request that has units)
             skip -= w.units(a.heads);
-            w.load(a, ++i);
+            w.load(a, ++i, ROWS);
         }
         const int tiles = w.hi - w.lo;
         tile = w.lo + static_cast<int>(skip % tiles);
@@ -98,7 +104,7 @@ struct Walker {
             row_tile = 0;
             if (++head == a.heads) {
                 head = 0;
-                do w.load(a, ++i);
+                do w.load(a, ++i, ROWS);
                 while (w.units(a.heads) == 0);
             }
         }
@@ -107,28 +113,32 @@ struct Walker {
     }
 };
 
-template <int D>
+// NT: query rows of an item in eights.
+template <int D, int NT>
 struct AttnShape {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kCtas = NT == 1 ? 3 : 2, kStages = NT == 1 ? 3 : 4;   // CTAs to an SM, tiles in a CTA's ring
     static constexpr int kTileBytes = kTileTokens * D;
     static constexpr int kScales = 4;   // pages in a tile at most
     static constexpr int kStageBytes = 2 * kTileBytes + 16 * kScales;
     static constexpr int kRowFloats = D + 4;
-    static constexpr int kMergeBytes = kMulWarps * kRowTile * kRowFloats * 4;
-    static constexpr int kSmem = kAttnStages * kStageBytes + kMergeBytes;
-    static constexpr int kPart = kRowTile * (D + 2);   // floats of a part: rows, then (maximum, sum) of each
+    static constexpr int kMergeBytes = kMulWarps * kRows * kRowFloats * 4;
+    static constexpr int kSmem = kStages * kStageBytes + kMergeBytes;
+    static constexpr int kPart = kRows * (D + 2);   // floats of a part: rows, then (maximum, sum) of each
 };
 
-template <int D>
-__global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
-    using S = AttnShape<D>;
+template <int D, int NT>
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+    using S = AttnShape<D, NT>;
+    constexpr int kRows = S::kRows, kStages = S::kStages;
     extern __shared__ __align__(128) uint8_t s_mem[];
-    __shared__ __align__(8) unsigned long long s_full[kAttnStages], s_empty[kAttnStages];
+    __shared__ __align__(8) unsigned long long s_full[kStages], s_empty[kStages];
     __shared__ long long s_sum[kAttnThreads + 1];
-    __shared__ float s_ml[kMulWarps][kRowTile][2], s_vref[kMulWarps];
+    __shared__ float s_ml[kMulWarps][kRows][2], s_vref[kMulWarps];
     __shared__ unsigned int s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int s = 0; s < kAttnStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             bar_init(smem_addr(&s_full[s]), 1);
             bar_init(smem_addr(&s_empty[s]), kMulWarps);
         }
@@ -145,7 +155,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
         long long mine = 0;
         for (int i = tid * per; i < min(n, (tid + 1) * per); ++i) {
             RequestWork w;
-            w.load(a, i);
+            w.load(a, i, kRows);
             mine += w.units(a.heads);
         }
 #pragma unroll
@@ -166,7 +176,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
     if (tid == 0) a.joins[c].last = 0;
     if (c >= ctas) return;
     const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
-    Walker at;
+    Walker<kRows> at;
     {
         // the thread's range of requests in which the share begins: the last whose sum in front is at most u0
         int lo = 0, hi = kAttnThreads;
@@ -221,8 +231,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
                     else if (part == 1) bulk_copy(stage + S::kTileBytes + j * span * D, src + static_cast<size_t>(P) * D + in_page, bytes, full);
                     else bulk_copy(stage + 2 * S::kTileBytes + 16 * j, src + 2 * static_cast<size_t>(P) * D, 16, full);
                 }
-                issued = min(issued + 1, kAttnStages);
-                if (++s == kAttnStages) {
+                issued = min(issued + 1, kStages);
+                if (++s == kStages) {
                     s = 0;
                     phase ^= 1;
                 }
@@ -238,7 +248,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
             unsigned int never = 0;
             for (int k = 0; k < issued; ++k) {
                 if (s == 0) phase ^= 1;
-                s = s == 0 ? kAttnStages - 1 : s - 1;
+                s = s == 0 ? kStages - 1 : s - 1;
                 bar_wait(smem_addr(&s_full[s]), phase, &never);
             }
         }
@@ -253,43 +263,46 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
     uint32_t s = 0, phase = 0;
     bool more = true, alive = true;
     while (more) {
-        const int rows = at.w.count * a.group, row0 = at.row_tile * kRowTile;
-        const int live_rows = min(kRowTile, rows - row0);
+        const int rows = at.w.count * a.group, row0 = at.row_tile * kRows;
+        const int live_rows = min(kRows, rows - row0);
         const int first_pos = at.w.held - at.w.count;
-        // queries: lane (g, qd) holds rows g and g + 8, of each 16-byte chunk c = qd + 4 j of dims the products 4 j .. 4 j + 3
-        uint32_t qf[D / 16][4];
-        int pos[2];
+        // queries, the products' second operand: lane (g, qd) holds row g of each eight, of every 16-byte chunk c = qd + 4 j of codes the products 4 j .. 4 j + 3
+        uint32_t qf[NT][D / 16][2];
+        int pos[NT][2];   // of the scores' rows 2 qd, 2 qd + 1
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = row0 + min(g + 8 * r, live_rows - 1), token = row / a.group, hq = at.head * a.group + row - token * a.group;
-            const bool live = g + 8 * r < live_rows;
-            pos[r] = first_pos + token;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = row0 + min(8 * nt + g, live_rows - 1), token = row / a.group, hq = at.head * a.group + row - token * a.group;
+            // (rows behind the last: the last again, nobody reads their results)
             const __half* const src = a.q + (at.w.start + token) * a.q_stride + static_cast<long>(hq) * D + 16 * qd;
 #pragma unroll
             for (int j = 0; j < D / 64; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    uint2 v = make_uint2(0u, 0u);
+                    uint2 v;
                     const __half* const p = src + 64 * j + 4 * k;
-                    if (live) {
-                        if (q_wide) v = *reinterpret_cast<const uint2*>(p);
-                        else {
-                            const __half2 x = __halves2half2(p[0], p[1]), y = __halves2half2(p[2], p[3]);
-                            v = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-                        }
+                    if (q_wide) v = *reinterpret_cast<const uint2*>(p);
+                    else {
+                        const __half2 x = __halves2half2(p[0], p[1]), y = __halves2half2(p[2], p[3]);
+                        v = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
                     }
-                    qf[4 * j + k][r] = v.x;
-                    qf[4 * j + k][2 + r] = v.y;
+                    qf[nt][4 * j + k][0] = v.x;
+                    qf[nt][4 * j + k][1] = v.y;
                 }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) pos[nt][e] = first_pos + (row0 + min(8 * nt + 2 * qd + e, live_rows - 1)) / a.group;
         }
         const int pos_min = first_pos + row0 / a.group, pos_max = first_pos + (row0 + live_rows - 1) / a.group;
 
-        float o[D / 8][4];
+        float o[NT][D / 16][4], m[NT][2], l[NT][2], vref = 0.f;
 #pragma unroll
-        for (int u = 0; u < D / 8; ++u)
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[u][k] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
+            for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[nt][u][k] = 0.f;
+        }
 
         const int tiles = at.run();
         const bool begins = at.tile == at.w.lo, ends = at.tile + tiles == at.w.hi;
@@ -307,74 +320,85 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
             if (w0 <= pos_max && (a.window <= 0 || w0 + 15 > pos_min - a.window)) {
                 float2 scales = *reinterpret_cast<const float2*>(stage + 2 * S::kTileBytes + 16 * ((16 * warp) >> span_shift));
                 if (!(scales.y < INFINITY)) scales = make_float2(__uint_as_float(0x7fc00000u), 0.f);   // values that are not numbers: the rows that see them
-                // scores: columns 2 qd, 2 qd + 1 of the tokens 0 .. 7 and 8 .. 15
-                float sc[2][4] = {};
+                // scores: tokens g (elements 0, 1) and g + 8 (2, 3), rows 2 qd and 2 qd + 1
+                float sc[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sc[nt][k] = 0.f;
                 const uint8_t* const keys = stage + 16 * warp * D;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int j = 0; j < D / 64; ++j) {
+                    const uint4 near = *reinterpret_cast<const uint4*>(keys + g * D + 16 * key_chunk<D>(g, qd + 4 * j));
+                    const uint4 far = *reinterpret_cast<const uint4*>(keys + (g + 8) * D + 16 * key_chunk<D>(g, qd + 4 * j));
+                    const uint32_t n4[4] = {near.x, near.y, near.z, near.w}, f4[4] = {far.x, far.y, far.z, far.w};
 #pragma unroll
-                    for (int j = 0; j < D / 64; ++j) {
-                        const int token = 8 * nt + g;
-                        const uint4 raw = *reinterpret_cast<const uint4*>(keys + token * D + 16 * key_chunk<D>(token, qd + 4 * j));
-                        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t kf[4] = {code_halves(n4[k], 0x4140), code_halves(f4[k], 0x4140), code_halves(n4[k], 0x4342), code_halves(f4[k], 0x4342)};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) mma_f16(sc[nt], qf[4 * j + k], code_halves(w[k], 0x4140), code_halves(w[k], 0x4342));
+                        for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt], kf, qf[nt][4 * j + k][0], qf[nt][4 * j + k][1]);
                     }
+                }
                 const float f = scales.x * a.scale_log2;
                 const bool masks = w0 + 15 > pos_min || (a.window > 0 && w0 <= pos_max - a.window);
-                float top[2] = {-INFINITY, -INFINITY};
+                bool jump = scales.y > vref;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         float x = sc[nt][k] * f;
                         if (masks) {
-                            const int token = w0 + 8 * nt + 2 * qd + (k & 1), p = pos[k >> 1];
+                            const int token = w0 + g + 8 * (k >> 1), p = pos[nt][k & 1];
                             if (token > p || (a.window > 0 && token <= p - a.window)) x = -INFINITY;
                         }
                         sc[nt][k] = x;
-                        top[k >> 1] = fmaxf(top[k >> 1], x);
+                        jump = jump || x > m[nt][k & 1] + kSlack;
                     }
-                bool moved = false;
-                float shift[2];
+                if (__any_sync(0xffffffffu, jump)) {
+                    const float vnew = fmaxf(vref, scales.y), vs = vnew > 0.f ? vref / vnew : 0.f;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    shift[r] = fmaxf(m[r], top[r]);
-                    moved = moved || shift[r] > m[r];
-                }
-                const float vnew = fmaxf(vref, scales.y);
-                if (__any_sync(0xffffffffu, moved || vnew > vref)) {
-                    const float vs = vnew > 0.f ? vref / vnew : 0.f;
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float x = shift[r] > m[r] ? exp2_approx(m[r] - shift[r]) : 1.f;
-                        l[r] *= x;
+                        for (int e = 0; e < 2; ++e) {
+                            float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
 #pragma unroll
-                        for (int u = 0; u < D / 8; ++u) {
-                            o[u][2 * r] *= x * vs;
-                            o[u][2 * r + 1] *= x * vs;
+                            for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+                            float down = 1.f;
+                            if (top > m[nt][e] + kSlack) {
+                                down = exp2_approx(m[nt][e] - top);   // (0 for the first)
+                                m[nt][e] = top;
+                            }
+                            l[nt][e] *= down;
+                            const float both = down * vs;
+#pragma unroll
+                            for (int u = 0; u < D / 16; ++u) {
+                                o[nt][u][e] *= both;
+                                o[nt][u][2 + e] *= both;
+                            }
                         }
-                        m[r] = shift[r];
-                    }
                     vref = vnew;
                 }
-                const float ratio = scales.y / fmaxf(vref, 1e-37f);
-                uint32_t pf[4];
+                // the values' scale against the largest so far: a power of two, by its bits (0 for those that are not numbers)
+                const int lower = static_cast<int>(__float_as_uint(scales.y)) - static_cast<int>(__float_as_uint(vref)) + 0x3f800000;
+                const float ratio = lower > 0 && scales.y > 0.f ? __int_as_float(lower) : 0.f;
+                uint32_t pf[NT][2];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kWeightOffset;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float p[4];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const float p0 = exp2_approx(sc[nt][2 * r] - base), p1 = exp2_approx(sc[nt][2 * r + 1] - base);
-                        l[r] += p0 + p1;
-                        pf[2 * nt + r] = pack_half2(p0 * ratio, p1 * ratio);
+                    for (int k = 0; k < 4; ++k) {
+                        const float mk = m[nt][k & 1];
+                        p[k] = exp2_approx(sc[nt][k] - ((mk == -INFINITY ? 0.f : mk) - kOffset));
                     }
+                    l[nt][0] += p[0] + p[2];
+                    l[nt][1] += p[1] + p[3];
+                    // (row g, tokens 2 qd, 2 qd + 1 and 8 further on, as the second product wants them)
+                    pf[nt][0] = transposed(pack_half2(p[0] * ratio, p[1] * ratio));
+                    pf[nt][1] = transposed(pack_half2(p[2] * ratio, p[3] * ratio));
                 }
-                // values: lane (g, qd) takes the chunk of dims of column g, of the tokens 2 qd, 2 qd + 1 and those 8 further on
+                // values, transposed: lane (g, qd) takes the D / 8 dims of column g, of the tokens 2 qd, 2 qd + 1 and those 8 further on
                 const uint8_t* const values = stage + S::kTileBytes + 16 * warp * D;
-                constexpr int kWords = D / 32;   // 4 dims each of a lane's D / 8
+                constexpr int kWords = D / 32;   // 4 dims each
                 uint32_t v[4][kWords];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -388,49 +412,47 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
                     }
                 }
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) {
-                    uint32_t pair[4];   // bytes of two tokens side by side: dims 0, 1 and 2, 3 of the first two tokens, then of the others
-                    pair[0] = __byte_perm(v[0][w], v[1][w], 0x5140);
-                    pair[1] = __byte_perm(v[0][w], v[1][w], 0x7362);
-                    pair[2] = __byte_perm(v[2][w], v[3][w], 0x5140);
-                    pair[3] = __byte_perm(v[2][w], v[3][w], 0x7362);
+                for (int w = 0; w < kWords; ++w)
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        const uint32_t which = (d & 1) ? 0x4342 : 0x4140;
-                        mma_f16(o[4 * w + d], pf, code_halves(pair[d >> 1], which), code_halves(pair[2 + (d >> 1)], which));
+                    for (int h = 0; h < 2; ++h) {
+                        // bytes of two tokens side by side, of dims 2 h and 2 h + 1 of the word
+                        const uint32_t near = __byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140), far = __byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140);
+                        const uint32_t vf[4] = {code_halves(near, 0x4140), code_halves(near, 0x4342), code_halves(far, 0x4140), code_halves(far, 0x4342)};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + h], vf, pf[nt][0], pf[nt][1]);
                     }
-                }
             }
             __syncwarp();
             if (lane == 0) bar_arrive(smem_addr(&s_empty[s]));
-            if (++s == kAttnStages) {
+            if (++s == kStages) {
                 s = 0;
                 phase ^= 1;
             }
         }
 
         // ---- the four warps' sums together ----
-        float* const s_o = reinterpret_cast<float*>(s_mem + kAttnStages * S::kStageBytes);
-        constexpr int kDims = D / 8;   // dims of a lane's column
+        float* const s_o = reinterpret_cast<float*>(s_mem + kStages * S::kStageBytes);
+        constexpr int kDims = D / 8;   // of a lane
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            float* const to = s_o + (warp * kRowTile + g + 8 * r) * S::kRowFloats;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int u = 0; u < kDims; u += 4)
-                    *reinterpret_cast<float4*>(to + (2 * qd + e) * kDims + u) = make_float4(o[u][2 * r + e], o[u + 1][2 * r + e], o[u + 2][2 * r + e], o[u + 3][2 * r + e]);
-            if (qd == 0) {
-                s_ml[warp][g + 8 * r][0] = m[r];
-                s_ml[warp][g + 8 * r][1] = l[r];
+                for (int b = 4; b < 32; b <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], b);
+                const int r = 8 * nt + 2 * qd + e;
+                float* const to = s_o + (warp * kRows + r) * S::kRowFloats + g * kDims;
+#pragma unroll
+                for (int u = 0; u < D / 16; u += 2)
+                    *reinterpret_cast<float4*>(to + 2 * u) = make_float4(o[nt][u][e], o[nt][u][2 + e], o[nt][u + 1][e], o[nt][u + 1][2 + e]);
+                if (g == 0) {
+                    s_ml[warp][r][0] = m[nt][e];
+                    s_ml[warp][r][1] = l[nt][e];
+                }
             }
-        }
         if (lane == 0) s_vref[warp] = vref;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kMulWarps) : "memory");
         {
-            constexpr int kEach = kRowTile * D / (32 * kMulWarps);   // dims of a thread
+            constexpr int kEach = kRows * D / (32 * kMulWarps);   // dims of a thread
             const int r = tid / (D / kEach), d0 = tid % (D / kEach) * kEach;
             float top = -INFINITY, sum = 0.f, acc[kEach];
 #pragma unroll
@@ -442,7 +464,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
                 // (a warp that saw nothing has zeros; one that met a NaN has no maximum, and its sum says so)
                 const float mw = s_ml[w][r][0], x = mw == top || mw == -INFINITY ? 1.f : exp2_approx(mw - top), y = x * s_vref[w];
                 sum = fmaf(s_ml[w][r][1], x, sum);
-                const float* const from = s_o + (w * kRowTile + r) * S::kRowFloats + d0;
+                const float* const from = s_o + (w * kRows + r) * S::kRowFloats + d0;
 #pragma unroll
                 for (int d = 0; d < kEach; d += 4) {
                     const float4 v = *reinterpret_cast<const float4*>(from + d);
@@ -458,25 +480,24 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
                     __half* const to = a.out + (at.w.start + token) * a.out_stride + static_cast<long>(hq) * D + d0;
                     const float inv = 1.f / sum;
 #pragma unroll
-                    for (int d = 0; d < kEach; ++d) acc[d] *= inv;
-                    if (out_wide) {
-#pragma unroll
-                        for (int d = 0; d < kEach; d += 8) {
-                            const float v[8] = {acc[d], acc[d + 1], acc[d + 2], acc[d + 3], acc[d + 4], acc[d + 5], acc[d + 6], acc[d + 7]};
-                            *reinterpret_cast<uint4*>(to + d) = pack_halves(v);
+                    for (int d = 0; d < kEach; d += 4) {
+                        const uint2 four = make_uint2(pack_half2(acc[d] * inv, acc[d + 1] * inv), pack_half2(acc[d + 2] * inv, acc[d + 3] * inv));
+                        if (out_wide) *reinterpret_cast<uint2*>(to + d) = four;
+                        else {
+                            to[d] = __ushort_as_half(static_cast<unsigned short>(four.x));
+                            to[d + 1] = __ushort_as_half(static_cast<unsigned short>(four.x >> 16));
+                            to[d + 2] = __ushort_as_half(static_cast<unsigned short>(four.y));
+                            to[d + 3] = __ushort_as_half(static_cast<unsigned short>(four.y >> 16));
                         }
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < kEach; ++d) to[d] = __float2half_rn(acc[d]);
                     }
                     if (a.lse && d0 == 0)
-                        a.lse[(at.w.start + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kWeightOffset + log2f(sum)) * 0.6931471805599453f;
+                        a.lse[(at.w.start + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(sum)) * 0.6931471805599453f;
                 }
             } else {
                 float* const part = a.partial + (2 * c + (begins ? 1 : 0)) * static_cast<long>(S::kPart);
 #pragma unroll
                 for (int d = 0; d < kEach; d += 4) *reinterpret_cast<float4*>(part + r * D + d0 + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-                if (d0 == 0) *reinterpret_cast<float2*>(part + kRowTile * D + 2 * r) = make_float2(top, sum);
+                if (d0 == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * r) = make_float2(top, sum);
                 if (begins && tid == 0) {
                     // the CTA that holds the item's last unit: the largest c' with total * c' / ctas <= that unit
                     const long long last_unit = u1 - at.left + (at.w.hi - at.tile) - 1;
@@ -490,9 +511,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) paged_attn_kernel(con
 }
 
 // Parts of an item that several CTAs share, in the CTAs' order, a CTA per row: its four warps take a quarter of the parts each.
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int kPart = AttnShape<D>::kPart, kEach = D / 32;
+    constexpr int kPart = AttnShape<D, NT>::kPart, kRows = 8 * NT, kEach = D / 32;
     __shared__ float s_acc[4][D], s_sum[4];
     pdl_wait_release();
     const PagedJoin join = a.joins[blockIdx.x];
@@ -501,7 +522,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     const int parts = join.last - c + 1;
     auto part_of = [&](int k) { return a.partial + (2 * (c + k) + (k == 0 ? 1 : 0)) * static_cast<long>(kPart); };
     float top = -INFINITY;
-    for (int k = lane; k < parts; k += 32) top = fmaxf(top, part_of(k)[kRowTile * D + 2 * r]);
+    for (int k = lane; k < parts; k += 32) top = fmaxf(top, part_of(k)[kRows * D + 2 * r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int k0 = parts * warp / 4, k1 = parts * (warp + 1) / 4;
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float* const p = part_of(min(base + k, k1 - 1));
-            ml[k] = *reinterpret_cast<const float2*>(p + kRowTile * D + 2 * r);
+            ml[k] = *reinterpret_cast<const float2*>(p + kRows * D + 2 * r);
 #pragma unroll
             for (int d = 0; d < kEach; ++d) v[k][d] = p[r * D + 32 * d + lane];
         }
@@ -534,29 +555,36 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     for (int d = threadIdx.x; d < D; d += 128)
         a.out[(join.token + token) * a.out_stride + static_cast<long>(hq) * D + d] = __float2half_rn((s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d]) * inv);
     if (a.lse && threadIdx.x == 0)
-        a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kWeightOffset + log2f(all)) * 0.6931471805599453f;
+        a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(all)) * 0.6931471805599453f;
 }
 
-template <int D>
+template <int D, int NT>
 void launch_typed(PagedAttnArgs a, int max_rows, void* scratch, int sms, cudaStream_t st) {
-    const int ctas = sms * kAttnCtas;
+    using S = AttnShape<D, NT>;
+    const int ctas = sms * S::kCtas;
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
-    TQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnShape<D>::kSmem));
-    launch_pdl(paged_attn_kernel<D>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), AttnShape<D>::kSmem, st, a);
-    const int rows = std::min(kRowTile, max_rows);
-    launch_pdl(paged_join_kernel<D>, dim3(static_cast<unsigned int>(ctas), static_cast<unsigned int>(rows)), dim3(128), 0, st, a);
+    TQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    launch_pdl(paged_attn_kernel<D, NT>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), S::kSmem, st, a);
+    launch_pdl(paged_join_kernel<D, NT>, dim3(static_cast<unsigned int>(ctas), static_cast<unsigned int>(std::min(S::kRows, max_rows))), dim3(128), 0, st, a);
+}
+template <int D, int NT>
+size_t scratch_of(int sms) {
+    using S = AttnShape<D, NT>;
+    const size_t ctas = static_cast<size_t>(sms) * S::kCtas;
+    return (ctas * sizeof(PagedJoin) + 255) / 256 * 256 + ctas * 2 * S::kPart * sizeof(float);
 }
 
 }  // namespace
 
 size_t paged_attn_scratch_bytes(int dim, int sms) {
-    const size_t ctas = static_cast<size_t>(sms) * kAttnCtas;
-    return (ctas * sizeof(PagedJoin) + 255) / 256 * 256 + ctas * 2 * kRowTile * (static_cast<size_t>(dim) + 2) * sizeof(float);
+    return dim == 64 ? std::max(scratch_of<64, 1>(sms), scratch_of<64, 2>(sms)) : std::max(scratch_of<128, 1>(sms), scratch_of<128, 2>(sms));
 }
 void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratch, int sms, cudaStream_t st) {
-    if (dim == 64) launch_typed<64>(a, max_rows, scratch, sms, st);
-    else launch_typed<128>(a, max_rows, scratch, sms, st);
+    // Eight rows at a time where no request has more: half the products and registers of sixteen.
+    const bool eight = max_rows <= 8;
+    if (dim == 64) eight ? launch_typed<64, 1>(a, max_rows, scratch, sms, st) : launch_typed<64, 2>(a, max_rows, scratch, sms, st);
+    else eight ? launch_typed<128, 1>(a, max_rows, scratch, sms, st) : launch_typed<128, 2>(a, max_rows, scratch, sms, st);
 }
 
 }  // namespace tq
