@@ -99,7 +99,7 @@ public:
             TQ_REQUIRE(!p || tq::is_device_pointer(p), "paged plan: outputs must be device pointers");
         begin(st);
         tq::PagedPlanArgs a{b_, staged(rows, n, 0, st), staged(counts, n, b_.max_requests, st), n, tokens, max_count, starts, lengths, slots, positions, tables,
-                            tables_width, d_status_};
+                            tables_width, d_status_, sms_};
         tq::launch_paged_plan(a, st);
         n_ = n;
         tokens_ = tokens;
@@ -116,6 +116,7 @@ public:
         a.counts = staged(lengths, n, b_.max_requests, st);
         a.n = n;
         a.status = d_status_;
+        a.sms = sms_;
         tq::launch_paged_truncate(a, st);
         n_ = -1;
     }

@@ -15,6 +15,7 @@
 // in the same banks otherwise.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 
 #include "tq_common.cuh"
@@ -74,6 +75,17 @@ enum PagedStatus : unsigned int {
     kPagedWait = 7         // a bounded wait ran out
 };
 
+// Lets a kernel have so much dynamic shared memory, once for each device (`set`: those that have been).
+template <typename Kernel>
+void allow_shared_memory(Kernel kernel, size_t bytes, std::atomic<unsigned long long>& set) {
+    int device = 0;
+    TQ_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (set.load(std::memory_order_relaxed) & bit)) return;
+    TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    set.fetch_or(bit, std::memory_order_relaxed);
+}
+
 // ---- launches (tq_paged_plan.cu) ---------------------------------------------------------------
 struct PagedPlanArgs {
     PagedBatch b;
@@ -87,6 +99,7 @@ struct PagedPlanArgs {
     int* tables;
     int tables_width;
     unsigned int* status;
+    int sms;
 };
 void launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st);
 // counts: the lengths to keep
@@ -118,6 +131,7 @@ void launch_paged_read(const PagedReadArgs& a, int dim, bool half, cudaStream_t 
 // An item that several CTAs share, as the CTA in which it begins leaves it for the kernel that adds the parts up.
 struct PagedJoin {
     int last;        // the CTA in which it ends; 0: nothing to join (CTA 0 is never a last one)
+    int cta;         // the one in which it begins
     int token;       // first token of its request
     int first_row;   // rows (token-major: row = token * group + head of the group) first_row ..
     int rows;        // ... and how many
@@ -135,6 +149,7 @@ struct PagedAttnArgs {
     float scale_log2;    // softmax scale times log2(e)
     float* partial;
     PagedJoin* joins;
+    int join_items, row_tiles;   // few rows: entries of `joins` where each item has one (0: one for each CTA), and row tiles of a request at most
     unsigned int* status;
 };
 size_t paged_attn_scratch_bytes(int dim, int sms);

@@ -17,6 +17,7 @@
 // Rounding: products of halves are exact and summed in fp32; the softmax is fp32; the weights are rounded to halves for the second product
 // (times 2^15, so that they are normal numbers down to 2^-29 of the largest), their sum is taken before that.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -31,6 +32,7 @@ using namespace paged_device;
 
 constexpr int kTileTokens = 64;       // tokens of a unit
 constexpr int kMulWarps = 4;
+constexpr int kLeastUnits = 1;        // of a CTA
 constexpr int kAttnThreads = 32 * (kMulWarps + 1);
 // The reference maximum of a row moves only when a score exceeds it by 2^kSlack: a vote instead of a reduction for most tiles.  Weights are held times 2^kOffset and at most
 // 2^15: halves that are normal numbers down to 2^-25 of the reference.
@@ -71,7 +73,8 @@ struct RequestWork {
         hi = (held + kTileTokens - 1) / kTileTokens;
         row_tiles = start + count <= a.tokens && count * a.group <= a.few_rows ? (count * a.group + tile_rows - 1) / tile_rows : 0;
     }
-    __device__ __forceinline__ long long units(int heads) const { return static_cast<long long>(row_tiles) * heads * (hi - lo); }
+    // (A unit is some 8 KB of the cache at least, twice at most: all of them are a 32-bit number.)
+    __device__ __forceinline__ unsigned int units(int heads) const { return static_cast<unsigned int>(row_tiles * heads) * static_cast<unsigned int>(hi - lo); }
 };
 
 // A CTA's share [u, end) of the units and where it stands in them: (request, KV head, row tile, tile), the tile running fastest.
@@ -79,8 +82,8 @@ template <int ROWS>
 struct Walker {
     RequestWork w;
     int i, n, head, row_tile, tile;
-    long long left;      // units of the share that are still to do, this item's included
-    __device__ __forceinline__ void place(const PagedAttnArgs& a, int request, long long skip, long long units) {
+    unsigned int left;   // units of the share that are still to do, this item's included
+    __device__ __forceinline__ void place(const PagedAttnArgs& a, int request, unsigned int skip, unsigned int units) {
         i = request;
         left = units;
         w.load(a, i, ROWS);
@@ -88,18 +91,18 @@ struct Walker {
             skip -= w.units(a.heads);
             w.load(a, ++i, ROWS);
         }
-        const int tiles = w.hi - w.lo;
+        const unsigned int tiles = static_cast<unsigned int>(w.hi - w.lo);
         tile = w.lo + static_cast<int>(skip % tiles);
         skip /= tiles;
-        row_tile = static_cast<int>(skip % w.row_tiles);
-        head = static_cast<int>(skip / w.row_tiles);
+        head = static_cast<int>(skip / static_cast<unsigned int>(w.row_tiles));
+        row_tile = static_cast<int>(skip) - head * w.row_tiles;
     }
     // Tiles of the present item that belong to the share.
-    __device__ __forceinline__ int run() const { return static_cast<int>(min(static_cast<long long>(w.hi - tile), left)); }
+    __device__ __forceinline__ int run() const { return static_cast<int>(min(static_cast<unsigned int>(w.hi - tile), left)); }
     // Behind that run; false at the share's end.
     __device__ __forceinline__ bool next(const PagedAttnArgs& a) {
-        left -= run();
-        if (left <= 0) return false;
+        left -= static_cast<unsigned int>(run());
+        if (left == 0) return false;
         if (++row_tile == w.row_tiles) {
             row_tile = 0;
             if (++head == a.heads) {
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
     constexpr int kRows = S::kRows, kStages = S::kStages;
     extern __shared__ __align__(128) uint8_t s_mem[];
     __shared__ __align__(8) unsigned long long s_full[kStages], s_empty[kStages];
-    __shared__ long long s_sum[kAttnThreads + 1];
+    __shared__ unsigned int s_sum[kAttnThreads + 1];
     __shared__ float s_ml[kMulWarps][kRows][2], s_vref[kMulWarps];
     __shared__ unsigned int s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -147,41 +150,44 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait_release();
-    const int n = min(a.n, a.b.header->requests);
-
-    // units in front of each thread's requests
-    const int per = (n + kAttnThreads - 1) / kAttnThreads;
+    // units in front of each thread's requests (a plan that was refused has none, which is known only when they have been read)
+    const int per = (a.n + kAttnThreads - 1) / kAttnThreads;
     {
-        long long mine = 0;
-        for (int i = tid * per; i < min(n, (tid + 1) * per); ++i) {
+        const int requests = a.b.header->requests;
+        unsigned int mine = 0;
+        for (int i = tid * per; i < min(a.n, (tid + 1) * per); ++i) {
             RequestWork w;
             w.load(a, i, kRows);
-            mine += w.units(a.heads);
+            const unsigned int units = i < requests ? w.units(a.heads) : 0u;
+            mine += units;
+            if (units == 0u && blockIdx.x == 0)   // (its items, which no CTA begins)
+                for (int k = i * a.heads * a.row_tiles; k < min((i + 1) * a.heads * a.row_tiles, a.join_items); ++k) a.joins[k].last = 0;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, mine, o);
+            const unsigned int t = __shfl_up_sync(0xffffffffu, mine, o);
             if (lane >= o) mine += t;
         }
         s_sum[tid + 1] = mine;
     }
     __syncthreads();
-    long long total = 0, before[kMulWarps + 1];
+    unsigned int total = 0, before[kMulWarps + 1];
 #pragma unroll
     for (int k = 0; k < kMulWarps + 1; ++k) {
         before[k] = total;
         total += s_sum[32 * (k + 1)];
     }
-    const long long ctas = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
-    if (tid == 0) a.joins[c].last = 0;
+    const unsigned int ctas = min(gridDim.x, (total + kLeastUnits - 1) / kLeastUnits), c = blockIdx.x;
+    if (tid == 0 && a.join_items == 0) a.joins[c].last = 0;
     if (c >= ctas) return;
-    const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
+    const unsigned int share = total / ctas, extra = total - share * ctas;   // the first `extra` CTAs have one unit more
+    const unsigned int u0 = c * share + min(c, extra), u1 = u0 + share + (c < extra ? 1u : 0u);
     Walker<kRows> at;
     {
         // the thread's range of requests in which the share begins: the last whose sum in front is at most u0
         int lo = 0, hi = kAttnThreads;
         auto front = [&](int t) {
-            long long b = 0;
+            unsigned int b = 0;
 #pragma unroll
             for (int k = 0; k < kMulWarps + 1; ++k)
                 if (k == t >> 5) b = before[k];
@@ -321,11 +327,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 float2 scales = *reinterpret_cast<const float2*>(stage + 2 * S::kTileBytes + 16 * ((16 * warp) >> span_shift));
                 if (!(scales.y < INFINITY)) scales = make_float2(__uint_as_float(0x7fc00000u), 0.f);   // values that are not numbers: the rows that see them
                 // scores: tokens g (elements 0, 1) and g + 8 (2, 3), rows 2 qd and 2 qd + 1
-                float sc[NT][4];
+                float sc[NT][4], odd[NT][4];   // (two chains of products)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) sc[nt][k] = 0.f;
+                    for (int k = 0; k < 4; ++k) sc[nt][k] = odd[nt][k] = 0.f;
                 const uint8_t* const keys = stage + 16 * warp * D;
 #pragma unroll
                 for (int j = 0; j < D / 64; ++j) {
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t kf[4] = {code_halves(n4[k], 0x4140), code_halves(f4[k], 0x4140), code_halves(n4[k], 0x4342), code_halves(f4[k], 0x4342)};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt], kf, qf[nt][4 * j + k][0], qf[nt][4 * j + k][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma_f16(k & 1 ? odd[nt] : sc[nt], kf, qf[nt][4 * j + k][0], qf[nt][4 * j + k][1]);
                     }
                 }
                 const float f = scales.x * a.scale_log2;
@@ -346,7 +352,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        float x = sc[nt][k] * f;
+                        float x = (sc[nt][k] + odd[nt][k]) * f;
                         if (masks) {
                             const int token = w0 + g + 8 * (k >> 1), p = pos[nt][k & 1];
                             if (token > p || (a.window > 0 && token <= p - a.window)) x = -INFINITY;
@@ -494,15 +500,27 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                         a.lse[(at.w.start + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(sum)) * 0.6931471805599453f;
                 }
             } else {
-                float* const part = a.partial + (2 * c + (begins ? 1 : 0)) * static_cast<long>(S::kPart);
+                float* const part = a.partial + static_cast<long>(2 * c + (begins ? 1 : 0)) * S::kPart;
 #pragma unroll
                 for (int d = 0; d < kEach; d += 4) *reinterpret_cast<float4*>(part + r * D + d0 + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
                 if (d0 == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * r) = make_float2(top, sum);
-                if (begins && tid == 0) {
-                    // the CTA that holds the item's last unit: the largest c' with total * c' / ctas <= that unit
-                    const long long last_unit = u1 - at.left + (at.w.hi - at.tile) - 1;
-                    a.joins[c] = {static_cast<int>(((last_unit + 1) * ctas - 1) / total), at.w.start, row0, live_rows, at.head};
-                }
+            }
+        }
+        if (begins && tid == 0) {
+            int last = 0;
+            if (!ends) {
+                // the CTA that holds the item's last unit
+                const unsigned int unit = u1 - at.left + static_cast<unsigned int>(at.w.hi - at.tile) - 1, longer = extra * (share + 1);
+                last = static_cast<int>(unit < longer ? unit / (share + 1) : extra + (unit - longer) / share);
+            }
+            if (a.join_items) {
+                // (an item of fewer row tiles than there can be: the others' entries are never its own)
+                const int item = (at.i * a.heads + at.head) * a.row_tiles + at.row_tile;
+                a.joins[item] = {last, static_cast<int>(c), at.w.start, row0, live_rows, at.head};
+                if (at.row_tile == 0)
+                    for (int k = at.w.row_tiles; k < a.row_tiles; ++k) a.joins[item + k].last = 0;
+            } else if (last) {
+                a.joins[c] = {last, static_cast<int>(c), at.w.start, row0, live_rows, at.head};
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kMulWarps) : "memory");
@@ -510,63 +528,86 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
     }
 }
 
-// Parts of an item that several CTAs share, in the CTAs' order, a CTA per row: its four warps take a quarter of the parts each.
+// Parts of an item that several CTAs share, a CTA per item and row: eight warps take an eighth of the parts each, in the CTAs' order, and are added up in theirs.  It is bound by
+// the latency of one load behind another, of which 8 parts' of a warp are on their way at once.  (A CTA per item: what one SM fetches from the L2 cache bounds it, 65 parts of a
+// single request 13 -> 14.5 us.)
+constexpr int kJoinWarps = 8;
 template <int D, int NT>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int kPart = AttnShape<D, NT>::kPart, kRows = 8 * NT, kEach = D / 32;
-    __shared__ float s_acc[4][D], s_sum[4];
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int kPart = AttnShape<D, NT>::kPart, kRows = 8 * NT, kEach = D / 32, kAtOnce = 8;
+    __shared__ __align__(16) float s_acc[kJoinWarps][D];
+    __shared__ float2 s_ml[kJoinWarps];
     pdl_wait_release();
     const PagedJoin join = a.joins[blockIdx.x];
-    const int r = blockIdx.y, c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = blockIdx.y, c = join.cta, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (join.last == 0 || r >= join.rows) return;
     const int parts = join.last - c + 1;
-    auto part_of = [&](int k) { return a.partial + (2 * (c + k) + (k == 0 ? 1 : 0)) * static_cast<long>(kPart); };
-    float top = -INFINITY;
-    for (int k = lane; k < parts; k += 32) top = fmaxf(top, part_of(k)[kRows * D + 2 * r]);
+    const int k0 = parts * warp / kJoinWarps, k1 = parts * (warp + 1) / kJoinWarps;
+    float acc[kEach] = {}, top = -INFINITY, sum = 0.f;
+    for (int base = k0; base < k1; base += kAtOnce) {
+        float2 ml[kAtOnce];
+        float v[kAtOnce][kEach];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int k0 = parts * warp / 4, k1 = parts * (warp + 1) / 4;
-    float acc[kEach] = {}, sum = 0.f;
-    for (int base = k0; base < k1; base += 8) {
-        float2 ml[8];
-        float v[8][kEach];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float* const p = part_of(min(base + k, k1 - 1));
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int part = min(base + k, k1 - 1);
+            const float* const p = a.partial + static_cast<long>(2 * (c + part) + (part == 0 ? 1 : 0)) * kPart;
             ml[k] = *reinterpret_cast<const float2*>(p + kRows * D + 2 * r);
-#pragma unroll
-            for (int d = 0; d < kEach; ++d) v[k][d] = p[r * D + 32 * d + lane];
+            if constexpr (kEach == 4) {
+                const float4 f = *reinterpret_cast<const float4*>(p + r * D + 4 * lane);
+                v[k][0] = f.x; v[k][1] = f.y; v[k][2] = f.z; v[k][3] = f.w;
+            } else {
+                const float2 f = *reinterpret_cast<const float2*>(p + r * D + 2 * lane);
+                v[k][0] = f.x; v[k][1] = f.y;
+            }
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kAtOnce; ++k) {
             if (base + k >= k1) continue;
-            const float x = ml[k].x == top || ml[k].x == -INFINITY ? 1.f : exp2_approx(ml[k].x - top);
-            sum = fmaf(ml[k].y, x, sum);
+            const float to = fmaxf(top, ml[k].x);
+            const float y = top == to || top == -INFINITY ? 1.f : exp2_approx(top - to), x = ml[k].x == to || ml[k].x == -INFINITY ? 1.f : exp2_approx(ml[k].x - to);
+            top = to;
+            sum = fmaf(ml[k].y, x, sum * y);
 #pragma unroll
-            for (int d = 0; d < kEach; ++d) acc[d] = fmaf(v[k][d], x, acc[d]);
+            for (int d = 0; d < kEach; ++d) acc[d] = fmaf(v[k][d], x, acc[d] * y);
         }
     }
 #pragma unroll
-    for (int d = 0; d < kEach; ++d) s_acc[warp][32 * d + lane] = acc[d];
-    if (lane == 0) s_sum[warp] = sum;
+    for (int d = 0; d < kEach; ++d) s_acc[warp][kEach * lane + d] = acc[d];
+    if (lane == 0) s_ml[warp] = make_float2(top, sum);
     __syncthreads();
-    const float all = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], inv = 1.f / all;
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
+    float all = 0.f, value = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float x = s_ml[w].x == top || s_ml[w].x == -INFINITY ? 1.f : exp2_approx(s_ml[w].x - top);
+        all = fmaf(s_ml[w].y, x, all);
+        value = fmaf(s_acc[w][d], x, value);
+    }
     const int row = join.first_row + r, token = row / a.group, hq = join.head * a.group + row - token * a.group;
-    for (int d = threadIdx.x; d < D; d += 128)
-        a.out[(join.token + token) * a.out_stride + static_cast<long>(hq) * D + d] = __float2half_rn((s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d]) * inv);
-    if (a.lse && threadIdx.x == 0)
-        a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(all)) * 0.6931471805599453f;
+    a.out[(join.token + token) * a.out_stride + static_cast<long>(hq) * D + d] = __float2half_rn(value / all);
+    if (a.lse && d == 0) a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(all)) * 0.6931471805599453f;
 }
 
 template <int D, int NT>
 void launch_typed(PagedAttnArgs a, int max_rows, void* scratch, int sms, cudaStream_t st) {
     using S = AttnShape<D, NT>;
     const int ctas = sms * S::kCtas;
+    // Items that there can be: where they are fewer than the CTAs each has its own entry, and the kernel behind as many CTAs.
+    a.row_tiles = (max_rows + S::kRows - 1) / S::kRows;
+    const long items = static_cast<long>(a.n) * a.heads * a.row_tiles;
+    a.join_items = items <= ctas ? static_cast<int>(items) : 0;
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
-    TQ_CUDA(cudaFuncSetAttribute(paged_attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    launch_pdl(paged_attn_kernel<D, NT>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), S::kSmem, st, a);
-    launch_pdl(paged_join_kernel<D, NT>, dim3(static_cast<unsigned int>(ctas), static_cast<unsigned int>(std::min(S::kRows, max_rows))), dim3(128), 0, st, a);
+    static std::atomic<unsigned long long> set{0};
+    allow_shared_memory(paged_attn_kernel<D, NT>, S::kSmem, set);
+    // (Both ask for all of the SM's memory as shared memory: an SM changes its division only when it is empty.)
+    launch_pdl_carved(paged_attn_kernel<D, NT>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), S::kSmem, 100, st, a);
+    launch_pdl_carved(paged_join_kernel<D, NT>, dim3(static_cast<unsigned int>(a.join_items ? a.join_items : ctas), static_cast<unsigned int>(std::min(S::kRows, max_rows))),
+                      dim3(32 * kJoinWarps), 0, 100, st, a);
 }
 template <int D, int NT>
 size_t scratch_of(int sms) {

@@ -5,6 +5,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -77,18 +78,20 @@ __device__ __forceinline__ bool seen_before(unsigned int* seen, int row) {
     return (atomicOr(&seen[row >> 5], bit) & bit) != 0;
 }
 
-// One cluster.  Every CTA reads all requests and takes the sums over them (4096 at most, from the L2 cache); behind the cluster's
-// barrier nobody reads what is about to change, and the CTAs share the output: tokens, pieces, new pages and the tables' copy, each
-// element found by a binary search in the sums.  A single launch, all or nothing: a batch that does not fit leaves the cache as it was, an
-// empty plan and a status.  It is bound by latency: a launch, two dependent loads, the sums' three barriers.
+// Every CTA reads all requests and takes the sums over them (4096 at most, from the L2 cache), and the CTAs share the output: tokens, pieces, new pages and the
+// tables' copy, each element found by a binary search in the sums.  All or nothing: a batch that does not fit leaves the cache as it was, an empty plan and a
+// status.  COMMIT: one cluster, behind whose barrier nobody reads the lengths and the number of free pages any more, which then change.  It is bound by latency: a
+// launch, two dependent loads, the sums' barriers.  Much output is written by as many CTAs as there are SMs (OUTPUT), with no barrier between them, in front of a cluster that only
+// commits (61 prompts of up to 8192 tokens, 3 MB: 54 us with one cluster of eight for both, 13 so).
+template <bool OUTPUT, bool COMMIT>
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs a) {
     pdl_wait_release();
     behind_wait(a.rows, a.counts);
     extern __shared__ int s_plan[];
     __shared__ unsigned int s_seen[kPagedMaxRequests / 32];
     __shared__ unsigned int s_error;
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+    // (the grid is the cluster where it commits)
+    const int rank = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
     const int n = a.n, P = a.b.page_tokens, tid = threadIdx.x;
     int* const s_row = s_plan;             // [n]
     int* const s_old = s_row + n;          // [n]
@@ -153,7 +156,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         s_page[n] = pages;
         s_piece[n] = pieces;
     }
-    cluster.sync();   // every CTA has read the lengths and the number of free pages (and its own sums are complete)
+    if constexpr (COMMIT) cg::this_cluster().sync();   // every CTA has read the lengths and the number of free pages (and its own sums are complete)
+    else __syncthreads();
 
     // page `idx` of request i, before the plan's writes to the tables
     auto page_of = [&](int i, int idx) {
@@ -161,21 +165,24 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         return idx < had ? a.b.tables[static_cast<size_t>(s_row[i]) * a.b.max_pages + idx] : a.b.stack[free_before - 1 - (s_page[i] + idx - had)];
     };
     const int t0 = rank * kPlanThreads + tid, step = ctas * kPlanThreads;
-    for (int t = t0; t < n; t += step) {
-        const int now = s_old[t] + s_start[t + 1] - s_start[t];
-        a.b.rows[t] = s_row[t];
-        a.b.starts[t] = s_start[t];
-        a.b.held[t] = now;
-        if (ok) a.b.lengths[s_row[t]] = now;
-        if (a.starts) a.starts[t] = s_start[t];
-        if (a.lengths) a.lengths[t] = now;
+    if constexpr (COMMIT) {
+        for (int t = t0; t < n; t += step) {
+            const int now = s_old[t] + s_start[t + 1] - s_start[t];
+            a.b.rows[t] = s_row[t];
+            a.b.starts[t] = s_start[t];
+            a.b.held[t] = now;
+            if (ok) a.b.lengths[s_row[t]] = now;
+            if (a.starts) a.starts[t] = s_start[t];
+            if (a.lengths) a.lengths[t] = now;
+        }
+        if (t0 == 0) {
+            a.b.starts[n] = tokens;
+            if (a.starts) a.starts[n] = tokens;
+            *a.b.header = {free_before - pages, ok ? n : 0, tokens, pieces};
+            if (!ok) raise_status(a.status, error);
+        }
     }
-    if (t0 == 0) {
-        a.b.starts[n] = tokens;
-        if (a.starts) a.starts[n] = tokens;
-        *a.b.header = {free_before - pages, ok ? n : 0, tokens, pieces};
-        if (!ok) raise_status(a.status, error);
-    }
+    if constexpr (!OUTPUT) return;
     for (int t = t0; t < pages; t += step) {
         const int i = owner_of(s_page, n, t), idx = (s_old[i] + P - 1) / P + t - s_page[i];
         a.b.tables[static_cast<size_t>(s_row[i]) * a.b.max_pages + idx] = a.b.stack[free_before - 1 - t];
@@ -277,8 +284,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_truncate_kernel(PagedPlanA
     }
 }
 
+// `ctas` CTAs, a cluster where there are 2 .. 8 of them and they are to be one.
 template <typename Kernel>
-void launch_cluster(Kernel kernel, int ctas, size_t smem, const PagedPlanArgs& a, cudaStream_t st) {
+void launch_cluster(Kernel kernel, int ctas, bool cluster, size_t smem, const PagedPlanArgs& a, cudaStream_t st, std::atomic<unsigned long long>& set) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -291,12 +299,13 @@ void launch_cluster(Kernel kernel, int ctas, size_t smem, const PagedPlanArgs& a
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if (smem > 40 * 1024) TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    cfg.numAttrs = cluster && ctas > 1 ? 2 : 1;
+    if (smem > 40 * 1024) allow_shared_memory(kernel, (5 * static_cast<size_t>(kPagedMaxRequests) + 3) * sizeof(int), set);
     TQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
-// CTAs of a plan's cluster: one for every 4096 elements of output, up to 8 (the portable most).
+// CTAs of a plan's cluster: one for every 4096 elements of output, up to 8 (the portable most); for more output than kOneCluster see the kernel.
+constexpr long kOneCluster = 100000;
 int plan_ctas(long elements) {
     int ctas = 1;
     while (ctas < 8 && static_cast<long>(ctas) * 4096 < elements) ctas *= 2;
@@ -371,10 +380,10 @@ __device__ __forceinline__ void decode16(float (&v)[16], const uint4& c, float s
     for (int j = 0; j < 16; ++j) v[j] = static_cast<float>(static_cast<int>((w[j >> 2] >> (8 * (j & 3))) & 255u) - 128) * scale;
 }
 
-// A group of THREADS threads writes one piece's tokens of one head's keys or values: largest magnitude, scale, codes.  The tokens are read
-// twice, the second time from the caches.  What it does not write again (older tokens whose scale stays) it does not read.
-// WARP: a warp per job, four jobs to a CTA, for the few tokens of a decode step; otherwise a CTA per job.
-template <int D, typename T, bool WIDE, bool WARP>
+// A warp (for the few tokens of a decode step, four jobs to a CTA) or a CTA writes one piece's tokens of one head's keys or values: largest magnitude, scale, codes.  A thread takes 16
+// dims of ITER tokens, all asked for at once, which stay in registers (read twice, the second time from the caches, 67 thousand fp32 tokens of 8 heads took 145 us).
+// Older tokens of the page are read only where its scale grows.
+template <int D, typename T, bool WIDE, bool WARP, int ITER>
 __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedAppendArgs a) {
     constexpr int kThreads = WARP ? 32 : 256, kChunks = D / 16, kRows = kThreads / kChunks;
     pdl_wait_release();
@@ -394,20 +403,21 @@ __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedApp
         const long rest = job >> 1;
         const int head = static_cast<int>(rest % a.heads);
         const PagedPiece piece = a.pieces[rest / a.heads];
-        if (piece.token + piece.count > a.tokens) continue;   // a plan that this launch was not made for
+        if (piece.token + piece.count > a.tokens || piece.count > ITER * kRows) continue;   // a plan that this launch was not made for
         const long row_stride = second ? a.value_stride : a.key_stride;
         const T* const src = static_cast<const T*>(second ? a.values : a.keys) + piece.token * row_stride + static_cast<long>(head) * D + 16 * c;
         uint8_t* const dst = a.layer + (static_cast<size_t>(piece.page) * a.heads + head) * block;
         uint8_t* const codes = dst + (second ? static_cast<size_t>(P) * D : 0);
         float* const scale_at = reinterpret_cast<float*>(dst + 2 * static_cast<size_t>(P) * D) + (second ? 1 : 0);
-        unsigned int top = 0;
-        float v[16];
-        for (int r = r0; r < piece.count; r += kRows) {
-            load16<T, WIDE>(v, src + r * row_stride);
+        float v[ITER][16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-        }
+        for (int i = 0; i < ITER; ++i) load16<T, WIDE>(v[i], src + min(r0 + i * kRows, piece.count - 1) * row_stride);   // (rows behind the last: the last again)
         const unsigned int held = piece.offset ? __float_as_uint(*scale_at) : 0u;
+        unsigned int top = 0;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
         top = __reduce_max_sync(0xffffffffu, top);
         if constexpr (!WARP) {
             if (lane == 0) s_top[threadIdx.x >> 5] = top;
@@ -421,20 +431,23 @@ __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedApp
         auto place = [&](int token) {
             return reinterpret_cast<uint4*>(codes + static_cast<size_t>(token) * D + 16 * (second ? value_chunk<D>(token, c) : key_chunk<D>(token, c)));
         };
-        if (finite && piece.offset && scale != held) {
-            const float ratio = __uint_as_float(held) * inverse;
-            for (int t = r0; t < piece.offset; t += kRows) {
-                decode16(v, *place(t), 1.f);
-                *place(t) = encode16(v, ratio);
-            }
-        }
-        for (int r = r0; r < piece.count; r += kRows) {
-            load16<T, WIDE>(v, src + r * row_stride);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int r = r0 + i * kRows;
+            if (r >= piece.count) continue;
             if (!finite) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = 0.f;
+                for (int j = 0; j < 16; ++j) v[i][j] = 0.f;
             }
-            *place(piece.offset + r) = encode16(v, inverse);
+            *place(piece.offset + r) = encode16(v[i], inverse);
+        }
+        if (finite && piece.offset && scale != held) {
+            const float ratio = __uint_as_float(held) * inverse;
+            float old[16];
+            for (int t = r0; t < piece.offset; t += kRows) {
+                decode16(old, *place(t), 1.f);
+                *place(t) = encode16(old, ratio);
+            }
         }
         if (!WARP) __syncthreads();   // s_top, and the scale that was read, are everyone's until here
         else __syncwarp();
@@ -447,12 +460,15 @@ void launch_append_typed(const PagedAppendArgs& a, int n, int max_count, cudaStr
     // pieces that the plan can have: each of the requests begins and ends in a page of its own
     const long most = std::min<long>(a.tokens, a.tokens / a.page_tokens + 2L * n) * a.heads * 2;
     if (most == 0) return;
-    // A warp takes 4 tokens (of 128 dims) at a time, a CTA 32.
-    const bool warp = std::min(max_count, a.page_tokens) <= 8;
-    if (warp)
-        launch_pdl(paged_append_kernel<D, T, WIDE, true>, dim3(static_cast<unsigned int>(std::min<long>((most + 3) / 4, 1 << 20))), dim3(128), 0, st, a);
-    else
-        launch_pdl(paged_append_kernel<D, T, WIDE, false>, dim3(static_cast<unsigned int>(std::min<long>(most, 1 << 20))), dim3(256), 0, st, a);
+    constexpr int kWarpRows = 512 / D, kCtaRows = 4096 / D;   // tokens at a time
+    const int longest = std::min(max_count, a.page_tokens);
+    auto warps = [&](auto kernel) { launch_pdl(kernel, dim3(static_cast<unsigned int>(std::min<long>((most + 3) / 4, 1 << 20))), dim3(128), 0, st, a); };
+    auto ctas = [&](auto kernel) { launch_pdl(kernel, dim3(static_cast<unsigned int>(std::min<long>(most, 1 << 20))), dim3(256), 0, st, a); };
+    if (longest <= kWarpRows) warps(paged_append_kernel<D, T, WIDE, true, 1>);
+    else if (longest <= 2 * kWarpRows) warps(paged_append_kernel<D, T, WIDE, true, 2>);
+    else if (longest <= kCtaRows) ctas(paged_append_kernel<D, T, WIDE, false, 1>);
+    else if (longest <= 2 * kCtaRows) ctas(paged_append_kernel<D, T, WIDE, false, 2>);
+    else ctas(paged_append_kernel<D, T, WIDE, false, D == 128 ? 4 : 2>);
 }
 
 // ---- pages back -------------------------------------------------------------------------------------
@@ -499,11 +515,20 @@ __global__ void __launch_bounds__(256) paged_read_kernel(PagedReadArgs a) {
 }  // namespace
 
 void launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
-    const long out = std::max<long>(a.slots || a.positions ? a.tokens : 0, a.tables ? static_cast<long>(a.n) * a.tables_width : 0);
-    launch_cluster(paged_plan_kernel, plan_ctas(std::max<long>(out, a.tokens / a.b.page_tokens)), (5 * static_cast<size_t>(a.n) + 3) * sizeof(int), a, st);
+    const long out = std::max({a.slots || a.positions ? static_cast<long>(a.tokens) : 0L, a.tables ? static_cast<long>(a.n) * a.tables_width : 0L,
+                               static_cast<long>(a.tokens / a.b.page_tokens)});
+    const size_t smem = (5 * static_cast<size_t>(a.n) + 3) * sizeof(int);
+    static std::atomic<unsigned long long> set_all{0}, set_output{0}, set_commit{0};
+    if (out <= kOneCluster) launch_cluster(paged_plan_kernel<true, true>, plan_ctas(out), true, smem, a, st, set_all);
+    else {
+        launch_cluster(paged_plan_kernel<true, false>, static_cast<int>(std::min<long>(a.sms, (out + kPlanThreads - 1) / kPlanThreads)), false, smem, a, st, set_output);
+        launch_cluster(paged_plan_kernel<false, true>, 1, true, smem, a, st, set_commit);
+    }
 }
 void launch_paged_truncate(const PagedPlanArgs& a, cudaStream_t st) {
-    launch_cluster(paged_truncate_kernel, plan_ctas(std::min<long>(static_cast<long>(a.n) * a.b.max_pages, a.b.num_pages)), (3 * static_cast<size_t>(a.n) + 1) * sizeof(int), a, st);
+    static std::atomic<unsigned long long> set{0};
+    launch_cluster(paged_truncate_kernel, plan_ctas(std::min<long>(static_cast<long>(a.n) * a.b.max_pages, a.b.num_pages)), true,
+                   (3 * static_cast<size_t>(a.n) + 1) * sizeof(int), a, st, set);
 }
 void launch_paged_init(uint8_t* layer, size_t blocks, size_t block_bytes, cudaStream_t st) {
     paged_init_kernel<<<static_cast<unsigned int>(std::min<size_t>(blocks, 4096)), 256, 0, st>>>(layer, blocks, block_bytes);

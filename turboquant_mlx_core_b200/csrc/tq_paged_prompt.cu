@@ -24,6 +24,7 @@
 //
 // Every wait is bounded; a warp that gives up flags it, all warps fall through to the end, where the tensor memory is freed.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -495,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         }
                         *reinterpret_cast<float2*>(part + kPairRows * D + 2 * pr) = make_float2(m, l);
                         if (begins && t == 0 && r_in == 0) {
-                            a.joins[c] = {at.last, at.start, at.row0, min(kPairRows, at.rows - at.row0), at.head};
+                            a.joins[c] = {at.last, static_cast<int>(c), at.start, at.row0, min(kPairRows, at.rows - at.row0), at.head};
                         }
                     }
                     fence_before();
@@ -850,9 +851,10 @@ template <int D>
 void launch_typed(PagedAttnArgs a, void* scratch, int sms, cudaStream_t st) {
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (sms * sizeof(PagedJoin) + 255) / 256 * 256);
-    TQ_CUDA(cudaFuncSetAttribute(paged_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<D>::kSmem)));
-    launch_pdl(paged_prompt_kernel<D>, dim3(static_cast<unsigned int>(sms)), dim3(kThreads), Shape<D>::kSmem, st, a);
-    launch_pdl(paged_prompt_join_kernel<D>, dim3(static_cast<unsigned int>(sms), kPairRows / kJoinRows), dim3(kJoinRows * D / 4), 0, st, a);
+    static std::atomic<unsigned long long> set{0};
+    allow_shared_memory(paged_prompt_kernel<D>, Shape<D>::kSmem, set);
+    launch_pdl_carved(paged_prompt_kernel<D>, dim3(static_cast<unsigned int>(sms)), dim3(kThreads), Shape<D>::kSmem, 100, st, a);
+    launch_pdl_carved(paged_prompt_join_kernel<D>, dim3(static_cast<unsigned int>(sms), kPairRows / kJoinRows), dim3(kJoinRows * D / 4), 0, 100, st, a);
 }
 
 }  // namespace

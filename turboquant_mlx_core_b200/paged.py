@@ -13,47 +13,61 @@ Tensors are torch CUDA tensors; rows, counts and lengths may be int32 numpy arra
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import numpy as np
 
 from . import _lib
 from ._lib import TQ_F16, TQ_F32, TQError, check
 from .api import _stream_ptr
 
+# A decode step's calls move microseconds of work each: their Python side is a handful of look-ups, and types are told by identity.
+_torch = None
 
-def _ints(x, what, n=None):
-    """Address of whole numbers of 32 bits, contiguous; `n`: how many there must be."""
+
+def _load_torch():
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
+def _ints(x, what, n):
+    """Address of n whole numbers of 32 bits, contiguous."""
     if x is None:
         return None
-    tensor = hasattr(x, "data_ptr")
-    if str(x.dtype).rpartition(".")[2] != "int32":
+    if hasattr(x, "data_ptr"):
+        fine, contiguous, size, at = x.dtype is _torch.int32, x.is_contiguous(), x.numel(), x.data_ptr()
+    else:
+        fine, contiguous, size, at = x.dtype == np.int32, x.flags["C_CONTIGUOUS"], x.size, x.ctypes.data
+    if not fine:
         raise TypeError(f"{what} must be int32, got {x.dtype}")
-    if not (x.is_contiguous() if tensor else x.flags["C_CONTIGUOUS"]):
+    if not contiguous:
         raise ValueError(f"{what} must be contiguous")
-    if n is not None and (x.numel() if tensor else x.size) != n:
+    if size != n:
         raise ValueError(f"{what} must have {n} elements")
-    return x.data_ptr() if tensor else x.ctypes.data
+    return at
 
 
 def _rows(x, heads, dim, what):
-    """[tokens, heads, dim] with contiguous heads: address, tokens, elements from token to token."""
+    """[tokens, heads, dim] with contiguous heads (`heads` 0: any number of them): address, tokens, heads, elements from token to token."""
     if not hasattr(x, "data_ptr"):
         raise TypeError(f"{what} must be a torch CUDA tensor")
-    if len(x.shape) != 3 or (heads and x.shape[1] != heads) or x.shape[2] != dim:
+    try:
+        tokens, n, d = x.shape
+        step, head, one = x.stride()
+    except ValueError:
+        d = None
+    if d != dim or (heads and n != heads):
         raise ValueError(f"{what} must be [tokens, {heads or 'heads'}, {dim}]")
-    stride = x.stride()
-    if stride[2] != 1 or (x.shape[1] > 1 and stride[1] != dim):
+    if one != 1 or (head != dim and n > 1):
         raise ValueError(f"the heads of a token of {what} must be contiguous")
-    row = x.shape[1] * dim
-    return x.data_ptr(), x.shape[0], stride[0] if x.shape[0] > 1 else max(row, stride[0])
+    return x.data_ptr(), tokens, n, step if tokens > 1 else max(n * dim, step)
 
 
 def _tag(x, what):
-    name = str(x.dtype)
-    if name.endswith("float16") and "bfloat" not in name:
+    if x.dtype is _torch.float16:
         return TQ_F16
-    if name.endswith("float32"):
+    if x.dtype is _torch.float32:
         return TQ_F32
     raise TypeError(f"{what}: expected float32 or float16, got {x.dtype}")
 
@@ -73,6 +87,7 @@ class PagedKVCache:
                                                 self.max_requests, self.max_pages_per_request, self.max_tokens)
         if not self._h:
             raise TQError("PagedKVCache: " + _lib.last_error())
+        _load_torch()
 
     @property
     def handle(self):
@@ -89,64 +104,69 @@ class PagedKVCache:
             max_count = int(counts.max(initial=0)) if max_count is None else max_count
         elif tokens is None or max_count is None:
             raise ValueError("plan: counts on the device need tokens and max_count")
-        n = int(counts.shape[0])
-        if tables is not None and (len(tables.shape) != 2 or tables.shape[0] != n):
-            raise ValueError("plan: tables must be [n, width]")
-        check(self._L.tq_paged_plan(self._h, _ints(rows, "rows", n), _ints(counts, "counts", n), n, int(tokens), int(max_count),
-                                    _ints(starts, "starts", n + 1), _ints(lengths, "lengths", n), _ints(slots, "slots", tokens),
-                                    _ints(positions, "positions", tokens), _ints(tables, "tables"),
-                                    0 if tables is None else int(tables.shape[1]), _stream_ptr(stream)), "PagedKVCache.plan")
+        n, width = counts.shape[0], 0
+        if tables is not None:
+            if len(tables.shape) != 2 or tables.shape[0] != n:
+                raise ValueError("plan: tables must be [n, width]")
+            width = tables.shape[1]
+        if self._L.tq_paged_plan(self._h, _ints(rows, "rows", n), _ints(counts, "counts", n), n, tokens, max_count, _ints(starts, "starts", n + 1),
+                                 _ints(lengths, "lengths", n), _ints(slots, "slots", tokens), _ints(positions, "positions", tokens),
+                                 _ints(tables, "tables", n * width), width, None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.plan")
 
     def truncate(self, lengths, rows=None, stream=None):
         """The request in row rows[i] (row i without rows) keeps its first lengths[i] tokens; 0 releases it."""
         if not hasattr(lengths, "data_ptr"):
             lengths = np.ascontiguousarray(lengths, np.int32)
-        n = int(lengths.shape[0])
-        check(self._L.tq_paged_truncate(self._h, _ints(rows, "rows", n), _ints(lengths, "lengths", n), n, _stream_ptr(stream)),
-              "PagedKVCache.truncate")
+        n = lengths.shape[0]
+        if self._L.tq_paged_truncate(self._h, _ints(rows, "rows", n), _ints(lengths, "lengths", n), n, None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.truncate")
 
     def append(self, layer: int, keys, values, stream=None):
         """Keys and values of the planned tokens, [tokens, heads, head_dim] fp32 or fp16; a token's heads are contiguous, tokens may be apart."""
-        kp, tokens, ks = _rows(keys, self.num_heads, self.head_dim, "keys")
-        vp, more, vs = _rows(values, self.num_heads, self.head_dim, "values")
-        if tokens != more or keys.dtype != values.dtype:
+        kp, tokens, _, ks = _rows(keys, self.num_heads, self.head_dim, "keys")
+        vp, more, _, vs = _rows(values, self.num_heads, self.head_dim, "values")
+        if tokens != more or keys.dtype is not values.dtype:
             raise ValueError("keys and values must have the same number of tokens and type")
-        check(self._L.tq_paged_append(self._h, int(layer), kp, vp, _tag(keys, "append"), tokens, ks, vs, _stream_ptr(stream)),
-              "PagedKVCache.append")
+        if self._L.tq_paged_append(self._h, layer, kp, vp, _tag(keys, "append"), tokens, ks, vs, None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.append")
 
     def attention(self, layer: int, queries, window: int = 0, scale: float = 0.0, out=None, lse=None, stream=None):
         """Causal attention of the planned tokens' queries, fp16 [tokens, q_heads, head_dim], over their requests; returns out.  A `window` of w
         lets a token see itself and the w - 1 before it.  lse: fp32 [tokens, q_heads], filled with the log of the softmax denominators."""
-        qp, tokens, qs = _rows(queries, None, self.head_dim, "queries")
-        if _tag(queries, "attention") != TQ_F16:
+        qp, tokens, q_heads, qs = _rows(queries, 0, self.head_dim, "queries")
+        half = _torch.float16
+        if queries.dtype is not half:
             raise TypeError("attention: queries must be float16")
         if out is None:
             out = queries.new_zeros(queries.shape)
-        op, more, os_ = _rows(out, int(queries.shape[1]), self.head_dim, "out")
-        if more != tokens or _tag(out, "attention") != TQ_F16:
+        op, more, _, os_ = _rows(out, q_heads, self.head_dim, "out")
+        if more != tokens or out.dtype is not half:
             raise ValueError("out must be float16 of the queries' shape")
-        if lse is not None and (tuple(lse.shape) != tuple(queries.shape[:2]) or _tag(lse, "attention") != TQ_F32 or not lse.is_contiguous()):
-            raise ValueError("lse must be contiguous float32 [tokens, q_heads]")
-        check(self._L.tq_paged_attention(self._h, int(layer), qp, tokens, int(queries.shape[1]), qs, int(window), float(scale), op, os_,
-                                         None if lse is None else lse.data_ptr(), _stream_ptr(stream)), "PagedKVCache.attention")
+        lp = None
+        if lse is not None:
+            if lse.dtype is not _torch.float32 or lse.shape != (tokens, q_heads) or not lse.is_contiguous():
+                raise ValueError("lse must be contiguous float32 [tokens, q_heads]")
+            lp = lse.data_ptr()
+        if self._L.tq_paged_attention(self._h, layer, qp, tokens, q_heads, qs, window, scale, op, os_, lp, None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.attention")
         return out
 
     def read_pages(self, layer: int, pages, keys=None, values=None, stream=None):
         """The values that whole pages hold (their numbers: an int32 tensor), into keys and values, [n, page_tokens, heads, head_dim] fp32 or
         fp16 tensors, either of them None."""
-        n = int(pages.shape[0])
-        shape, tags = (n, self.page_tokens, self.num_heads, self.head_dim), set()
-        for x in (keys, values):
+        n, tag, at = pages.shape[0], None, [None, None]
+        for i, x in enumerate((keys, values)):
             if x is None:
                 continue
-            if tuple(x.shape) != shape or not x.is_contiguous():
-                raise ValueError(f"keys and values must be contiguous {list(shape)}")
-            tags.add(_tag(x, "read_pages"))
-        if len(tags) > 1:
-            raise ValueError("keys and values must have the same type")
-        check(self._L.tq_paged_read(self._h, int(layer), _ints(pages, "pages", n), n, None if keys is None else keys.data_ptr(),
-                                    None if values is None else values.data_ptr(), tags.pop() if tags else TQ_F16, _stream_ptr(stream)),
-              "PagedKVCache.read_pages")
+            if x.shape != (n, self.page_tokens, self.num_heads, self.head_dim) or not x.is_contiguous():
+                raise ValueError(f"keys and values must be contiguous {[n, self.page_tokens, self.num_heads, self.head_dim]}")
+            if tag not in (None, _tag(x, "read_pages")):
+                raise ValueError("keys and values must have the same type")
+            tag, at[i] = _tag(x, "read_pages"), x.data_ptr()
+        if self._L.tq_paged_read(self._h, layer, _ints(pages, "pages", n), n, *at, TQ_F16 if tag is None else tag,
+                                 None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.read_pages")
 
     def free_pages(self) -> int:
         """Free pages, once all work is done (waits for the device)."""
