@@ -182,7 +182,7 @@ public:
         const long max_rows = static_cast<long>(max_count_) * a.group;
         const bool many = max_rows > kFewRows;
         a.few_rows = many && n_ == 1 ? 0 : kFewRows;
-        if (many) tq::launch_paged_prompt(a, dim_, scratch_.as<char>() + prompt_scratch_, sms_, st);
+        if (many) tq::launch_paged_prompt(a, dim_, max_rows, scratch_.as<char>() + prompt_scratch_, sms_, st);
         if (a.few_rows) tq::launch_paged_attention(a, dim_, static_cast<int>(std::min<long>(max_rows, kFewRows)), scratch_.as<void>(), sms_, st);
     }
     void check_status() {

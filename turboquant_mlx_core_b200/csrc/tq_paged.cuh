@@ -157,7 +157,7 @@ size_t paged_attn_scratch_bytes(int dim, int sms);
 void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratch, int sms, cudaStream_t st);
 // The others (tq_paged_prompt.cu).
 size_t paged_prompt_scratch_bytes(int dim, int sms);
-void launch_paged_prompt(PagedAttnArgs a, int dim, void* scratch, int sms, cudaStream_t st);
+void launch_paged_prompt(PagedAttnArgs a, int dim, long max_rows, void* scratch, int sms, cudaStream_t st);
 
 // ---- what the attention kernels share -------------------------------------------------------------
 namespace paged_device {

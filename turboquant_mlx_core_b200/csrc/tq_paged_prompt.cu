@@ -10,7 +10,7 @@
 //   O_t [128 x D]   += P_t (tensor memory) . V (shared memory, transposed: rows are dims)
 //
 //   warps 0-3, 4-7   tile 0, tile 1: a thread per row reads its scores twice (largest one; weights) and writes its result
-//   warps 8, 9       one lane issues the products of tile 0, tile 1; a commit behind S_t(j + 1) also says that O_t += P_t(j) V(j) is done, so that the softmax may
+//   warps 8, 9       one lane issues the scores' products, the values'; a commit behind S_t(j + 1) also says that O_t += P_t(j) V(j) is done, so that the softmax may
 //                    rescale O without a barrier of its own.  The products of the next item's first scores follow the last of this one's without a
 //                    pause, while the softmax warps still write the results
 //   warp 10          walks the CTA's share and tells the others, item by item, what is next (four items ahead at most)
@@ -258,7 +258,7 @@ constexpr int kSegments = 4;
 constexpr int kSegmentReaders = 30;   // warps: softmax, products, queries, keys, values
 
 struct Bars {
-    unsigned long long q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2], o_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], seg_full[kSegments], seg_empty[kSegments], done[2];
+    unsigned long long q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], o_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], seg_full[kSegments], seg_empty[kSegments], done[2];
 };
 
 // The larger of powers of two and zeros by their bits, of those that are numbers.
@@ -301,16 +301,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             for (int b = 0; b < 2; ++b) {
                 bar_init(bar(s_bar.s_full[k][b]), 1);
                 bar_init(bar(s_bar.p_full[k][b]), 4);
+                bar_init(bar(s_bar.o_done[k][b]), 1);
             }
-            bar_init(bar(s_bar.o_done[k]), 1);
             bar_init(bar(s_bar.o_empty[k]), 4);
             bar_init(bar(s_bar.done[k]), 1);
         }
         for (int k = 0; k < kStages; ++k) {
             bar_init(bar(s_bar.k_full[k]), 4);
-            bar_init(bar(s_bar.k_empty[k]), 2);
+            bar_init(bar(s_bar.k_empty[k]), 1);
             bar_init(bar(s_bar.v_full[k]), 4);
-            bar_init(bar(s_bar.v_empty[k]), 2);
+            bar_init(bar(s_bar.v_empty[k]), 1);
         }
         for (int k = 0; k < kSegments; ++k) {
             bar_init(bar(s_bar.seg_full[k]), 1);
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         const float down = jump ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
                         const float vnew = fmaxf(vref, vt), both = vnew > 0.f ? down * (vref / vnew) : 0.f;
                         if (j > 0) {
-                            if (!wait(s_bar.o_done[t], (n - 1) & 1)) break;
+                            if (!wait(s_bar.o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
                             fence_after();
 #pragma unroll 1
                             for (int q = 0; q < D; q += 16) {
@@ -450,16 +450,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     const float2 both_sums = unpack2(add2(sums[0], sums[1]));
                     const float sum = both_sums.x + both_sums.y;
                     l = fmaf(sum, exp2_approx(-lower), l);
-                    // P V of the tile before is done by now, mostly; every tile waits for it, so that the barrier is never two phases on.  (That of the one before it is: the
-                    // scores of this tile came behind it.)
-                    if (n > 0 && !wait(s_bar.o_done[t], (n - 1) & 1)) break;
                     tmem_st_wait();
                     fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(bar(s_bar.p_full[t][n & 1]));
                 }
                 done += tiles;
-                if (wait(s_bar.o_done[t], (done - 1) & 1)) {
+                if (wait(s_bar.o_done[t][(done - 1) & 1], ((done - 1) >> 1) & 1)) {
                     fence_after();
                     const bool begins = at.begins, ends = at.ends;
                     const float unit = vref * (1.f / kHeadroom);
@@ -512,9 +509,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         give_registers<kMmaRegs>();
         constexpr uint32_t kIdescS = instr_desc(kTokens), kIdescO = instr_desc(D);
         if (warp < kScheduleWarp && elect_one()) {
-            // One thread for each of the two tiles: a commit holds its thread up until the products in front are done, and what comes between it and the next
-            // product is beside the other tile's products then.  (One thread for both: 3.7 thousand cycles a unit with nothing else to do, of which the products take 2.1.)
-            const int t = warp - kMmaWarp;
+            // One thread for the scores, up to two tiles of the cache ahead, one for P V: a commit holds its thread up until the products in front are done, and what comes between it and
+            // the next product is beside the other thread's products then.  (One thread for all: 3.7 thousand cycles for 128 tokens with nothing else to do, of which the products take 2.1; one
+            // for each row tile, with 35 rows in one tile: 2.7 thousand cycles for 64 tokens.)
+            const bool first = warp == kMmaWarp;
             bool go = true;
             auto until = [&](unsigned long long& b, uint32_t phase) {
                 if (go && !bar_wait(smem_addr(&b), phase, flag)) {
@@ -523,83 +521,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 }
                 return go;
             };
-            auto ready = [&](unsigned long long& b, uint32_t phase) {
-                uint32_t done;
-                asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(smem_addr(&b)), "r"(phase) : "memory");
-                return done != 0;
-            };
-            const uint64_t q_desc = smem_desc(base + S::kQ + t * S::kQBytes, S::kRowGroup), k_desc = smem_desc(base + S::kK, S::kRowGroup), v_desc = smem_desc(base + S::kV, S::kDimGroup);
-            const uint32_t t_s = tmem + t * 2 * kTokens, t_o = tmem + 4 * kTokens + t * D;
-            // Scores run up to two tiles of the cache ahead of P V.  s_...: where they are (segment, tile in it, tiles of it, whether it has a tile t).
-            uint32_t q_n = 0, o_n = 0, kc = 0, vc = 0, s_n = 0, p_n = 0, ahead = 0;   // s_n, p_n: scores and P V of this tile so far; ahead: the share's tiles
-            uint32_t s_seg_n = 0;
-            until(s_bar.seg_full[0], 0);
-            int s_tiles = s_seg[0].tiles, s_j = 0;
-            bool s_mine = t == 0 || s_seg[0].two();
-            int tiles = s_tiles, j = 0;
-            bool mine = s_mine;
-            while (go && tiles > 0) {
-                while (ahead < 2 && s_tiles > 0) {
-                    // With a P V to do meanwhile nothing is waited for.
-                    const bool first = s_mine && s_j == 0;
-                    if (ahead > 0 && !(ready(s_bar.k_full[kc % kStages], (kc / kStages) & 1) && (!first || ready(s_bar.q_full[t], q_n & 1)))) break;
-                    if (!until(s_bar.k_full[kc % kStages], (kc / kStages) & 1)) break;
-                    const bool last = s_j + 1 == s_tiles;
-                    if (s_mine) {
-                        if (first && !until(s_bar.q_full[t], q_n++ & 1)) break;
-                        fence_after();
-                        const uint64_t k = k_desc + (kc % kStages) * (S::kKBytes >> 4);
-                        const uint32_t to = t_s + (s_n & 1) * kTokens;
+            const uint64_t q_desc = smem_desc(base + S::kQ, S::kRowGroup), k_desc = smem_desc(base + S::kK, S::kRowGroup), v_desc = smem_desc(base + S::kV, S::kDimGroup);
+            uint32_t turns = 0, items = 0, n[2] = {0, 0};   // tiles of the cache; items of each row tile (a bit each, the parity); scores, or P V, of each row tile
+            while (until(s_bar.seg_full[seg_n % kSegments], (seg_n / kSegments) & 1)) {
+                const int tiles = s_seg[seg_n % kSegments].tiles, pair = s_seg[seg_n % kSegments].two() ? 2 : 1;
+                if (tiles == 0) break;
+#pragma unroll 1
+                for (int j = 0; j < tiles; ++j, ++turns) {
+                    const uint32_t stage = turns % kStages, turn = (turns / kStages) & 1;
+                    if (!until(first ? s_bar.k_full[stage] : s_bar.v_full[stage], turn)) break;
 #pragma unroll
-                        for (int s = 0; s < D / 16; ++s) umma_ss(to, q_desc + 16 * s, k + 16 * s, kIdescS, s > 0);
-                        umma_commit(bar(s_bar.s_full[t][s_n & 1]));
-                        umma_commit(bar(s_bar.k_empty[kc % kStages]));
-                        if (last) umma_commit(bar(s_bar.q_empty[t]));
-                        ++s_n;
-                    } else {
-                        bar_arrive(bar(s_bar.k_empty[kc % kStages]));
-                    }
-                    ++kc;
-                    ++ahead;
-                    ++s_j;
-                    if (last) {
-                        ++s_seg_n;
-                        if (!until(s_bar.seg_full[s_seg_n % kSegments], (s_seg_n / kSegments) & 1)) break;
-                        s_tiles = s_seg[s_seg_n % kSegments].tiles;
-                        s_mine = t == 0 || s_seg[s_seg_n % kSegments].two();
-                        s_j = 0;
-                    }
-                }
-                if (!go || !until(s_bar.v_full[vc % kStages], (vc / kStages) & 1)) break;
-                const bool last = j + 1 == tiles;
-                if (mine) {
-                    if (j == 0 && !until(s_bar.o_empty[t], (o_n++ & 1) ^ 1)) break;
-                    if (!until(s_bar.p_full[t][p_n & 1], (p_n >> 1) & 1)) break;
-                    fence_after();
-                    const uint64_t v = v_desc + (vc % kStages) * (S::kVBytes >> 4);
-                    const uint32_t from = t_s + (p_n & 1) * kTokens;
+                    for (int t = 0; t < 2; ++t) {
+                        if (t >= pair) continue;
+                        const uint32_t place = n[t] & 1, t_s = tmem + (2 * t + place) * kTokens;
+                        if (first) {
+                            if (j == 0 && !until(s_bar.q_full[t], (items >> t) & 1)) break;
+                            // P of two tiles before was where these scores go
+                            if (n[t] >= 2 && !until(s_bar.o_done[t][place], ((n[t] >> 1) - 1) & 1)) break;
+                            fence_after();
+                            const uint64_t q = q_desc + t * (S::kQBytes >> 4), k = k_desc + stage * (S::kKBytes >> 4);
 #pragma unroll
-                    for (int s = 0; s < kTokens / 16; ++s) umma_ts(t_o, from + 8 * s, v + 16 * s, kIdescO, j > 0 || s > 0);
-                    umma_commit(bar(s_bar.o_done[t]));
-                    umma_commit(bar(s_bar.v_empty[vc % kStages]));
-                    ++p_n;
-                } else {
-                    bar_arrive(bar(s_bar.v_empty[vc % kStages]));
+                            for (int s = 0; s < D / 16; ++s) umma_ss(t_s, q + 16 * s, k + 16 * s, kIdescS, s > 0);
+                            umma_commit(bar(s_bar.s_full[t][place]));
+                            if (j + 1 == tiles) umma_commit(bar(s_bar.q_empty[t]));
+                        } else {
+                            if (j == 0 && !until(s_bar.o_empty[t], ((items >> t) & 1) ^ 1)) break;
+                            if (!until(s_bar.p_full[t][place], (n[t] >> 1) & 1)) break;
+                            fence_after();
+                            const uint64_t v = v_desc + stage * (S::kVBytes >> 4);
+#pragma unroll
+                            for (int s = 0; s < kTokens / 16; ++s) umma_ts(tmem + 4 * kTokens + t * D, t_s + 8 * s, v + 16 * s, kIdescO, j > 0 || s > 0);
+                            umma_commit(bar(s_bar.o_done[t][place]));
+                        }
+                        ++n[t];
+                    }
+                    if (!go) break;
+                    umma_commit(bar(first ? s_bar.k_empty[stage] : s_bar.v_empty[stage]));
                 }
-                ++vc;
-                --ahead;
-                ++j;
-                if (last) {
-                    bar_arrive(bar(s_bar.seg_empty[seg_n % kSegments]));
-                    ++seg_n;
-                    // (the scores are a segment ahead at least, or at the end with it)
-                    if (!until(s_bar.seg_full[seg_n % kSegments], (seg_n / kSegments) & 1)) break;
-                    tiles = s_seg[seg_n % kSegments].tiles;
-                    mine = t == 0 || s_seg[seg_n % kSegments].two();
-                    j = 0;
-                }
+                items ^= pair == 2 ? 3u : 1u;
+                bar_arrive(bar(s_bar.seg_empty[seg_n % kSegments]));
+                ++seg_n;
             }
             if (!go) {   // what was issued ends before the tensor memory goes
+                const int t = warp - kMmaWarp;
                 umma_commit(bar(s_bar.done[t]));
                 unsigned int never = 0;
                 bar_wait(bar(s_bar.done[t]), 0, &never);
@@ -848,13 +812,14 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) paged_prompt_join_kernel(co
 }
 
 template <int D>
-void launch_typed(PagedAttnArgs a, void* scratch, int sms, cudaStream_t st) {
+void launch_typed(PagedAttnArgs a, long max_rows, void* scratch, int sms, cudaStream_t st) {
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (sms * sizeof(PagedJoin) + 255) / 256 * 256);
     static std::atomic<unsigned long long> set{0};
     allow_shared_memory(paged_prompt_kernel<D>, Shape<D>::kSmem, set);
     launch_pdl_carved(paged_prompt_kernel<D>, dim3(static_cast<unsigned int>(sms)), dim3(kThreads), Shape<D>::kSmem, 100, st, a);
-    launch_pdl_carved(paged_prompt_join_kernel<D>, dim3(static_cast<unsigned int>(sms), kPairRows / kJoinRows), dim3(kJoinRows * D / 4), 0, 100, st, a);
+    launch_pdl_carved(paged_prompt_join_kernel<D>, dim3(static_cast<unsigned int>(sms), static_cast<unsigned int>((std::min<long>(kPairRows, max_rows) + kJoinRows - 1) / kJoinRows)),
+                      dim3(kJoinRows * D / 4), 0, 100, st, a);
 }
 
 }  // namespace
@@ -862,9 +827,9 @@ void launch_typed(PagedAttnArgs a, void* scratch, int sms, cudaStream_t st) {
 size_t paged_prompt_scratch_bytes(int dim, int sms) {
     return (sms * sizeof(PagedJoin) + 255) / 256 * 256 + static_cast<size_t>(sms) * 2 * kPairRows * (static_cast<size_t>(dim) + 2) * sizeof(float);
 }
-void launch_paged_prompt(PagedAttnArgs a, int dim, void* scratch, int sms, cudaStream_t st) {
-    if (dim == 64) launch_typed<64>(a, scratch, sms, st);
-    else launch_typed<128>(a, scratch, sms, st);
+void launch_paged_prompt(PagedAttnArgs a, int dim, long max_rows, void* scratch, int sms, cudaStream_t st) {
+    if (dim == 64) launch_typed<64>(a, max_rows, scratch, sms, st);
+    else launch_typed<128>(a, max_rows, scratch, sms, st);
 }
 
 }  // namespace tq
