@@ -1,18 +1,17 @@
 // Attention over the paged 8-bit KV cache for many query rows of a request: prompts, chunks of them, drafts of several
-// tokens.  Bound by the tensor cores and the exponentials; the products are tcgen05.mma with S, P and O in tensor memory.
+// tokens.  The products are tcgen05.mma with S, P and O in tensor memory.
 //
 // The rows of a request and KV head (new tokens times the heads of the group, token-major) go in items of 256: two tiles of 128, whose softmaxes run in
-// turn with each other's products.  The cache comes in tiles of 128 tokens.  As in tq_paged_attention.cu every CTA, one to an SM, takes an equal share of
-// all (request, KV head, 256 rows, 128 tokens) units, an item's beginning and end counted as two more, and an item that ends in another CTA than it begins in is added up behind.
+// turn with each other's products.  The cache comes in tiles of 64 tokens.  As in tq_paged_attention.cu every CTA, one to an SM, takes an equal share of
+// all (request, KV head, 256 rows, 64 tokens) units, an item's beginning and end counted as kItemUnits more, and an item that ends in another CTA than it begins in is added up behind.
 //
-//   S_t [128 x 128]  = Q_t [128 x D] (shared memory) . K [128 x D]^T (shared memory)        fp16 products, fp32 sums
+//   S_t [128 x 64]   = Q_t [128 x D] (shared memory) . K [64 x D]^T (shared memory)         fp16 products, fp32 sums; two of them in turn for each t
 //   P_t              = 2^(S_t f - m + 11)  fp16, over S_t's own columns of tensor memory
 //   O_t [128 x D]   += P_t (tensor memory) . V (shared memory, transposed: rows are dims)
 //
-//   warps 0-3, 4-7   tile 0, tile 1: a thread per row reads its scores twice (largest one; weights) and writes its result
-//   warps 8, 9       one lane issues the scores' products, the values'; a commit behind S_t(j + 1) also says that O_t += P_t(j) V(j) is done, so that the softmax may
-//                    rescale O without a barrier of its own.  The products of the next item's first scores follow the last of this one's without a
-//                    pause, while the softmax warps still write the results
+//   warps 0-3, 4-7   tile 0, tile 1: a thread per row reads its 64 scores once, keeps them in registers for the largest one and the weights, and writes its result
+//   warps 8, 9       one lane issues the scores' products, the values'; the commit behind P_t(j) V(j) also says that O_t may be rescaled, and that the scores of two tiles on may go where
+//                    P_t(j) was.  The products of the next item's first scores follow the last of this one's without a pause, while the softmax warps still write the results
 //   warp 10          walks the CTA's share and tells the others, item by item, what is next (four items ahead at most)
 //   warps 12-15      queries of tile 0, tile 1, of the next item as soon as the last scores of this one are there
 //   warps 16-23      keys: bytes to shared memory a tile ahead, then as halves (code * 2^(e - e_max + 5), exact) to their place for the products
@@ -21,6 +20,13 @@
 // Scales are powers of two: within a tile the pages' go into the halves without a rounding (but for codes 2^29 below the tile's largest scale), the tile's own goes into the
 // exponent's factor (keys) or, as an integer, into the exponent (values: P V is kept in units of the largest scale so far).  The reference maximum m
 // moves only when a score exceeds it by 2^4, which rarely happens after the first tiles; weights are at most 2^15 then.
+//
+// What bounds it: 256 rows against 64 tokens (D = 128) take 2.7 thousand cycles.  A softmax warp is at work for 2.3 of them, 8 % wait; the products alone would take 1.24 (the scores'
+// 64 columns read 6 KB of shared memory in the 32 cycles that their arithmetic takes, 48 in fact), the exponentials alone 1.02, the softmax of both tiles with nothing beside it 1.17, all
+// roles' instructions fill 54 % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 178 us, 0.68 PFLOP/s of the
+// causal products, 41 % of a plain matrix product's rate.  Tried beside it, of the same prompt when it took 183: scores read twice in loops of 32 columns, a third less code, 191; two warps to a
+// row's 64 scores and half as many for the conversions 195; keys and values two tiles ahead 185.  Tiles of 128 tokens with one set of scores and one thread for all products: 699 for 8192 tokens, 668
+// with these.
 //
 // Every wait is bounded; a warp that gives up flags it, all warps fall through to the end, where the tensor memory is freed.
 #include <algorithm>
@@ -380,10 +386,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const int token = at.start + in_row / a.group, hq = at.head * a.group + in_row % a.group, pos = at.first + in_row / a.group;
                 const bool live = row < at.rows;
                 const int oldest = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+                const bool idle = at.row0 + t * kRows + 32 * (warp & 3) >= at.rows;   // a warp without rows: it keeps the others' count (16 requests of 35 rows: 48 us, 56 with the softmax of what is not there)
                 float m = -INFINITY, l = 0.f, vref = 0.f;
                 for (int j = 0; j < tiles; ++j) {
                     const uint32_t ref = (count + j) & (kRefs - 1), n = done + j;
                     if (!wait(s_bar.s_full[t][n & 1], (n >> 1) & 1)) break;
+                    if (idle) {
+                        if (lane == 0) bar_arrive(bar(s_bar.p_full[t][n & 1]));
+                        continue;
+                    }
                     fence_after();
                     const uint32_t t_s = t_s0 + (n & 1) * kTokens;
                     uint32_t x[32], y[32];
@@ -579,9 +590,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const Segment& at = s_seg[seg_n % kSegments];
                 if (t == 1 && !at.two()) continue;
                 if (!wait(s_bar.q_empty[t], (q_n++ & 1) ^ 1)) break;
+                // Rows behind the last: zeros beside live ones of a softmax warp, what is there for warps without.  (With the last row in their place 148 CTAs asked the same place of the
+                // L2 cache for it a hundred times each, 20 us for a request of 35 rows.)
+                const int rows_here = min(kRows, at.rows - at.row0 - t * kRows), live = (rows_here + 7) / 8, groups = (rows_here + 31) / 32 * 4;
                 uint8_t* const dst = s_mem + S::kQ + t * S::kQBytes + (lane & 7) * 16 + (lane >> 3) * 128;
 #pragma unroll 1
-                for (int g = part; g < kRows / 8; g += 2) {
+                for (int g = part; g < live; g += 2) {
                     const int row = min(at.row0 + t * kRows + 8 * g + (lane & 7), at.rows - 1);   // (rows behind the last: the last again, nobody reads their results)
                     const int token = row / a.group, hq = at.head * a.group + row - token * a.group;
                     const __half* const src = a.q + (at.start + token) * a.q_stride + static_cast<long>(hq) * D + 8 * (lane >> 3);
@@ -595,6 +609,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         }
                     }
                 }
+                for (int g = live + ((live ^ part) & 1); g < groups; g += 2)
+                    for (int k = 0; k < D / 32; ++k) *reinterpret_cast<uint4*>(dst + g * S::kRowGroup + 4 * k * 128) = make_uint4(0u, 0u, 0u, 0u);
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 publish_smem();
                 __syncwarp();
@@ -762,53 +778,84 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     }
 }
 
-// Parts of the items that several CTAs share, in the CTAs' order: a thread takes four dims of a row, eight rows to a CTA.
+// Parts of the items that several CTAs share, in the CTAs' order: a thread takes four dims of ROWS rows, eight rows apart.  Bound by the latency of its loads (entry, parts, one behind
+// the other), so what a thread reads is on its way at once: two parts of four rows where items are full (a prompt, 148 items of two parts, 38 MB: 7 us less than a row at a
+// time), eight parts of a row where they are not (few rows over a long cache, cut into many).
 constexpr int kJoinRows = 8;
-template <int D>
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kJoinRows * D / 4) paged_prompt_join_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int kPart = Shape<D>::kPart;
     pdl_wait_release();
     const PagedJoin join = a.joins[blockIdx.x];
-    const int c = blockIdx.x, r = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, d4 = threadIdx.x / kJoinRows;
-    if (join.last == 0 || r >= join.rows) return;
+    const int c = blockIdx.x, r0 = blockIdx.y * (kJoinRows * ROWS) + threadIdx.x % kJoinRows, d4 = threadIdx.x / kJoinRows;
+    if (join.last == 0 || r0 >= join.rows) return;
     const int parts = join.last - c + 1;
     auto part_of = [&](int k) { return a.partial + (2 * (c + k) + (k == 0 ? 1 : 0)) * static_cast<long>(kPart); };
-    float top = -INFINITY, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int base = 0; base < parts; base += 2) {
-        float2 ml[2];
-        float4 v[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float* const p = part_of(min(base + k, parts - 1));
-            ml[k] = *reinterpret_cast<const float2*>(p + kPairRows * D + 2 * r);
-            v[k] = *reinterpret_cast<const float4*>(p + (d4 * kPairRows + r) * 4);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (base + k >= parts) continue;
-            const float to = fmaxf(top, ml[k].x);
-            const float x = top == to || top == -INFINITY ? 1.f : exp2_approx(top - to), y = ml[k].x == to || ml[k].x == -INFINITY ? 1.f : exp2_approx(ml[k].x - to);
+    struct Sum {
+        float top, sum;
+        float4 acc;
+        __device__ __forceinline__ void add(float2 ml, float4 v) {
+            const float to = fmaxf(top, ml.x);
+            const float x = top == to || top == -INFINITY ? 1.f : exp2_approx(top - to), y = ml.x == to || ml.x == -INFINITY ? 1.f : exp2_approx(ml.x - to);
             top = to;
-            sum = sum * x + ml[k].y * y;
-            acc.x = acc.x * x + v[k].x * y;
-            acc.y = acc.y * x + v[k].y * y;
-            acc.z = acc.z * x + v[k].z * y;
-            acc.w = acc.w * x + v[k].w * y;
+            sum = sum * x + ml.y * y;
+            acc.x = acc.x * x + v.x * y;
+            acc.y = acc.y * x + v.y * y;
+            acc.z = acc.z * x + v.z * y;
+            acc.w = acc.w * x + v.w * y;
         }
+    };
+    auto load = [&](int k, int r, float2& ml, float4& v) {
+        const float* const p = part_of(k);
+        ml = *reinterpret_cast<const float2*>(p + kPairRows * D + 2 * r);
+        v = *reinterpret_cast<const float4*>(p + (d4 * kPairRows + r) * 4);
+    };
+    auto store = [&](int r, const Sum& s) {
+        const float inv = 1.f / s.sum;
+        const int row = join.first_row + r, token = row / a.group, hq = join.head * a.group + row - token * a.group;
+        __half* const dst = a.out + (join.token + token) * a.out_stride + static_cast<long>(hq) * D + 4 * d4;
+        const uint2 four = make_uint2(pack_half2(s.acc.x * inv, s.acc.y * inv), pack_half2(s.acc.z * inv, s.acc.w * inv));
+        if (reinterpret_cast<uintptr_t>(dst) % 8 == 0) *reinterpret_cast<uint2*>(dst) = four;
+        else {
+            dst[0] = __ushort_as_half(static_cast<unsigned short>(four.x));
+            dst[1] = __ushort_as_half(static_cast<unsigned short>(four.x >> 16));
+            dst[2] = __ushort_as_half(static_cast<unsigned short>(four.y));
+            dst[3] = __ushort_as_half(static_cast<unsigned short>(four.y >> 16));
+        }
+        if (a.lse && d4 == 0) a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (s.top - kOffset + log2f(s.sum)) * 0.6931471805599453f;
+    };
+    const Sum none{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    if (ROWS > 1 && parts == 2) {
+        float2 ml[ROWS][2];
+        float4 v[ROWS][2];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) load(k, min(r0 + kJoinRows * i, join.rows - 1), ml[i][k], v[i][k]);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            if (r0 + kJoinRows * i >= join.rows) break;
+            Sum s = none;
+            s.add(ml[i][0], v[i][0]);
+            s.add(ml[i][1], v[i][1]);
+            store(r0 + kJoinRows * i, s);
+        }
+        return;
     }
-    const float inv = 1.f / sum;
-    const int row = join.first_row + r, token = row / a.group, hq = join.head * a.group + row - token * a.group;
-    __half* const dst = a.out + (join.token + token) * a.out_stride + static_cast<long>(hq) * D + 4 * d4;
-    const uint2 four = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
-    if (reinterpret_cast<uintptr_t>(dst) % 8 == 0) *reinterpret_cast<uint2*>(dst) = four;
-    else {
-        dst[0] = __ushort_as_half(static_cast<unsigned short>(four.x));
-        dst[1] = __ushort_as_half(static_cast<unsigned short>(four.x >> 16));
-        dst[2] = __ushort_as_half(static_cast<unsigned short>(four.y));
-        dst[3] = __ushort_as_half(static_cast<unsigned short>(four.y >> 16));
+#pragma unroll 1
+    for (int r = r0; r < min(join.rows, r0 + kJoinRows * ROWS); r += kJoinRows) {
+        Sum s = none;
+        for (int base = 0; base < parts; base += 8) {
+            float2 ml[8];
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) load(min(base + k, parts - 1), r, ml[k], v[k]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (base + k < parts) s.add(ml[k], v[k]);
+        }
+        store(r, s);
     }
-    if (a.lse && d4 == 0) a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(sum)) * 0.6931471805599453f;
 }
 
 template <int D>
@@ -818,8 +865,11 @@ void launch_typed(PagedAttnArgs a, long max_rows, void* scratch, int sms, cudaSt
     static std::atomic<unsigned long long> set{0};
     allow_shared_memory(paged_prompt_kernel<D>, Shape<D>::kSmem, set);
     launch_pdl_carved(paged_prompt_kernel<D>, dim3(static_cast<unsigned int>(sms)), dim3(kThreads), Shape<D>::kSmem, 100, st, a);
-    launch_pdl_carved(paged_prompt_join_kernel<D>, dim3(static_cast<unsigned int>(sms), static_cast<unsigned int>((std::min<long>(kPairRows, max_rows) + kJoinRows - 1) / kJoinRows)),
-                      dim3(kJoinRows * D / 4), 0, 100, st, a);
+    const auto join = [&](auto kernel, int rows) {
+        launch_pdl_carved(kernel, dim3(static_cast<unsigned int>(sms), static_cast<unsigned int>((std::min<long>(kPairRows, max_rows) + rows - 1) / rows)), dim3(kJoinRows * D / 4), 0, 100, st, a);
+    };
+    if (max_rows >= kPairRows) join(paged_prompt_join_kernel<D, 4>, 4 * kJoinRows);
+    else join(paged_prompt_join_kernel<D, 1>, kJoinRows);
 }
 
 }  // namespace
