@@ -205,8 +205,8 @@ public:
     }
 
 private:
-    // Query rows of a request (new tokens times query heads to a KV head) that the kernel for few rows takes: 14 rows of 16 requests over 4096 tokens 31 us there, 50 in the other one;
-    // 21 rows, which it would read the cache for twice, 48 and 50; 20 rows of 4 requests over 32768 tokens 132 and 135; 35 rows, three times, 52 and 49.
+    // Query rows of a request (new tokens times query heads to a KV head) that the kernel for few rows takes, 16 at a time.  Over 4096 tokens of 16 requests, there and in the kernel for many:
+    // 14 rows 32 and 49 us, 21 rows 48 and 48, 35 rows 67 and 49; 20 rows over 32768 tokens of 4 requests 132 and 132.
     static constexpr int kFewRows = 16;
 
     void check_layer(int layer) const { TQ_REQUIRE(layer >= 0 && layer < static_cast<int>(layers_.size()), "Layer index out of range"); }
