@@ -135,13 +135,13 @@ def bounds(x, k, v, w, o, lse, scale, seen):
     A score is a sum of D exact products, added in fp32 (an addition may lose two units of 2^-24 of the partial sums' magnitude, at
     most sum |q||k|), then two roundings and the exponential's two units: relative error of a weight, against the others,
     a = 2 (D + 8) 2^-24 scale max sum |q||k| + 2^-20.  Weights are rounded to halves: 2^-11 of each.  Small ones are
-    subnormal halves, multiples of 2^-24 and so 2^-25 off at most; the kernels hold weights times 2^11, against a
-    maximum that is no larger than the row's: 2^-36 of the largest weight at most, n 2^-36 max |v| of the sum.  The sums of n terms in fp32: 2 n 2^-24 at worst, of sum w|v|; n 2^-24 for the denominator.
+    subnormal halves, multiples of 2^-24 and so 2^-25 off at most; the kernels hold weights times 2^11 (few rows) or 2^7 (many), against a
+    maximum that is no larger than the row's: 2^-25-7 = 2^-32 of the largest weight at most, n 2^-32 max |v| of the sum.  The sums of n terms in fp32: 2 n 2^-24 at worst, of sum w|v|; n 2^-24 for the denominator.
     The result is rounded to a half: 2^-11 of it, or 2^-25 where it is subnormal."""
     d, n = k.shape[1], k.shape[0]
     reach = (np.where(seen, np.abs(x) @ np.abs(k).T, 0)).max(1) * scale
     a = (2 * (d + 8) * 2.0 ** -24 * reach + 2.0 ** -20)[:, None]
     mass = w @ np.abs(v)
     near = np.where(seen[:, :, None], np.abs(v)[None], 0).max((0, 1)) if v.size < 1 << 22 else np.abs(v).max(0)
-    before = mass * (2.0 ** -11 + 2 * a + 3 * n * 2.0 ** -24) + n * 2.0 ** -36 * near
+    before = mass * (2.0 ** -11 + 2 * a + 3 * n * 2.0 ** -24) + n * 2.0 ** -32 * near
     return (np.abs(o) + before) * 2.0 ** -11 + 2.0 ** -25 + before, 2 * a[:, 0] + n * 2.0 ** -24 + 2.0 ** -22 * (np.abs(lse) + 16)

@@ -6,7 +6,7 @@
 // all (request, KV head, 256 rows, 64 tokens) units, an item's beginning and end counted as kItemUnits more, and an item that ends in another CTA than it begins in is added up behind.
 //
 //   S_t [128 x 64]   = Q_t [128 x D] (shared memory) . K [64 x D]^T (shared memory)         fp16 products, fp32 sums; two of them in turn for each t
-//   P_t              = 2^(S_t f - m + 11)  fp16, over S_t's own columns of tensor memory
+//   P_t              = 2^(S_t f - m + 7)  fp16, over S_t's own columns of tensor memory
 //   O_t [128 x D]   += P_t (tensor memory) . V (shared memory, transposed: rows are dims)
 //
 //   warps 0-3, 4-7   tile 0, tile 1: a thread per row reads its 64 scores once, keeps them in registers for the largest one and the weights, and writes its result
@@ -19,11 +19,13 @@
 //
 // Scales are powers of two: within a tile the pages' go into the halves without a rounding (but for codes 2^29 below the tile's largest scale), the tile's own goes into the
 // exponent's factor (keys) or, as an integer, into the exponent (values: P V is kept in units of the largest scale so far).  The reference maximum m
-// moves only when a score exceeds it by 2^4, which rarely happens after the first tiles; weights are at most 2^15 then.
+// moves only when a score exceeds it by 2^8; weights are at most 2^15 then.  Where keys are of unequal strength one of a warp's 32 rows often has such a score (simulated, with norms spread by e^0.5: in 12 of
+// 63 tiles, in 19 with 2^4), and its O is then read, multiplied and written back, behind the weights, so that the products before it end meanwhile: 4096 such tokens 181 us, 190 with 2^4,
+// 199 with that and O in front of the weights; 175 where no row moves.
 //
 // What bounds it: 256 rows against 64 tokens (D = 128) take 2.7 thousand cycles.  A softmax warp is at work for 2.3 of them, 8 % wait; the products alone would take 1.24 (the scores'
 // 64 columns read 6 KB of shared memory in the 32 cycles that their arithmetic takes, 48 in fact), the exponentials alone 1.02, the softmax of both tiles with nothing beside it 1.17, all
-// roles' instructions fill 54 % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 178 us, 0.68 PFLOP/s of the
+// roles' instructions fill 54 % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 175 us, 0.69 PFLOP/s of the
 // causal products, 41 % of a plain matrix product's rate.  Tried beside it, of the same prompt when it took 183: scores read twice in loops of 32 columns, a third less code, 191; two warps to a
 // row's 64 scores and half as many for the conversions 195; keys and values two tiles ahead 185.  Tiles of 128 tokens with one set of scores and one thread for all products: 699 for 8192 tokens, 668
 // with these.
@@ -54,8 +56,9 @@ constexpr int kWarpTokens = 16;      // of a tile's tokens that a warp turns int
 constexpr int kItemUnits = 4;        // what an item's beginning and end cost, in units
 constexpr int kStages = 4;           // of keys and of values, as halves
 constexpr int kRefs = 8;             // tiles whose scales are kept
-// Weights are held times 2^11, and at most 2^15: halves that are normal numbers down to 2^-25 of the reference, and 2^-36 of it off below.
-constexpr float kOffset = 11.f, kSlack = 4.f;
+// Weights are held times 2^7, and at most 2^15: halves that are normal numbers down to 2^-21 of the reference, and 2^-32 of it off below: of 131072 tokens' values 2^-15 of the largest one
+// at the very worst, 1/16 of the result's rounding.
+constexpr float kOffset = 7.f, kSlack = 8.f;
 constexpr float kHeadroom = 32.f;    // largest factor of a code in the halves
 constexpr uint32_t kTmemAll = 512;
 
@@ -125,18 +128,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
             "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
-                   "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                   "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-                 :
-                 : "memory");
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        : : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+            "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+            "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -418,23 +418,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     top *= f;   // (f is positive; NaN columns do not count)
                     const bool jump = top > m + kSlack || (m == -INFINITY && top > m);
-                    if (__any_sync(0xffffffffu, jump || vt > vref)) {
+                    float both = 1.f;
+                    const bool moves = __any_sync(0xffffffffu, jump || vt > vref);
+                    if (moves) {
                         const float to = jump ? top : m;
                         const float down = jump ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
-                        const float vnew = fmaxf(vref, vt), both = vnew > 0.f ? down * (vref / vnew) : 0.f;
-                        if (j > 0) {
-                            if (!wait(s_bar.o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
-                            fence_after();
-#pragma unroll 1
-                            for (int q = 0; q < D; q += 16) {
-                                uint32_t o[16];
-                                tmem_ld16(t_o + q, o);
-                                tmem_ld_wait16(o);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * both);
-                                tmem_st16(t_o + q, o);
-                            }
-                        }
+                        const float vnew = fmaxf(vref, vt);
+                        both = vnew > 0.f ? down * (vref / vnew) : 0.f;
                         l *= down;
                         m = to;
                         vref = vnew;
@@ -461,6 +451,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     const float2 both_sums = unpack2(add2(sums[0], sums[1]));
                     const float sum = both_sums.x + both_sums.y;
                     l = fmaf(sum, exp2_approx(-lower), l);
+                    if (moves && j > 0) {   // O to the new reference: behind the weights, which take as long as the products that it waits for
+                        if (!wait(s_bar.o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
+                        fence_after();
+#pragma unroll 1
+                        for (int q = 0; q < D; q += 32) {
+                            tmem_ld(t_o + q, x);
+                            tmem_ld_wait(x);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * both);
+                            tmem_st(t_o + q, x);
+                        }
+                    }
                     tmem_st_wait();
                     fence_before();
                     __syncwarp();
