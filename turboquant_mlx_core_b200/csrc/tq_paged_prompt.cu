@@ -406,10 +406,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     tmem_ld_wait(x);
                     tmem_ld_wait(y);
                     if (__any_sync(0xffffffffu, newest < kTokens - 1 || eldest > 0)) {
+                        // a bit for each column
+                        const uint64_t seen = (newest >= 63 ? ~0ull : newest < 0 ? 0ull : (2ull << newest) - 1) & (eldest <= 0 ? ~0ull : eldest > 63 ? 0ull : ~0ull << eldest);
+                        const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            if (e > newest || e < eldest) x[e] = 0xff800000u;   // (minus infinity, times f)
-                            if (32 + e > newest || 32 + e < eldest) y[e] = 0xff800000u;
+                            if (!(lo >> e & 1)) x[e] = 0xff800000u;   // (minus infinity, times f)
+                            if (!(hi >> e & 1)) y[e] = 0xff800000u;
                         }
                     }
                     float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
