@@ -580,7 +580,9 @@ int tq_paged_read(tq_paged_cache_t cache, int layer, const int* pages, int n, vo
  *  max(0, p - window + 1) .. p, all up to p with window 0.  q_heads is a multiple of the KV heads, whose groups are
  *  contiguous.  scale 0: 1 / sqrt(head_dim).  out fp16 of the queries' shape, strides in elements from token to token; lse
  *  (may be NULL): fp32 [tokens, q_heads], the log of each softmax denominator, with which parts merge
- *  (tq_exchange_merge_attention).  Rows behind the last request's are left as they are.  Results do not depend on the order in which CTAs run. */
+ *  (tq_exchange_merge_attention).  Rows behind the last request's are left as they are.  Results do not depend on the order in which CTAs run.  Where a
+ *  request has more than 16 query rows (new tokens times the group), the pages of 64 tokens in a row are taken together: numbers of a page whose scale is 2^29 below the largest
+ *  among them count as 0. */
 int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window,
                        float scale, void* out_fp16, long out_stride, float* lse, void* stream);
 /** Non-zero, once, when a call that has finished found its batch impossible or a wait on the device ran out. */

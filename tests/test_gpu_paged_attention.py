@@ -190,3 +190,69 @@ def test_results_repeat_to_the_bit(tq):
         again = run(c, q)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
     c.close()
+
+
+@pytest.mark.parametrize("last", [1, 9])
+@pytest.mark.parametrize("big", [2.0 ** 36, 2.0 ** 100])
+def test_values_of_any_size(tq, last, big):
+    """Most values are zeros, whose pages have the smallest scale there is, one is 2^130 or more above it: sums of weights are what they are without it."""
+    rng = np.random.default_rng(12)
+    dim, group, tokens = 64, 8, 40000     # (several tiles to a CTA)
+    c = tq.PagedKVCache(1, 1, dim, 640, 64, 1, 640, tokens)
+    m = Model(1, dim, 640, 64)
+    for count in (tokens, last):
+        k, v = rng.standard_normal((count, 1, dim)), np.zeros((count, 1, dim))
+        if count == tokens:
+            k[0, 0] = -4
+            v[0, 0] = big
+        k, v = k.astype(np.float32), v.astype(np.float32)
+        m.plan([count])
+        m.append(0, k)
+        m.append(1, v)
+        c.plan(np.array([count], np.int32))
+        c.append(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    q = (2 + 0.1 * rng.standard_normal((last, group, dim))).astype(np.float16)
+    out, lse = run(c, torch.from_numpy(q).cuda())
+    _, sums, _, ltol = m.attention(q)
+    assert (np.abs(lse.cpu().numpy() - sums) <= ltol).all() and not torch.isnan(out).any()
+    c.close()
+
+
+def test_scales_that_vanish(tq):
+    """Zero keys and a scale so small that their product is no number of 32 bits: equal weights, and masked tokens are out."""
+    c = tq.PagedKVCache(1, 1, 64, 4, 64, 1, 4, 200)
+    v = torch.arange(150, device="cuda").half()[:, None, None].expand(150, 1, 64).contiguous()
+    c.plan(np.array([150], np.int32))
+    c.append(0, torch.zeros_like(v), v)
+    q = torch.ones((150, 2, 64), dtype=torch.float16, device="cuda")
+    out, lse = run(c, q, scale=1e-30)
+    seen = torch.arange(150, device="cuda", dtype=torch.float64)
+    codes = torch.cat([torch.round(x / s) * s for x, s in ((seen[:64], 0.5), (seen[64:128], 1.0), (seen[128:], 2.0))])
+    mean = torch.cumsum(codes, 0) / (seen + 1)
+    # equal weights are halves exactly, sums of codes in halves below 2^16 exact; a division, a product and a half's rounding
+    assert (out.double() - mean[:, None, None]).abs().le(mean[:, None, None] * (2.0 ** -11 + 2.0 ** -22)).all()
+    # the logarithm of 2^7 n is below 16: a unit of 2^-20 off; the difference and the product with log 2 half a unit below 8 each, 2^-22
+    assert (lse.double() - torch.log(seen + 1)[:, None]).abs().le(2.0 ** -19).all()
+    c.close()
+
+
+@pytest.mark.parametrize("window", [0, 30])
+@pytest.mark.parametrize("large", [1e15, 3e38, -3e38])
+def test_large_numbers_that_are_not_seen(tq, window, large):
+    """Tokens from the 129th on are as large as they can be: the rows before them, in the same tile, are what they are without."""
+    rng = np.random.default_rng(13)
+    c = tq.PagedKVCache(1, 1, 128, 8, 64, 1, 8, 250)
+    m = Model(1, 128, 8, 64)
+    k, v = rng.standard_normal((250, 1, 128)).astype(np.float32), rng.standard_normal((250, 1, 128)).astype(np.float32)
+    k[128:] = v[128:] = large
+    m.plan([250])
+    c.plan(np.array([250], np.int32))
+    c.append(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    q = queries(rng, 250, 1, 128)
+    out, lse = run(c, torch.from_numpy(q).cuda(), window=window)
+    m = Model(1, 128, 8, 64)
+    m.plan([128])
+    m.append(0, k[:128])
+    m.append(1, v[:128])
+    compare(out[:128], lse[:128], m.attention(q[:128], window))
+    c.close()

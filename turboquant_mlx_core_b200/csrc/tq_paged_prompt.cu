@@ -59,6 +59,7 @@ constexpr int kRefs = 8;             // tiles whose scales are kept
 // Weights are held times 2^7, and at most 2^15: halves that are normal numbers down to 2^-21 of the reference, and 2^-32 of it off below: of 131072 tokens' values 2^-15 of the largest one
 // at the very worst, 1/16 of the result's rounding.
 constexpr float kOffset = 7.f, kSlack = 8.f;
+constexpr int kLeastLower = -60;     // of a tile's values against the largest so far: a weight times 2^-60 is 0 as a half, and their sum, which is taken of these, far from it
 constexpr float kHeadroom = 32.f;    // largest factor of a code in the halves
 constexpr uint32_t kTmemAll = 512;
 
@@ -401,8 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     tmem_ld(t_s, x);
                     tmem_ld(t_s + 32, y);
                     const int tb = (tile0 + j) * kTokens;
-                    const float f = s_kref[ref] * a.scale_log2, vt = s_vref[ref];
+                    const float f = fmaxf(s_kref[ref] * a.scale_log2, 1.1754944e-38f);   // (not 0: minus infinity times it)
                     const int newest = pos - tb, eldest = oldest - tb;   // columns eldest .. newest are seen
+                    const float vt = newest >= 0 && eldest < kTokens ? s_vref[ref] : 0.f;   // (what a row does not see leaves its unit alone)
                     tmem_ld_wait(x);
                     tmem_ld_wait(y);
                     if (__any_sync(0xffffffffu, newest < kTokens - 1 || eldest > 0)) {
@@ -433,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         vref = vnew;
                     }
                     // the values' scale against the largest so far, as a whole number in the exponent
-                    const float lower = vt > 0.f ? static_cast<float>((static_cast<int>(__float_as_uint(vt)) - static_cast<int>(__float_as_uint(vref))) >> 23) : 0.f;
+                    const float lower = vt > 0.f ? static_cast<float>(max((static_cast<int>(__float_as_uint(vt)) - static_cast<int>(__float_as_uint(vref))) >> 23, kLeastLower)) : 0.f;
                     const float shift = (m == -INFINITY ? 0.f : m) - kOffset - lower;
                     const unsigned long long f2 = pack2(f, f), shift2 = pack2(-shift, -shift);
                     unsigned long long sums[2] = {0ull, 0ull};
