@@ -211,3 +211,29 @@ def test_caches_side_by_side(tq):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
     for c in caches:
         c.close()
+
+
+@pytest.mark.parametrize("handle", [False, True])
+def test_results_without_a_place_on_another_stream(tq, handle):
+    """The zeros that attention makes room with are in front of it, whatever the current stream has to do first."""
+    c = tq.PagedKVCache(1, 2, 128, 8, 64, 2, 8, 40)
+    x = torch.randn((40, 2, 128), device="cuda").half()
+    c.plan(np.array([5, 30], np.int32), 40, 30)
+    c.append(0, x, x)
+    want = c.attention(0, x)
+    big = torch.randn((6000, 6000), device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        big = big @ big * 1e-4
+    out = c.attention(0, x, stream=side.cuda_stream if handle else side)
+    torch.cuda.synchronize()
+    c.check_status()
+    assert torch.equal(out, want) and (want[:35] != 0).any() and (want[35:] == 0).all()
+    with torch.cuda.stream(side):          # (no stream named: the default one)
+        for _ in range(4):
+            big = big @ big * 1e-4
+        out = c.attention(0, x)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    c.close()

@@ -72,6 +72,19 @@ def _tag(x, what):
     raise TypeError(f"{what}: expected float32 or float16, got {x.dtype}")
 
 
+def _zeros_like(x, stream):
+    """Zeros in front of a call on `stream`, by that stream."""
+    if not x.is_cuda:
+        return x.new_zeros(x.shape)
+    cuda = _torch.cuda
+    if stream is None:
+        stream = cuda.default_stream(x.device)
+    elif not hasattr(stream, "cuda_stream"):
+        stream = cuda.ExternalStream(int(stream), x.device)
+    with cuda.stream(stream):
+        return x.new_zeros(x.shape)
+
+
 class PagedKVCache:
     """Keys and values of up to `max_requests` requests in `num_pages` pages of `page_tokens` tokens, 8 bits each with a power of
     two for each page and head."""
@@ -139,7 +152,7 @@ class PagedKVCache:
         if queries.dtype is not half:
             raise TypeError("attention: queries must be float16")
         if out is None:
-            out = queries.new_zeros(queries.shape)
+            out = _zeros_like(queries, stream)
         op, more, _, os_ = _rows(out, q_heads, self.head_dim, "out")
         if more != tokens or out.dtype is not half:
             raise ValueError("out must be float16 of the queries' shape")
