@@ -548,7 +548,7 @@ int tq_hybrid_attention(tq_kv_cache_t cache, tq_decode_buffer_t buf, int layer, 
  * its plan too. */
 typedef struct tq_paged_cache_s* tq_paged_cache_t;
 
-/** head_dim 64 or 128; max_requests (rows of the block tables) up to 4096; max_tokens: new tokens of a plan at most.  All
+/** head_dim 64 or 128; num_heads up to 65536; max_requests (rows of the block tables) up to 4096; max_tokens: new tokens of a plan at most.  All
  *  memory is allocated here: num_layers * num_pages * num_heads * (2 * page_tokens * head_dim + 32) bytes, and tables. */
 tq_paged_cache_t tq_paged_cache_create(int num_layers, int num_heads, int head_dim, int num_pages, int page_tokens, int max_requests,
                                        int max_pages_per_request, int max_tokens);

@@ -10,7 +10,7 @@ from tests.paged_model import FLOOR, Model, exponent
     ({"num_layers": 0}, "positive"), ({"num_heads": 0}, "positive"), ({"num_pages": -1}, "positive"), ({"head_dim": 96}, "head_dim"),
     ({"page_tokens": 48}, "page"), ({"page_tokens": 256}, "page"), ({"max_requests": 0}, "max_requests"), ({"max_requests": 4097}, "max_requests"),
     ({"max_pages_per_request": 0}, "positive"), ({"max_tokens": 0}, "positive"), ({"num_pages": 1 << 24, "page_tokens": 128}, "tokens"),
-    ({"num_pages": 1 << 23, "num_heads": 256}, "pages times heads")])
+    ({"num_pages": 1 << 23, "num_heads": 256}, "pages times heads"), ({"num_pages": 1, "num_heads": 65537}, "65536 heads")])
 def test_caches_that_cannot_be(change, what):
     sizes = dict(num_layers=1, num_heads=2, head_dim=128, num_pages=4, page_tokens=64, max_requests=2, max_pages_per_request=4, max_tokens=8)
     with pytest.raises(tq.TQError, match=what):

@@ -18,6 +18,7 @@ public:
     PagedKVCache(int layers, int heads, int dim, int pages, int page_tokens, int max_requests, int max_pages, int max_tokens)
         : heads_(heads), dim_(dim), max_tokens_(max_tokens) {
         TQ_REQUIRE(layers > 0 && heads > 0 && pages > 0, "paged cache: layers, heads and pages must be positive");
+        TQ_REQUIRE(heads <= 65536, "paged cache: at most 65536 heads");   // (the kernels count requests times heads in 32 bits)
         TQ_REQUIRE(dim == 64 || dim == 128, "paged cache: head_dim must be 64 or 128");
         TQ_REQUIRE(page_tokens == 16 || page_tokens == 32 || page_tokens == 64 || page_tokens == 128, "paged cache: a page holds 16, 32, 64 or 128 tokens");
         TQ_REQUIRE(max_requests > 0 && max_requests <= tq::kPagedMaxRequests, "paged cache: max_requests must be 1 .. " + std::to_string(tq::kPagedMaxRequests));
