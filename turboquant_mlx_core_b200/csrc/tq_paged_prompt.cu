@@ -23,7 +23,7 @@
 // 63 tiles, in 19 with 2^4), and its O is then read, multiplied and written back, behind the weights, so that the products before it end meanwhile: 4096 such tokens 181 us, 190 with 2^4,
 // 199 with that and O in front of the weights; 175 where no row moves.
 //
-// What bounds it: 256 rows against 64 tokens (D = 128) take 2.7 thousand cycles.  A softmax warp is at work for 2.3 of them, 8 % wait; the products alone would take 1.24 (the scores'
+// What bounds it: 256 rows against 64 tokens (D = 128) take 2.7 thousand cycles.  A softmax warp is at work for 2.3 of them, waits for scores for 0.3 and writes results for 0.2; the products alone would take 1.24 (the scores'
 // 64 columns read 6 KB of shared memory in the 32 cycles that their arithmetic takes, 48 in fact), the exponentials alone 1.02, the softmax of both tiles with nothing beside it 1.17, all
 // roles' instructions fill 54 % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 175 us, 0.69 PFLOP/s of the
 // causal products, 41 % of a plain matrix product's rate.  Tried beside it, of the same prompt when it took 183: scores read twice in loops of 32 columns, a third less code, 191; two warps to a
