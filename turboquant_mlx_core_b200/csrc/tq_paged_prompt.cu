@@ -28,7 +28,8 @@
 // roles' instructions fill 54 % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 175 us, 0.69 PFLOP/s of the
 // causal products, 41 % of a plain matrix product's rate.  Tried beside it, of the same prompt when it took 183: scores read twice in loops of 32 columns, a third less code, 191; two warps to a
 // row's 64 scores and half as many for the conversions 195; keys and values two tiles ahead 185.  Tiles of 128 tokens with one set of scores and one thread for all products: 699 for 8192 tokens, 668
-// with these.
+// with these.  Part of what the softmax takes longer here than alone is the supply of its instructions: copies of its step in a row, alone, 771 cycles each while the code is below 20 KB, 933 at 37 KB, 1100
+// at 68 KB and 2045 at 147 KB; the roles' loops here are some 30 KB together.
 //
 // Every wait is bounded; a warp that gives up flags it, all warps fall through to the end, where the tensor memory is freed.
 #include <algorithm>
@@ -399,12 +400,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     fence_after();
                     const uint32_t t_s = t_s0 + (n & 1) * kTokens;
                     uint32_t x[32], y[32];
+                    const float kref = s_kref[ref], vref_here = s_vref[ref];
                     tmem_ld(t_s, x);
                     tmem_ld(t_s + 32, y);
                     const int tb = (tile0 + j) * kTokens;
-                    const float f = fmaxf(s_kref[ref] * a.scale_log2, 1.1754944e-38f);   // (not 0: minus infinity times it)
+                    const float f = fmaxf(kref * a.scale_log2, 1.1754944e-38f);   // (not 0: minus infinity times it)
                     const int newest = pos - tb, eldest = oldest - tb;   // columns eldest .. newest are seen
-                    const float vt = newest >= 0 && eldest < kTokens ? s_vref[ref] : 0.f;   // (what a row does not see leaves its unit alone)
+                    const float vt = newest >= 0 && eldest < kTokens ? vref_here : 0.f;   // (what a row does not see leaves its unit alone)
                     tmem_ld_wait(x);
                     tmem_ld_wait(y);
                     if (__any_sync(0xffffffffu, newest < kTokens - 1 || eldest > 0)) {
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 return go;
             };
             const uint64_t q_desc = smem_desc(base + S::kQ, S::kRowGroup), k_desc = smem_desc(base + S::kK, S::kRowGroup), v_desc = smem_desc(base + S::kV, S::kDimGroup);
-            uint32_t turns = 0, items = 0, n[2] = {0, 0};   // tiles of the cache; items of each row tile (a bit each, the parity); scores, or P V, of each row tile
+            uint32_t turns = 0, items = 0, n0 = 0, n1 = 0;   // tiles of the cache; items of each row tile (a bit each, the parity); scores, or P V, of each row tile
             while (until(s_bar.seg_full[seg_n % kSegments], (seg_n / kSegments) & 1)) {
                 const int tiles = s_seg[seg_n % kSegments].tiles, pair = s_seg[seg_n % kSegments].two() ? 2 : 1;
                 if (tiles == 0) break;
@@ -548,14 +550,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 for (int j = 0; j < tiles; ++j, ++turns) {
                     const uint32_t stage = turns % kStages, turn = (turns / kStages) & 1;
                     if (!until(first ? s_bar.k_full[stage] : s_bar.v_full[stage], turn)) break;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (t >= pair) continue;
-                        const uint32_t place = n[t] & 1, t_s = tmem + (2 * t + place) * kTokens;
+#pragma unroll 1
+                    for (int t = 0; t < pair; ++t) {
+                        const uint32_t nt = t ? n1 : n0, place = nt & 1, t_s = tmem + (2 * t + place) * kTokens;
                         if (first) {
                             if (j == 0 && !until(s_bar.q_full[t], (items >> t) & 1)) break;
                             // P of two tiles before was where these scores go
-                            if (n[t] >= 2 && !until(s_bar.o_done[t][place], ((n[t] >> 1) - 1) & 1)) break;
+                            if (nt >= 2 && !until(s_bar.o_done[t][place], ((nt >> 1) - 1) & 1)) break;
                             fence_after();
                             const uint64_t q = q_desc + t * (S::kQBytes >> 4), k = k_desc + stage * (S::kKBytes >> 4);
 #pragma unroll
@@ -564,14 +565,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                             if (j + 1 == tiles) umma_commit(bar(s_bar.q_empty[t]));
                         } else {
                             if (j == 0 && !until(s_bar.o_empty[t], ((items >> t) & 1) ^ 1)) break;
-                            if (!until(s_bar.p_full[t][place], (n[t] >> 1) & 1)) break;
+                            if (!until(s_bar.p_full[t][place], (nt >> 1) & 1)) break;
                             fence_after();
                             const uint64_t v = v_desc + stage * (S::kVBytes >> 4);
 #pragma unroll
                             for (int s = 0; s < kTokens / 16; ++s) umma_ts(tmem + 4 * kTokens + t * D, t_s + 8 * s, v + 16 * s, kIdescO, j > 0 || s > 0);
                             umma_commit(bar(s_bar.o_done[t][place]));
                         }
-                        ++n[t];
+                        if (t) ++n1; else ++n0;
                     }
                     if (!go) break;
                     umma_commit(bar(first ? s_bar.k_empty[stage] : s_bar.v_empty[stage]));
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const uint32_t ref = largest_scale(key_bits);
                 const __half2 fa = __float2half2_rn(code_factor(__shfl_sync(0xffffffffu, key_bits, page), ref)), off = __hmul2(fa, __float2half2_rn(-1152.f));
                 uint8_t* const dst = s_mem + S::kK + stage * S::kKBytes + 2 * w * S::kRowGroup + (lane & 7) * 16;
-#pragma unroll 2
+#pragma unroll 1
                 for (int s = 0; s < D / 32; ++s) {
                     const int r = 8 * (s & 1) + (lane & 7), c0 = (lane >> 3) + 2 * (s & 2);
                     const uint4 b4 = *reinterpret_cast<const uint4*>(raw + r * D + 16 * raw_chunk<D>(r, key_chunk<D>(r, c0)));
