@@ -182,35 +182,36 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
             if (!ok) raise_status(a.status, error);
         }
     }
-    if constexpr (!OUTPUT) return;
-    for (int t = t0; t < pages; t += step) {
-        const int i = owner_of(s_page, n, t), idx = (s_old[i] + P - 1) / P + t - s_page[i];
-        a.b.tables[static_cast<size_t>(s_row[i]) * a.b.max_pages + idx] = a.b.stack[free_before - 1 - t];
-    }
-    for (int t = t0; t < pieces; t += step) {
-        const int i = owner_of(s_piece, n, t), idx = s_old[i] / P + t - s_piece[i], count_i = s_start[i + 1] - s_start[i];
-        const int first = max(s_old[i], idx * P), last = min(s_old[i] + count_i, (idx + 1) * P);
-        a.b.pieces[t] = {s_start[i] + first - s_old[i], last - first, page_of(i, idx), first - idx * P};
-    }
-    if (a.slots || a.positions) {
-        for (int t = t0; t < a.tokens; t += step) {
-            int slot = -1, position = 0;
-            if (t < tokens) {
-                const int i = owner_of(s_start, n, t);
-                position = s_old[i] + t - s_start[i];
-                const int idx = position / P;
-                if (a.slots) slot = page_of(i, idx) * P + position - idx * P;
-            }
-            if (a.slots) a.slots[t] = slot;
-            if (a.positions) a.positions[t] = position;
+    if constexpr (OUTPUT) {
+        for (int t = t0; t < pages; t += step) {
+            const int i = owner_of(s_page, n, t), idx = (s_old[i] + P - 1) / P + t - s_page[i];
+            a.b.tables[static_cast<size_t>(s_row[i]) * a.b.max_pages + idx] = a.b.stack[free_before - 1 - t];
         }
-    }
-    if (a.tables) {
-        const long cells = static_cast<long>(n) * a.tables_width;
-        for (long t = t0; t < cells; t += step) {
-            const int i = static_cast<int>(t / a.tables_width), idx = static_cast<int>(t - static_cast<long>(i) * a.tables_width);
-            const int has = (s_old[i] + s_start[i + 1] - s_start[i] + P - 1) / P;
-            a.tables[t] = idx < has ? page_of(i, idx) : -1;
+        for (int t = t0; t < pieces; t += step) {
+            const int i = owner_of(s_piece, n, t), idx = s_old[i] / P + t - s_piece[i], count_i = s_start[i + 1] - s_start[i];
+            const int first = max(s_old[i], idx * P), last = min(s_old[i] + count_i, (idx + 1) * P);
+            a.b.pieces[t] = {s_start[i] + first - s_old[i], last - first, page_of(i, idx), first - idx * P};
+        }
+        if (a.slots || a.positions) {
+            for (int t = t0; t < a.tokens; t += step) {
+                int slot = -1, position = 0;
+                if (t < tokens) {
+                    const int i = owner_of(s_start, n, t);
+                    position = s_old[i] + t - s_start[i];
+                    const int idx = position / P;
+                    if (a.slots) slot = page_of(i, idx) * P + position - idx * P;
+                }
+                if (a.slots) a.slots[t] = slot;
+                if (a.positions) a.positions[t] = position;
+            }
+        }
+        if (a.tables) {
+            const long cells = static_cast<long>(n) * a.tables_width;
+            for (long t = t0; t < cells; t += step) {
+                const int i = static_cast<int>(t / a.tables_width), idx = static_cast<int>(t - static_cast<long>(i) * a.tables_width);
+                const int has = (s_old[i] + s_start[i + 1] - s_start[i] + P - 1) / P;
+                a.tables[t] = idx < has ? page_of(i, idx) : -1;
+            }
         }
     }
 }
