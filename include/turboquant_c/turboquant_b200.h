@@ -544,7 +544,7 @@ int tq_hybrid_attention(tq_kv_cache_t cache, tq_decode_buffer_t buf, int layer, 
  *
  * A step is a plan, then an append and an attention per layer, in stream order.  All calls on a cache must be ordered (one stream, or
  * events between streams); they work on the cache's device whichever is current.  Data pointers are device pointers, except for rows, counts and
- * lengths, which may be host memory where the stream is not being captured.  A captured graph that appends or attends holds
+ * lengths, which may be host memory, read before the call returns, where the stream is not being captured.  A captured graph that appends or attends holds
  * its plan too. */
 typedef struct tq_paged_cache_s* tq_paged_cache_t;
 

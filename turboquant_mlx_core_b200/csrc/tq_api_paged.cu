@@ -1,5 +1,6 @@
 // C-ABI of the paged 8-bit KV cache (include/turboquant_c/turboquant_b200.h, tq_paged_*).  The reference's cache holds one
 // sequence (include/turboquant/kv_cache.h:42-133); this one is what a server keeps beside it for the requests of a batch.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <memory>
@@ -30,6 +31,7 @@ public:
         device_ = tq::current_device();
         sms_ = tq::sm_count(device_);
         b_.max_requests = max_requests;
+        numbers_.resize(static_cast<size_t>(max_requests));
         b_.max_pages = max_pages;
         b_.num_pages = pages;
         b_.page_tokens = page_tokens;
@@ -215,11 +217,13 @@ private:
         tq::ensure_device(device_);
         use_.note(st);
     }
-    // Host numbers on the device; a copy from pageable memory is staged before the call returns.
+    // Host numbers on the device.  They are the caller's again when the call returns: a copy from pageable memory is staged before it returns, one from
+    // page-locked memory reads it when the stream comes to it, so that the caller's numbers go through pageable memory first, whatever they are in.
     const int* staged(const int* p, int n, int at, cudaStream_t st) {
         if (!p || n == 0 || tq::is_device_pointer(p)) return p;
         TQ_REQUIRE(!tq::stream_is_capturing(st), "paged cache: a captured plan needs its numbers in device memory");
-        TQ_CUDA(cudaMemcpyAsync(staged_ + at, p, 4ul * n, cudaMemcpyHostToDevice, st));
+        std::copy(p, p + n, numbers_.begin());
+        TQ_CUDA(cudaMemcpyAsync(staged_ + at, numbers_.data(), 4ul * n, cudaMemcpyHostToDevice, st));
         return staged_ + at;
     }
 
@@ -230,6 +234,7 @@ private:
     std::vector<DeviceBuffer> layers_;
     DeviceBuffer state_, scratch_;
     int* staged_ = nullptr;
+    std::vector<int> numbers_;
     tq::PagedBatch b_{};
     unsigned int* h_status_ = nullptr;
     unsigned int* d_status_ = nullptr;
