@@ -181,6 +181,7 @@ public:
         a.page_shift = b_.page_tokens == 16 ? 4 : b_.page_tokens == 32 ? 5 : b_.page_tokens == 64 ? 6 : 7;
         a.scale_log2 = static_cast<float>((scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(dim_))) * 1.4426950408889634);
         a.status = d_status_;
+        a.one = max_count_ == 1;
         // The device finds the requests of each kernel; a batch of one has one.
         const long max_rows = static_cast<long>(max_count_) * a.group;
         const bool many = max_rows > kFewRows;

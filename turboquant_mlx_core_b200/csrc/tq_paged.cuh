@@ -145,6 +145,7 @@ struct PagedAttnArgs {
     float* lse;          // or null
     long q_stride, out_stride;
     int n, tokens, heads, group, window, page_shift;
+    bool one;            // every request has one new token at most
     int few_rows;        // requests of more query rows (new tokens times the group) go through tq_paged_prompt.cu
     float scale_log2;    // softmax scale times log2(e)
     float* partial;

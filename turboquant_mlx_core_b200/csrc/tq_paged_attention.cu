@@ -63,6 +63,10 @@ __device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t which) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), off);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// 2^-x, x byte r of `lower` (0 from 2^-127 on).
+__device__ __forceinline__ float unit_ratio(uint32_t lower, int r) {
+    return __int_as_float(max(127 - static_cast<int>(lower >> (8 * r) & 0xffu), 0) << 23);
+}
 // A request's part of the work, in units: its tiles times its row tiles (times the KV heads).
 struct RequestWork {
     int row, start, count, held, lo, hi;   // tiles lo .. hi - 1
@@ -134,14 +138,17 @@ struct AttnShape {
     static constexpr int kPart = kRows * (D + 2);   // floats of a part: rows, then (maximum, sum) of each
 };
 
-template <int D, int NT>
+// ONE: every request has one new token, so that its rows see the same and one unit of the values does for all of them.  Otherwise a window's or the drafts' end may lie between
+// rows, and each has its own.  (Its own for single tokens too: 32 requests of 197 thousand tokens in all, 16 rows to each of 4 heads, 71.3 us for 68.3; of 395 thousand, 5 rows to each of 8,
+// 135.6 for 134.3.)
+template <int D, int NT, bool ONE>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     using S = AttnShape<D, NT>;
     constexpr int kRows = S::kRows, kStages = S::kStages;
     extern __shared__ __align__(128) uint8_t s_mem[];
     __shared__ __align__(8) unsigned long long s_full[kStages], s_empty[kStages];
     __shared__ unsigned int s_sum[kAttnThreads + 1];
-    __shared__ float s_ml[kMulWarps][kRows][2], s_vref[kMulWarps];
+    __shared__ float s_ml[kMulWarps][kRows][2], s_vref[kMulWarps][kRows];
     __shared__ unsigned int s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
@@ -303,7 +310,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
         }
         const int pos_min = first_pos + row0 / a.group, pos_max = first_pos + (row0 + live_rows - 1) / a.group;
 
-        float o[NT][D / 16][4], m[NT][2], l[NT][2], vref = 0.f;
+        float o[NT][D / 16][4], m[NT][2], l[NT][2];
+        // o is in units of the largest of the values' scales that its row has met: their exponents, a byte for each of the lane's rows (ONE: for all of them, the lowest byte).
+        uint32_t units = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = -INFINITY;
@@ -351,7 +360,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 }
                 const float f = scales.x * a.scale_log2;
                 const bool masks = w0 + 15 > pos_min || (a.window > 0 && w0 <= pos_max - a.window);
-                bool jump = scales.y > vref;
+                // the values' exponent, for the rows that see some of these tokens: what a row does not see leaves its unit alone
+                uint32_t value_units = __float_as_uint(scales.y) >> 23;
+                if constexpr (!ONE) {
+                    value_units *= 0x01010101u;
+                    if (masks) {
+#pragma unroll
+                        for (int r = 0; r < 2 * NT; ++r)
+                            if (w0 > pos[r >> 1][r & 1] || (a.window > 0 && w0 + 15 <= pos[r >> 1][r & 1] - a.window)) value_units &= ~(0xffu << (8 * r));
+                    }
+                }
+                const uint32_t units_now = ONE ? max(units, value_units) : __vmaxu4(units, value_units);
+                bool jump = units_now != units;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -365,7 +385,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                         jump = jump || x > m[nt][k & 1] + kSlack;
                     }
                 if (__any_sync(0xffffffffu, jump)) {
-                    const float vnew = fmaxf(vref, scales.y), vs = vnew > 0.f ? vref / vnew : 0.f;
+                    const uint32_t raised = units_now - units;   // (byte by byte)
+                    units = units_now;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -379,18 +400,15 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                                 m[nt][e] = top;
                             }
                             l[nt][e] *= down;
-                            const float both = down * vs;
+                            const float both = down * unit_ratio(raised, ONE ? 0 : 2 * nt + e);
 #pragma unroll
                             for (int u = 0; u < D / 16; ++u) {
                                 o[nt][u][e] *= both;
                                 o[nt][u][2 + e] *= both;
                             }
                         }
-                    vref = vnew;
                 }
-                // the values' scale against the largest so far: a power of two, by its bits (0 for those that are not numbers)
-                const int lower = static_cast<int>(__float_as_uint(scales.y)) - static_cast<int>(__float_as_uint(vref)) + 0x3f800000;
-                const float ratio = lower > 0 && scales.y > 0.f ? __int_as_float(lower) : 0.f;
+                const uint32_t lower = units - value_units;   // (byte by byte; of a row that sees nothing here the weights are 0)
                 uint32_t pf[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -403,8 +421,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                     l[nt][0] += p[0] + p[2];
                     l[nt][1] += p[1] + p[3];
                     // (row g, tokens 2 qd, 2 qd + 1 and 8 further on, as the second product wants them)
-                    pf[nt][0] = transposed(pack_half2(p[0] * ratio, p[1] * ratio));
-                    pf[nt][1] = transposed(pack_half2(p[2] * ratio, p[3] * ratio));
+                    const float r0 = unit_ratio(lower, ONE ? 0 : 2 * nt), r1 = unit_ratio(lower, ONE ? 0 : 2 * nt + 1);
+                    pf[nt][0] = transposed(pack_half2(p[0] * r0, p[1] * r1));
+                    pf[nt][1] = transposed(pack_half2(p[2] * r0, p[3] * r1));
                 }
                 // values, transposed: lane (g, qd) takes the D / 8 dims of column g, of the tokens 2 qd, 2 qd + 1 and those 8 further on
                 const uint8_t* const values = stage + S::kTileBytes + 16 * warp * D;
@@ -457,9 +476,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 if (g == 0) {
                     s_ml[warp][r][0] = m[nt][e];
                     s_ml[warp][r][1] = l[nt][e];
+                    s_vref[warp][r] = __uint_as_float((units >> (ONE ? 0 : 8 * (2 * nt + e)) & 0xffu) << 23);
                 }
             }
-        if (lane == 0) s_vref[warp] = vref;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kMulWarps) : "memory");
         {
             constexpr int kEach = kRows * D / (32 * kMulWarps);   // dims of a thread
@@ -472,7 +491,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
 #pragma unroll
             for (int w = 0; w < kMulWarps; ++w) {
                 // (a warp that saw nothing has zeros; one that met a NaN has no maximum, and its sum says so)
-                const float mw = s_ml[w][r][0], x = mw == top || mw == -INFINITY ? 1.f : exp2_approx(mw - top), y = x * s_vref[w];
+                const float mw = s_ml[w][r][0], x = mw == top || mw == -INFINITY ? 1.f : exp2_approx(mw - top), y = x * s_vref[w][r];
                 sum = fmaf(s_ml[w][r][1], x, sum);
                 const float* const from = s_o + (w * kRows + r) * S::kRowFloats + d0;
 #pragma unroll
@@ -607,9 +626,12 @@ void launch_typed(PagedAttnArgs a, int max_rows, void* scratch, int sms, cudaStr
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
     static std::atomic<unsigned long long> set{0};
-    allow_shared_memory(paged_attn_kernel<D, NT>, S::kSmem, set);
+    static std::atomic<unsigned long long> set_one{0};
+    if (a.one) allow_shared_memory(paged_attn_kernel<D, NT, true>, S::kSmem, set_one);
+    else allow_shared_memory(paged_attn_kernel<D, NT, false>, S::kSmem, set);
     // (Both ask for all of the SM's memory as shared memory: an SM changes its division only when it is empty.)
-    launch_pdl_carved(paged_attn_kernel<D, NT>, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), S::kSmem, 100, st, a);
+    const auto attend = [&](auto kernel) { launch_pdl_carved(kernel, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), S::kSmem, 100, st, a); };
+    a.one ? attend(paged_attn_kernel<D, NT, true>) : attend(paged_attn_kernel<D, NT, false>);
     launch_pdl_carved(paged_join_kernel<D, NT>, dim3(static_cast<unsigned int>(a.join_items ? a.join_items : ctas), static_cast<unsigned int>(std::min(S::kRows, max_rows))),
                       dim3(32 * kJoinWarps), 0, 100, st, a);
 }
