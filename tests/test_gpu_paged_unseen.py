@@ -96,3 +96,26 @@ def test_few_rows_within_their_own_bound(tq, dim, group, last, window):
     q = queries(rng, 4 * last, 2 * group, dim)
     compare(*run(c, torch.from_numpy(q).cuda(), window=window), attention(m, q, window))
     c.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("group,last,window", [(1, 60, 100), (7, 30, 100), (2, 200, 130), (1, 300, 257)])
+@pytest.mark.parametrize("large", [2.0 ** 20, 2.0 ** 27, 1e15])
+def test_a_window_that_ends_inside_a_tile_of_many_rows(tq, dim, page, group, last, window, large):
+    """A value is large at the beginning of 64 tokens, and windows begin there, behind it in its page and in the pages behind: a row goes by the
+    scales that it sees, in these 64 tokens and in the ones behind them."""
+    rng = np.random.default_rng(dim + page + last)
+    requests, edge = 25, 128
+
+    def change(k, v, i):
+        v[edge] = large
+        k[edge] = 0
+    # row 0 sees from edge - 3 on
+    c, m = served(tq, rng, 4, dim, page, [edge + window - 4], [last], change, requests)
+    q = queries(rng, last, 4 * group, dim)
+    out, lse = run(c, torch.from_numpy(q).cuda().repeat(requests, 1, 1), window=window)
+    want = attention(m, q, window)
+    for o, l in zip(out.split(last), lse.split(last)):
+        assert not compare(o, l, want)[4:].any()
+    c.close()

@@ -18,7 +18,7 @@
 //   warps 24-31      values, transposed on the way; both in two groups that take every second tile
 //
 // Scales are powers of two: within a tile the pages' go into the halves without a rounding (but for codes 2^29 below the tile's largest scale), the tile's own goes into the
-// exponent's factor (keys) or, as an integer, into the exponent (values: P V is kept in units of the largest scale so far).  The reference maximum m
+// exponent's factor (keys) or, as an integer, into the exponent (values: P V is kept in units of the largest scale that the row has seen).  The reference maximum m
 // moves only when a score exceeds it by 2^8; weights are at most 2^15 then.  Where keys are of unequal strength one of a warp's 32 rows often has such a score (simulated, with norms spread by e^0.5: in 12 of
 // 63 tiles, in 19 with 2^4), and its O is then read, multiplied and written back, behind the weights, so that the products before it end meanwhile: 4096 such tokens 181 us, 190 with 2^4,
 // 199 with that and O in front of the weights; 175 where no row moves.
@@ -62,6 +62,7 @@ constexpr int kRefs = 8;             // tiles whose scales are kept
 constexpr float kOffset = 7.f, kSlack = 8.f;
 constexpr int kLeastLower = -60;     // of a tile's values against the largest so far: a weight times 2^-60 is 0 as a half, and their sum, which is taken of these, far from it
 constexpr float kHeadroom = 32.f;    // largest factor of a code in the halves
+constexpr float kLeastFactor = 5.9604645e-8f;   // the least one, 2^-24: a half's last place
 constexpr uint32_t kTmemAll = 512;
 
 template <int D>
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     __shared__ __align__(8) Bars s_bar;
     __shared__ long long s_sum[kWarps];
     __shared__ float s_kref[kRefs], s_vref[kRefs];
+    __shared__ __align__(16) float s_vpart[kRefs][kTokens / kWarpTokens];   // the values' scales of a tile's parts, of one page each
     __shared__ __align__(16) Segment s_seg[kSegments];
     __shared__ uint32_t s_tmem;
     __shared__ unsigned int s_abort;
@@ -389,7 +391,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const bool live = row < at.rows;
                 const int oldest = a.window > 0 ? max(0, pos - a.window + 1) : 0;
                 const bool idle = at.row0 + t * kRows + 32 * (warp & 3) >= at.rows;   // a warp without rows: it keeps the others' count (16 requests of 35 rows: 48 us, 56 with the softmax of what is not there)
-                float m = -INFINITY, l = 0.f, vref = 0.f;
+                // O is in units of vref: the largest of the values' scales that the row has seen (vseen), or the tile's where it sees only part of the tile and the rest is larger.  It comes down
+                // again behind such a tile: a window that begins there has all its other tokens in front.
+                float m = -INFINITY, l = 0.f, vref = 0.f, vseen = 0.f;
                 for (int j = 0; j < tiles; ++j) {
                     const uint32_t ref = (count + j) & (kRefs - 1), n = done + j;
                     if (!wait(s_bar.s_full[t][n & 1], (n >> 1) & 1)) break;
@@ -406,13 +410,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     const int tb = (tile0 + j) * kTokens;
                     const float f = fmaxf(kref * a.scale_log2, 1.1754944e-38f);   // (not 0: minus infinity times it)
                     const int newest = pos - tb, eldest = oldest - tb;   // columns eldest .. newest are seen
-                    const float vt = newest >= 0 && eldest < kTokens ? vref_here : 0.f;   // (what a row does not see leaves its unit alone)
+                    float vt = newest >= 0 && eldest < kTokens ? vref_here : 0.f, vpart = vt;   // (what a row does not see leaves its unit alone)
                     tmem_ld_wait(x);
                     tmem_ld_wait(y);
                     if (__any_sync(0xffffffffu, newest < kTokens - 1 || eldest > 0)) {
                         // a bit for each column
                         const uint64_t seen = (newest >= 63 ? ~0ull : newest < 0 ? 0ull : (2ull << newest) - 1) & (eldest <= 0 ? ~0ull : eldest > 63 ? 0ull : ~0ull << eldest);
                         const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+                        const float4 parts = *reinterpret_cast<const float4*>(s_vpart[ref]);
+                        vpart = fmaxf(fmaxf(lo & 0xffffu ? parts.x : 0.f, lo >> 16 ? parts.y : 0.f), fmaxf(hi & 0xffffu ? parts.z : 0.f, hi >> 16 ? parts.w : 0.f));
+                        if (code_factor(__float_as_uint(vpart), __float_as_uint(vt)) < kLeastFactor) vt = 0.f;   // (all that it sees counts as 0)
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             if (!(lo >> e & 1)) x[e] = 0xff800000u;   // (minus infinity, times f)
@@ -426,11 +433,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     top *= f;   // (f is positive; NaN columns do not count)
                     const bool jump = top > m + kSlack || (m == -INFINITY && top > m);
                     float both = 1.f;
-                    const bool moves = __any_sync(0xffffffffu, jump || vt > vref);
+                    vseen = fmaxf(vseen, vpart);
+                    const float vnew = fmaxf(vseen, vt);
+                    const bool moves = __any_sync(0xffffffffu, jump || vnew != vref);
                     if (moves) {
                         const float to = jump ? top : m;
                         const float down = jump ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
-                        const float vnew = fmaxf(vref, vt);
                         both = vnew > 0.f ? down * (vref / vnew) : 0.f;
                         l *= down;
                         m = to;
@@ -731,9 +739,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4*>(to + 128) = make_uint4(h[4], h[5], h[6], h[7]);
                 }
-                if (w == 0 && lane == 0) {   // (in place before the scores are)
-                    s_kref[now.n & (kRefs - 1)] = ref > 0u ? __uint_as_float(ref) * (1.f / kHeadroom) : 1.f;
-                    s_vref[now.n & (kRefs - 1)] = __uint_as_float(value_ref);
+                if (w == 0) {   // (in place before the scores are)
+                    const uint32_t part = __shfl_sync(0xffffffffu, value_bits, min(kWarpTokens * (lane & 3) >> a.page_shift, ((min(kTokens, seg_tokens) + P - 1) >> a.page_shift) - 1));
+                    if (lane < kTokens / kWarpTokens) s_vpart[now.n & (kRefs - 1)][lane] = __uint_as_float(part);
+                    if (lane == 0) {
+                        s_kref[now.n & (kRefs - 1)] = ref > 0u ? __uint_as_float(ref) * (1.f / kHeadroom) : 1.f;
+                        s_vref[now.n & (kRefs - 1)] = __uint_as_float(value_ref);
+                    }
                 }
             } else {
                 // a lane takes four dims of eight tokens
