@@ -545,7 +545,8 @@ int tq_hybrid_attention(tq_kv_cache_t cache, tq_decode_buffer_t buf, int layer, 
  * A step is a plan, then an append and an attention per layer, in stream order.  All calls on a cache must be ordered (one stream, or
  * events between streams); they work on the cache's device whichever is current.  Data pointers are device pointers, except for rows, counts and
  * lengths, which may be host memory, read before the call returns, where the stream is not being captured.  A captured graph that appends or attends holds
- * its plan too. */
+ * its plan too, and ends the one in force: an append or attention behind a replay that was made for a plan of other sizes (n, tokens,
+ * max_count) does nothing, and tq_paged_status tells. */
 typedef struct tq_paged_cache_s* tq_paged_cache_t;
 
 /** head_dim 64 or 128; num_heads up to 65536; max_requests (rows of the block tables) up to 4096; max_tokens: new tokens of a plan at most.  All
@@ -585,7 +586,8 @@ int tq_paged_read(tq_paged_cache_t cache, int layer, const int* pages, int n, vo
  *  among them count as 0. */
 int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window,
                        float scale, void* out_fp16, long out_stride, float* lse, void* stream);
-/** Non-zero, once, when a call that has finished found its batch impossible or a wait on the device ran out. */
+/** Non-zero, once, when a call that has finished found its batch impossible or another plan on the device than the one that it was made for, or a wait
+ *  on the device ran out. */
 int tq_paged_status(tq_paged_cache_t cache);
 /** Free pages, once all work on the device is done (waits for it); -1 on error. */
 int tq_paged_free_pages(tq_paged_cache_t cache);

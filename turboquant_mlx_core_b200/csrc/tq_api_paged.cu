@@ -104,9 +104,7 @@ public:
         tq::PagedPlanArgs a{b_, staged(rows, n, 0, st), staged(counts, n, b_.max_requests, st), n, tokens, max_count, starts, lengths, slots, positions, tables,
                             tables_width, d_status_, sms_};
         tq::launch_paged_plan(a, st);
-        n_ = n;
-        tokens_ = tokens;
-        max_count_ = std::min(max_count, tokens);
+        plan_ = {n, tokens, std::min(max_count, tokens)};
     }
     void truncate(const int* rows, const int* lengths, int n, cudaStream_t st) {
         TQ_REQUIRE(n >= 0 && n <= b_.max_requests, "paged truncate: more requests than the cache was made for");
@@ -121,21 +119,21 @@ public:
         a.status = d_status_;
         a.sms = sms_;
         tq::launch_paged_truncate(a, st);
-        n_ = -1;
+        plan_.n = -1;
     }
     void append(int layer, const void* keys, const void* values, int dtype, int tokens, long key_stride, long value_stride, cudaStream_t st) {
         check_layer(layer);
-        TQ_REQUIRE(n_ >= 0, "paged append: no plan in force");
+        TQ_REQUIRE(plan_.n >= 0, "paged append: no plan in force");
         TQ_REQUIRE(dtype == TQ_F32 || dtype == TQ_F16, "paged append: keys and values must be fp32 or fp16");
-        TQ_REQUIRE(tokens == tokens_, "paged append: the plan is for " + std::to_string(tokens_) + " tokens");
-        if (n_ == 0 || max_count_ == 0) return;
+        TQ_REQUIRE(tokens == plan_.tokens, "paged append: the plan is for " + std::to_string(plan_.tokens) + " tokens");
+        if (plan_.n == 0 || plan_.most == 0) return;
         TQ_REQUIRE(tq::is_device_pointer(keys) && tq::is_device_pointer(values), "paged append: keys and values must be device pointers");
         const long row = static_cast<long>(heads_) * dim_;
         TQ_REQUIRE(key_stride >= row && value_stride >= row, "paged append: a token's stride is shorter than its heads");
         begin(st);
         tq::PagedAppendArgs a{b_.header, b_.pieces, layers_[static_cast<size_t>(layer)].as<uint8_t>(), keys, values, key_stride, value_stride, heads_,
-                              b_.page_tokens, tokens, b_.num_pages};
-        tq::launch_paged_append(a, dim_, dtype == TQ_F16, n_, max_count_, st);
+                              b_.page_tokens, plan_, d_status_};
+        tq::launch_paged_append(a, dim_, dtype == TQ_F16, st);
     }
     void read(int layer, const int* pages, int n, void* keys, void* values, int dtype, cudaStream_t st) {
         check_layer(layer);
@@ -153,13 +151,13 @@ public:
     }
     void attention(int layer, const void* q, int tokens, int q_heads, long q_stride, int window, float scale, void* out, long out_stride, float* lse, cudaStream_t st) {
         check_layer(layer);
-        TQ_REQUIRE(n_ >= 0, "paged attention: no plan in force");
-        TQ_REQUIRE(tokens == tokens_, "paged attention: the plan is for " + std::to_string(tokens_) + " tokens");
+        TQ_REQUIRE(plan_.n >= 0, "paged attention: no plan in force");
+        TQ_REQUIRE(tokens == plan_.tokens, "paged attention: the plan is for " + std::to_string(plan_.tokens) + " tokens");
         TQ_REQUIRE(q_heads > 0 && q_heads % heads_ == 0, "paged attention: query heads must be a multiple of KV heads");
         TQ_REQUIRE(q_heads / heads_ <= 1024, "paged attention: more than 1024 query heads to a KV head");
         TQ_REQUIRE(window >= 0, "paged attention: negative window");
         TQ_REQUIRE(std::isfinite(scale) && scale >= 0.f, "paged attention: the scale must be finite, and 0 (1 / sqrt(head_dim)) or positive");
-        if (n_ == 0 || max_count_ == 0) return;
+        if (plan_.n == 0 || plan_.most == 0) return;
         TQ_REQUIRE(tq::is_device_pointer(q) && tq::is_device_pointer(out) && (!lse || tq::is_device_pointer(lse)),
                    "paged attention: queries and results must be device pointers");
         const long row = static_cast<long>(q_heads) * dim_;
@@ -173,19 +171,17 @@ public:
         a.lse = lse;
         a.q_stride = q_stride;
         a.out_stride = out_stride;
-        a.n = n_;
-        a.tokens = tokens;
+        a.sizes = plan_;
         a.heads = heads_;
         a.group = q_heads / heads_;
         a.window = window;
         a.page_shift = b_.page_tokens == 16 ? 4 : b_.page_tokens == 32 ? 5 : b_.page_tokens == 64 ? 6 : 7;
         a.scale_log2 = static_cast<float>((scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(dim_))) * 1.4426950408889634);
         a.status = d_status_;
-        a.one = max_count_ == 1;
         // The device finds the requests of each kernel; a batch of one has one.
-        const long max_rows = static_cast<long>(max_count_) * a.group;
+        const long max_rows = static_cast<long>(plan_.most) * a.group;
         const bool many = max_rows > kFewRows;
-        a.few_rows = many && n_ == 1 ? 0 : kFewRows;
+        a.few_rows = many && plan_.n == 1 ? 0 : kFewRows;
         if (many) tq::launch_paged_prompt(a, dim_, max_rows, scratch_.as<char>() + prompt_scratch_, sms_, st);
         if (a.few_rows) tq::launch_paged_attention(a, dim_, static_cast<int>(std::min<long>(max_rows, kFewRows)), scratch_.as<void>(), sms_, st);
     }
@@ -197,8 +193,9 @@ public:
                                            "a negative count, one above max_count, or more tokens in all than announced",
                                            "a request would be longer than max_pages_per_request pages", "not enough free pages",
                                            "truncation to a length that the request does not have", "a page number outside the cache",
-                                           "a wait on the device ran out"};
-        throw tq::Error(std::string("paged cache: ") + what[code < 8 ? code : 0]);
+                                           "a wait on the device ran out",
+                                           "the plan on the device is not the one that a call was made for"};
+        throw tq::Error(std::string("paged cache: ") + what[code < 9 ? code : 0]);
     }
     int free_pages() {
         tq::ensure_device(device_);
@@ -229,7 +226,7 @@ private:
     }
 
     int heads_, dim_, max_tokens_, device_ = 0, sms_ = 0;
-    int n_ = -1, tokens_ = 0, max_count_ = 0;   // of the plan in force (n_ < 0: none)
+    tq::PagedSizes plan_{-1, 0, 0};   // of the plan in force (n < 0: none)
     size_t prompt_scratch_ = 0;
     tq::StreamUse use_;
     std::vector<DeviceBuffer> layers_;

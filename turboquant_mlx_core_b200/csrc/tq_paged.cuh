@@ -41,10 +41,16 @@ __device__ __forceinline__ int value_chunk(int token, int c) {
     else return c ^ ((token >> 1) & 3);
 }
 
+// What the host says of a plan: its requests, its tokens and one request's at most.
+struct PagedSizes {
+    int n, tokens, most;
+};
 // What the device keeps of the last plan, beside the arrays of PagedBatch.
-struct PagedHeader {
+struct __align__(16) PagedHeader {
     int free_pages;      // pages on the stack
     int requests, tokens, pieces;   // of the plan (all 0 where it was refused)
+    PagedSizes sizes;    // n below 0: a truncation came behind it
+    int unused;
 };
 // A run of new tokens in one page.
 struct PagedPiece {
@@ -72,7 +78,8 @@ enum PagedStatus : unsigned int {
     kPagedNoPages = 4,     // not enough free pages
     kPagedBadLength = 5,   // truncation to a length that the request does not have
     kPagedBadPage = 6,     // a page number outside the cache
-    kPagedWait = 7         // a bounded wait ran out
+    kPagedWait = 7,        // a bounded wait ran out
+    kPagedOtherPlan = 8    // the plan on the device is not the one that a launch was made for
 };
 
 // Lets a kernel have so much dynamic shared memory, once for each device (`set`: those that have been).
@@ -113,9 +120,11 @@ struct PagedAppendArgs {
     const void* keys;
     const void* values;
     long key_stride, value_stride;   // elements from token to token
-    int heads, page_tokens, tokens, num_pages;
+    int heads, page_tokens;
+    PagedSizes sizes;
+    unsigned int* status;
 };
-void launch_paged_append(const PagedAppendArgs& a, int dim, bool half, int n, int max_count, cudaStream_t st);
+void launch_paged_append(const PagedAppendArgs& a, int dim, bool half, cudaStream_t st);
 
 struct PagedReadArgs {
     const uint8_t* layer;
@@ -144,8 +153,8 @@ struct PagedAttnArgs {
     __half* out;
     float* lse;          // or null
     long q_stride, out_stride;
-    int n, tokens, heads, group, window, page_shift;
-    bool one;            // every request has one new token at most
+    PagedSizes sizes;
+    int heads, group, window, page_shift;
     int few_rows;        // requests of more query rows (new tokens times the group) go through tq_paged_prompt.cu
     float scale_log2;    // softmax scale times log2(e)
     float* partial;
@@ -162,6 +171,18 @@ void launch_paged_prompt(PagedAttnArgs a, int dim, long max_rows, void* scratch,
 
 // ---- what the attention kernels share -------------------------------------------------------------
 namespace paged_device {
+
+// Requests and pieces of the plan on the device; none, with a status, where it is of other sizes than the launch (a captured step came between a plan and the call): the launch's grid, its
+// choice of kernels and the caller's rows need not fit it.
+struct Planned {
+    int requests, pieces;
+};
+__device__ __forceinline__ Planned planned(const PagedHeader* header, const PagedSizes& sizes, unsigned int* status) {
+    const int4 plan = reinterpret_cast<const int4*>(header)[0], made = reinterpret_cast<const int4*>(header)[1];   // (both on their way at once)
+    if (made.x == sizes.n && made.y == sizes.tokens && made.z == sizes.most) return {plan.y, plan.w};
+    if (blockIdx.x == 0 && threadIdx.x == 0) raise_status(status, kPagedOtherPlan);
+    return {0, 0};
+}
 
 constexpr uint32_t kPagedWaitLimit = 400u * 1000 * 1000;   // cycles: 0.2 s at 2 GHz
 

@@ -79,7 +79,7 @@ struct RequestWork {
         const int first = held - count;   // position of the first new token
         lo = a.window > 0 ? max(0, first - a.window + 1) / kTileTokens : 0;
         hi = (held + kTileTokens - 1) / kTileTokens;
-        row_tiles = start + count <= a.tokens && count * a.group <= a.few_rows ? (count * a.group + tile_rows - 1) / tile_rows : 0;
+        row_tiles = count * a.group <= a.few_rows ? (count * a.group + tile_rows - 1) / tile_rows : 0;
     }
     // (A unit is some 8 KB of the cache at least, twice at most: all of them are a 32-bit number.)
     __device__ __forceinline__ unsigned int units(int heads) const { return static_cast<unsigned int>(row_tiles * heads) * static_cast<unsigned int>(hi - lo); }
@@ -162,11 +162,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
     }
     pdl_wait_release();
     // units in front of each thread's requests (a plan that was refused has none, which is known only when they have been read)
-    const int per = (a.n + kAttnThreads - 1) / kAttnThreads;
+    const int per = (a.sizes.n + kAttnThreads - 1) / kAttnThreads;
     {
-        const int requests = a.b.header->requests;
+        const int requests = planned(a.b.header, a.sizes, a.status).requests;
         unsigned int mine = 0;
-        for (int i = tid * per; i < min(a.n, (tid + 1) * per); ++i) {
+        for (int i = tid * per; i < min(a.sizes.n, (tid + 1) * per); ++i) {
             RequestWork w;
             w.load(a, i, kRows);
             const unsigned int units = i < requests ? w.units(a.heads) : 0u;
@@ -621,17 +621,18 @@ void launch_typed(PagedAttnArgs a, int max_rows, void* scratch, int sms, cudaStr
     const int ctas = sms * S::kCtas;
     // Items that there can be: where they are fewer than the CTAs each has its own entry, and the kernel behind as many CTAs.
     a.row_tiles = (max_rows + S::kRows - 1) / S::kRows;
-    const long items = static_cast<long>(a.n) * a.heads * a.row_tiles;
+    const long items = static_cast<long>(a.sizes.n) * a.heads * a.row_tiles;
     a.join_items = items <= ctas ? static_cast<int>(items) : 0;
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
     static std::atomic<unsigned long long> set{0};
     static std::atomic<unsigned long long> set_one{0};
-    if (a.one) allow_shared_memory(paged_attn_kernel<D, NT, true>, S::kSmem, set_one);
+    const bool one = a.sizes.most == 1;
+    if (one) allow_shared_memory(paged_attn_kernel<D, NT, true>, S::kSmem, set_one);
     else allow_shared_memory(paged_attn_kernel<D, NT, false>, S::kSmem, set);
     // (Both ask for all of the SM's memory as shared memory: an SM changes its division only when it is empty.)
     const auto attend = [&](auto kernel) { launch_pdl_carved(kernel, dim3(static_cast<unsigned int>(ctas)), dim3(kAttnThreads), S::kSmem, 100, st, a); };
-    a.one ? attend(paged_attn_kernel<D, NT, true>) : attend(paged_attn_kernel<D, NT, false>);
+    one ? attend(paged_attn_kernel<D, NT, true>) : attend(paged_attn_kernel<D, NT, false>);
     launch_pdl_carved(paged_join_kernel<D, NT>, dim3(static_cast<unsigned int>(a.join_items ? a.join_items : ctas), static_cast<unsigned int>(std::min(S::kRows, max_rows))),
                       dim3(32 * kJoinWarps), 0, 100, st, a);
 }

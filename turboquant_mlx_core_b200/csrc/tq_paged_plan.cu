@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         if (t0 == 0) {
             a.b.starts[n] = tokens;
             if (a.starts) a.starts[n] = tokens;
-            *a.b.header = {free_before - pages, ok ? n : 0, tokens, pieces};
+            *a.b.header = {free_before - pages, ok ? n : 0, tokens, pieces, {n, a.tokens, min(a.max_count, a.tokens)}, 0};
             if (!ok) raise_status(a.status, error);
         }
     }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_truncate_kernel(PagedPlanA
         }
     }
     if (t0 == 0) {
-        *a.b.header = {free_before + pages, 0, 0, 0};
+        *a.b.header = {free_before + pages, 0, 0, 0, {-1, 0, 0}, 0};
         if (!ok) raise_status(a.status, s_error);
     }
 }
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedApp
     pdl_wait_release();
     behind_wait(a.pieces, a.header, a.keys, a.values);
     const int lane = threadIdx.x & 31, tid = WARP ? lane : threadIdx.x;
-    const long jobs = static_cast<long>(a.header->pieces) * a.heads * 2;
+    const long jobs = static_cast<long>(paged_device::planned(a.header, a.sizes, a.status).pieces) * a.heads * 2;
     const int P = a.page_tokens, c = tid % kChunks, r0 = tid / kChunks;
     const size_t block = paged_block_bytes(P, D);
     long job = blockIdx.x, stride = gridDim.x;
@@ -404,7 +404,6 @@ __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedApp
         const long rest = job >> 1;
         const int head = static_cast<int>(rest % a.heads);
         const PagedPiece piece = a.pieces[rest / a.heads];
-        if (piece.token + piece.count > a.tokens || piece.count > ITER * kRows) continue;   // a plan that this launch was not made for
         const long row_stride = second ? a.value_stride : a.key_stride;
         const T* const src = static_cast<const T*>(second ? a.values : a.keys) + piece.token * row_stride + static_cast<long>(head) * D + 16 * c;
         uint8_t* const dst = a.layer + (static_cast<size_t>(piece.page) * a.heads + head) * block;
@@ -457,12 +456,12 @@ __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedApp
 }
 
 template <int D, typename T, bool WIDE>
-void launch_append_typed(const PagedAppendArgs& a, int n, int max_count, cudaStream_t st) {
+void launch_append_typed(const PagedAppendArgs& a, cudaStream_t st) {
     // pieces that the plan can have: each of the requests begins and ends in a page of its own
-    const long most = std::min<long>(a.tokens, a.tokens / a.page_tokens + 2L * n) * a.heads * 2;
+    const long most = std::min<long>(a.sizes.tokens, a.sizes.tokens / a.page_tokens + 2L * a.sizes.n) * a.heads * 2;
     if (most == 0) return;
     constexpr int kWarpRows = 512 / D, kCtaRows = 4096 / D;   // tokens at a time
-    const int longest = std::min(max_count, a.page_tokens);
+    const int longest = std::min(a.sizes.most, a.page_tokens);
     auto warps = [&](auto kernel) { launch_pdl(kernel, dim3(static_cast<unsigned int>(std::min<long>((most + 3) / 4, 1 << 20))), dim3(128), 0, st, a); };
     auto ctas = [&](auto kernel) { launch_pdl(kernel, dim3(static_cast<unsigned int>(std::min<long>(most, 1 << 20))), dim3(256), 0, st, a); };
     if (longest <= kWarpRows) warps(paged_append_kernel<D, T, WIDE, true, 1>);
@@ -535,13 +534,13 @@ void launch_paged_init(uint8_t* layer, size_t blocks, size_t block_bytes, cudaSt
     paged_init_kernel<<<static_cast<unsigned int>(std::min<size_t>(blocks, 4096)), 256, 0, st>>>(layer, blocks, block_bytes);
     TQ_CUDA(cudaGetLastError());
 }
-void launch_paged_append(const PagedAppendArgs& a, int dim, bool half, int n, int max_count, cudaStream_t st) {
+void launch_paged_append(const PagedAppendArgs& a, int dim, bool half, cudaStream_t st) {
     const int es = half ? 2 : 4;
     const bool wide = ((reinterpret_cast<uintptr_t>(a.keys) | reinterpret_cast<uintptr_t>(a.values) | static_cast<uintptr_t>(a.key_stride * es) |
                         static_cast<uintptr_t>(a.value_stride * es)) & 15) == 0;
     auto go = [&](auto d, auto t) {
-        if (wide) launch_append_typed<d(), decltype(t), true>(a, n, max_count, st);
-        else launch_append_typed<d(), decltype(t), false>(a, n, max_count, st);
+        if (wide) launch_append_typed<d(), decltype(t), true>(a, st);
+        else launch_append_typed<d(), decltype(t), false>(a, st);
     };
     using D64 = std::integral_constant<int, 64>;
     using D128 = std::integral_constant<int, 128>;

@@ -164,7 +164,7 @@ __device__ __forceinline__ int next_request(const PagedAttnArgs& a, int i, int n
         x.start = a.b.starts[mine];
         x.count = a.b.starts[mine + 1] - x.start;
         x.held = a.b.held[mine];
-        const bool many = base + lane < n && x.start + x.count <= a.tokens && x.count * a.group > a.few_rows;
+        const bool many = base + lane < n && x.count * a.group > a.few_rows;
         const unsigned int found = __ballot_sync(0xffffffffu, many);
         if (found) {
             const int src = __ffs(static_cast<int>(found)) - 1;
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait_release();
-    const int n = min(a.n, a.b.header->requests);
+    const int n = planned(a.b.header, a.sizes, a.status).requests;
     const int per = (n + kWarps - 1) / kWarps;
     {
         const int end = min(n, (warp + 1) * per);

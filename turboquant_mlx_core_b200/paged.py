@@ -189,7 +189,8 @@ class PagedKVCache:
         return n
 
     def check_status(self):
-        """Raise if a finished call found its batch impossible (then nothing of the batch was done) or a wait on the device ran out."""
+        """Raise if a finished call found its batch impossible or another plan on the device than its own (then nothing of it was done), or a wait on the
+        device ran out."""
         check(self._L.tq_paged_status(self._h), "PagedKVCache")
 
     def close(self):
