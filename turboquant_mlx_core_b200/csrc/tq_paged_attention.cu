@@ -261,13 +261,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 s_abort = 1;
                 raise_status(a.status, kPagedWait);
             }
-            // copies on their way land before the CTA's memory is another's (the flag does not cut this short)
-            unsigned int never = 0;
-            for (int k = 0; k < issued; ++k) {
-                if (s == 0) phase ^= 1;
-                s = s == 0 ? kStages - 1 : s - 1;
-                bar_wait(smem_addr(&s_full[s]), phase, &never);
-            }
+        }
+        // Copies on their way land before the CTA's memory is another's: also where a multiplying warp gives up when all have been issued.  (The flag does not cut this short.)
+        unsigned int never = 0;
+        for (int k = 0; k < issued; ++k) {
+            if (s == 0) phase ^= 1;
+            s = s == 0 ? kStages - 1 : s - 1;
+            bar_wait(smem_addr(&s_full[s]), phase, &never);
         }
         return;
     }

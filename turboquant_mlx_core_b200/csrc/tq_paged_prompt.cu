@@ -589,12 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 bar_arrive(bar(s_bar.seg_empty[seg_n % kSegments]));
                 ++seg_n;
             }
-            if (!go) {   // what was issued ends before the tensor memory goes
-                const int t = warp - kMmaWarp;
-                umma_commit(bar(s_bar.done[t]));
-                unsigned int never = 0;
-                bar_wait(bar(s_bar.done[t]), 0, &never);
-            }
+            // What was issued ends before the tensor memory goes: also where another warp has given up and this thread was through.
+            umma_commit(bar(s_bar.done[warp - kMmaWarp]));
+            unsigned int never = 0;
+            bar_wait(bar(s_bar.done[warp - kMmaWarp]), 0, &never);
         }
         __syncwarp();
         if (warp >= kQueryWarp) {
