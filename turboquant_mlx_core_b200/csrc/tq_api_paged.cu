@@ -178,12 +178,14 @@ public:
         a.page_shift = b_.page_tokens == 16 ? 4 : b_.page_tokens == 32 ? 5 : b_.page_tokens == 64 ? 6 : 7;
         a.scale_log2 = static_cast<float>((scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(dim_))) * 1.4426950408889634);
         a.status = d_status_;
+        // Up to kFewRows query rows of a request (new tokens times query heads to a KV head) go to the kernel for few rows.  Over 4096 tokens of 16 requests, there and in the kernel for
+        // many: 14 rows 30 and 49 us; in a form that took several times 16 rows of a request, 21 rows 48 and 48, 35 rows 67 and 49; 20 rows over 32768 tokens of 4 requests 132 and 132.
         // The device finds the requests of each kernel; a batch of one has one.
         const long max_rows = static_cast<long>(plan_.most) * a.group;
-        const bool many = max_rows > kFewRows;
-        a.few_rows = many && plan_.n == 1 ? 0 : kFewRows;
+        const bool many = max_rows > tq::kFewRows;
+        a.few_rows = many && plan_.n == 1 ? 0 : tq::kFewRows;
         if (many) tq::launch_paged_prompt(a, dim_, max_rows, scratch_.as<char>() + prompt_scratch_, sms_, st);
-        if (a.few_rows) tq::launch_paged_attention(a, dim_, static_cast<int>(std::min<long>(max_rows, kFewRows)), scratch_.as<void>(), sms_, st);
+        if (a.few_rows) tq::launch_paged_attention(a, dim_, static_cast<int>(std::min<long>(max_rows, tq::kFewRows)), scratch_.as<void>(), sms_, st);
     }
     void check_status() {
         const unsigned int code = *static_cast<volatile unsigned int*>(h_status_);
@@ -206,10 +208,6 @@ public:
     }
 
 private:
-    // Query rows of a request (new tokens times query heads to a KV head) that the kernel for few rows takes, 16 at a time.  Over 4096 tokens of 16 requests, there and in the kernel for many:
-    // 14 rows 32 and 49 us, 21 rows 48 and 48, 35 rows 67 and 49; 20 rows over 32768 tokens of 4 requests 132 and 132.
-    static constexpr int kFewRows = 16;
-
     void check_layer(int layer) const { TQ_REQUIRE(layer >= 0 && layer < static_cast<int>(layers_.size()), "Layer index out of range"); }
     void begin(cudaStream_t st) {
         tq::ensure_device(device_);

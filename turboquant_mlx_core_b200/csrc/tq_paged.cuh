@@ -159,11 +159,12 @@ struct PagedAttnArgs {
     float scale_log2;    // softmax scale times log2(e)
     float* partial;
     PagedJoin* joins;
-    int join_items, row_tiles;   // few rows: entries of `joins` where each item has one (0: one for each CTA), and row tiles of a request at most
+    int join_items;      // few rows: entries of `joins` where each item has one (0: one for each CTA)
     unsigned int* status;
 };
 size_t paged_attn_scratch_bytes(int dim, int sms);
-// The requests of at most a.few_rows rows.
+// The requests of at most a.few_rows rows, which are kFewRows or, where no request has more (max_rows), fewer.
+constexpr int kFewRows = 16;
 void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratch, int sms, cudaStream_t st);
 // The others (tq_paged_prompt.cu).
 size_t paged_prompt_scratch_bytes(int dim, int sms);

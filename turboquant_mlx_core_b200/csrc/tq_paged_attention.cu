@@ -3,10 +3,10 @@
 //
 //   s = q . k scale,  o = sum softmax(s) v          q [tokens, heads * group, D] fp16, k and v code * 2^e of a page and head
 //
-// The query rows of a request and KV head are its new tokens times the heads of the group, token-major.  paged_attn_kernel takes them 8 or 16 at a time (8 NT; eight where no request has
-// more): the decode step's kernel, bound by the bytes of the cache.  Every CTA streams an equal share of all (request, KV head, 8 NT
-// rows, 64 tokens) units, whatever the requests' lengths, which only the device knows: it sums them up first and finds its share by
-// itself.  An item (request, KV head, 8 NT rows) that ends in another CTA than it begins in is added up by paged_join_kernel, in order.
+// The query rows of a request and KV head are its new tokens times the heads of the group, token-major; there are 16 at most here, and paged_attn_kernel has room for 8 or 16 (8 NT; eight
+// where no request has more): the decode step's kernel, bound by the bytes of the cache.  Every CTA streams an equal share of all (request, KV head, 64 tokens) units, whatever the
+// requests' lengths, which only the device knows: it sums them up first and finds its share by itself.  An item (request, KV head) that ends in another CTA than it begins in is added up
+// by paged_join_kernel, in order.
 //
 // One warp copies (bulk copies into a ring, an mbarrier per stage); four multiply, 16 tokens of a tile each, with a softmax of
 // their own, so that they meet only at an item's end.  Products are mma.sync.m16n8k16 on halves with the tokens (then the dims) as the 16 rows and the query rows as
@@ -36,7 +36,6 @@ using namespace paged_device;
 
 constexpr int kTileTokens = 64;       // tokens of a unit
 constexpr int kMulWarps = 4;
-constexpr int kLeastUnits = 1;        // of a CTA
 constexpr int kAttnThreads = 32 * (kMulWarps + 1);
 // The reference maximum of a row moves only when a score exceeds it by 2^kSlack: a vote instead of a reduction for most tiles.  Weights are held times 2^kOffset and at most
 // 2^15: halves that are normal numbers down to 2^-25 of the reference.
@@ -67,43 +66,38 @@ __device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t which) {
 __device__ __forceinline__ float unit_ratio(uint32_t lower, int r) {
     return __int_as_float(max(127 - static_cast<int>(lower >> (8 * r) & 0xffu), 0) << 23);
 }
-// A request's part of the work, in units: its tiles times its row tiles (times the KV heads).
+// A request's part of the work, in units: its tiles (times the KV heads).
 struct RequestWork {
-    int row, start, count, held, lo, hi;   // tiles lo .. hi - 1
-    int row_tiles;
-    __device__ __forceinline__ void load(const PagedAttnArgs& a, int i, int tile_rows) {
+    int row, start, count, held, lo, hi;   // tiles lo .. hi - 1 (none: not this kernel's)
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, int i) {
         row = a.b.rows[i];
         start = a.b.starts[i];
         count = a.b.starts[i + 1] - start;
         held = a.b.held[i];
         const int first = held - count;   // position of the first new token
         lo = a.window > 0 ? max(0, first - a.window + 1) / kTileTokens : 0;
-        hi = (held + kTileTokens - 1) / kTileTokens;
-        row_tiles = count * a.group <= a.few_rows ? (count * a.group + tile_rows - 1) / tile_rows : 0;
+        hi = count > 0 && count * a.group <= a.few_rows ? (held + kTileTokens - 1) / kTileTokens : lo;
     }
     // (A unit is some 8 KB of the cache at least, twice at most: all of them are a 32-bit number.)
-    __device__ __forceinline__ unsigned int units(int heads) const { return static_cast<unsigned int>(row_tiles * heads) * static_cast<unsigned int>(hi - lo); }
+    __device__ __forceinline__ unsigned int units(int heads) const { return static_cast<unsigned int>(heads) * static_cast<unsigned int>(hi - lo); }
 };
 
-// A CTA's share [u, end) of the units and where it stands in them: (request, KV head, row tile, tile), the tile running fastest.
-template <int ROWS>
+// A CTA's share [u, end) of the units and where it stands in them: (request, KV head, tile), the tile running fastest.
 struct Walker {
     RequestWork w;
-    int i, n, head, row_tile, tile;
+    int i, head, tile;
     unsigned int left;   // units of the share that are still to do, this item's included
     __device__ __forceinline__ void place(const PagedAttnArgs& a, int request, unsigned int skip, unsigned int units) {
         i = request;
         left = units;
-        w.load(a, i, ROWS);
+        w.load(a, i);
         while (skip >= w.units(a.heads)) {   // (the share begins inside a request that has units)
             skip -= w.units(a.heads);
-            w.load(a, ++i, ROWS);
+            w.load(a, ++i);
         }
         const unsigned int tiles = static_cast<unsigned int>(w.hi - w.lo);
         tile = w.lo + static_cast<int>(skip % tiles);
-        skip /= tiles;
-        head = static_cast<int>(skip / static_cast<unsigned int>(w.row_tiles));
-        row_tile = static_cast<int>(skip) - head * w.row_tiles;
+        head = static_cast<int>(skip / tiles);
     }
     // Tiles of the present item that belong to the share.
     __device__ __forceinline__ int run() const { return static_cast<int>(min(static_cast<unsigned int>(w.hi - tile), left)); }
@@ -111,13 +105,10 @@ struct Walker {
     __device__ __forceinline__ bool next(const PagedAttnArgs& a) {
         left -= static_cast<unsigned int>(run());
         if (left == 0) return false;
-        if (++row_tile == w.row_tiles) {
-            row_tile = 0;
-            if (++head == a.heads) {
-                head = 0;
-                do w.load(a, ++i, ROWS);
-                while (w.units(a.heads) == 0);
-            }
+        if (++head == a.heads) {
+            head = 0;
+            do w.load(a, ++i);
+            while (w.units(a.heads) == 0);
         }
         tile = w.lo;
         return true;
@@ -168,11 +159,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
         unsigned int mine = 0;
         for (int i = tid * per; i < min(a.sizes.n, (tid + 1) * per); ++i) {
             RequestWork w;
-            w.load(a, i, kRows);
+            w.load(a, i);
             const unsigned int units = i < requests ? w.units(a.heads) : 0u;
             mine += units;
             if (units == 0u && blockIdx.x == 0)   // (its items, which no CTA begins)
-                for (int k = i * a.heads * a.row_tiles; k < min((i + 1) * a.heads * a.row_tiles, a.join_items); ++k) a.joins[k].last = 0;
+                for (int k = i * a.heads; k < min((i + 1) * a.heads, a.join_items); ++k) a.joins[k].last = 0;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -188,12 +179,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
         before[k] = total;
         total += s_sum[32 * (k + 1)];
     }
-    const unsigned int ctas = min(gridDim.x, (total + kLeastUnits - 1) / kLeastUnits), c = blockIdx.x;
+    const unsigned int ctas = min(gridDim.x, total), c = blockIdx.x;
     if (tid == 0 && a.join_items == 0) a.joins[c].last = 0;
     if (c >= ctas) return;
     const unsigned int share = total / ctas, extra = total - share * ctas;   // the first `extra` CTAs have one unit more
     const unsigned int u0 = c * share + min(c, extra), u1 = u0 + share + (c < extra ? 1u : 0u);
-    Walker<kRows> at;
+    Walker at;
     {
         // the thread's range of requests in which the share begins: the last whose sum in front is at most u0
         int lo = 0, hi = kAttnThreads;
@@ -280,15 +271,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
     uint32_t s = 0, phase = 0;
     bool more = true, alive = true;
     while (more) {
-        const int rows = at.w.count * a.group, row0 = at.row_tile * kRows;
-        const int live_rows = min(kRows, rows - row0);
+        const int rows = at.w.count * a.group;
         const int first_pos = at.w.held - at.w.count;
         // queries, the products' second operand: lane (g, qd) holds row g of each eight, of every 16-byte chunk c = qd + 4 j of codes the products 4 j .. 4 j + 3
         uint32_t qf[NT][D / 16][2];
         int pos[NT][2];   // of the scores' rows 2 qd, 2 qd + 1
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int row = row0 + min(8 * nt + g, live_rows - 1), token = row / a.group, hq = at.head * a.group + row - token * a.group;
+            const int row = min(8 * nt + g, rows - 1), token = row / a.group, hq = at.head * a.group + row - token * a.group;
             // (rows behind the last: the last again, nobody reads their results)
             const __half* const src = a.q + (at.w.start + token) * a.q_stride + static_cast<long>(hq) * D + 16 * qd;
 #pragma unroll
@@ -306,9 +296,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                     qf[nt][4 * j + k][1] = v.y;
                 }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) pos[nt][e] = first_pos + (row0 + min(8 * nt + 2 * qd + e, live_rows - 1)) / a.group;
+            for (int e = 0; e < 2; ++e) pos[nt][e] = first_pos + min(8 * nt + 2 * qd + e, rows - 1) / a.group;
         }
-        const int pos_min = first_pos + row0 / a.group, pos_max = first_pos + (row0 + live_rows - 1) / a.group;
+        const int pos_min = first_pos, pos_max = first_pos + (rows - 1) / a.group;
 
         float o[NT][D / 16][4], m[NT][2], l[NT][2];
         // o is in units of the largest of the values' scales that its row has met: their exponents, a byte for each of the lane's rows (ONE: for all of them, the lowest byte).
@@ -504,8 +494,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 }
             }
             if (begins && ends) {
-                if (r < live_rows) {
-                    const int row = row0 + r, token = row / a.group, hq = at.head * a.group + row - token * a.group;
+                if (r < rows) {
+                    const int token = r / a.group, hq = at.head * a.group + r - token * a.group;
                     __half* const to = a.out + (at.w.start + token) * a.out_stride + static_cast<long>(hq) * D + d0;
                     const float inv = 1.f / sum;
 #pragma unroll
@@ -537,13 +527,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 last = static_cast<int>(unit < longer ? unit / (share + 1) : extra + (unit - longer) / share);
             }
             if (a.join_items) {
-                // (an item of fewer row tiles than there can be: the others' entries are never its own)
-                const int item = (at.i * a.heads + at.head) * a.row_tiles + at.row_tile;
-                a.joins[item] = {last, static_cast<int>(c), at.w.start, row0, live_rows, at.head};
-                if (at.row_tile == 0)
-                    for (int k = at.w.row_tiles; k < a.row_tiles; ++k) a.joins[item + k].last = 0;
+                a.joins[at.i * a.heads + at.head] = {last, static_cast<int>(c), at.w.start, 0, rows, at.head};
             } else if (last) {
-                a.joins[c] = {last, static_cast<int>(c), at.w.start, row0, live_rows, at.head};
+                a.joins[c] = {last, static_cast<int>(c), at.w.start, 0, rows, at.head};
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kMulWarps) : "memory");
@@ -610,18 +596,18 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
         all = fmaf(s_ml[w].y, x, all);
         value = fmaf(s_acc[w][d], x, value);
     }
-    const int row = join.first_row + r, token = row / a.group, hq = join.head * a.group + row - token * a.group;
+    const int token = r / a.group, hq = join.head * a.group + r - token * a.group;
     a.out[(join.token + token) * a.out_stride + static_cast<long>(hq) * D + d] = __float2half_rn(value / all);
     if (a.lse && d == 0) a.lse[(join.token + token) * static_cast<long>(a.heads * a.group) + hq] = (top - kOffset + log2f(all)) * 0.6931471805599453f;
 }
 
+static_assert(kFewRows <= AttnShape<128, 2>::kRows, "a request's rows are one item");
 template <int D, int NT>
 void launch_typed(PagedAttnArgs a, int max_rows, void* scratch, int sms, cudaStream_t st) {
     using S = AttnShape<D, NT>;
     const int ctas = sms * S::kCtas;
     // Items that there can be: where they are fewer than the CTAs each has its own entry, and the kernel behind as many CTAs.
-    a.row_tiles = (max_rows + S::kRows - 1) / S::kRows;
-    const long items = static_cast<long>(a.sizes.n) * a.heads * a.row_tiles;
+    const long items = static_cast<long>(a.sizes.n) * a.heads;
     a.join_items = items <= ctas ? static_cast<int>(items) : 0;
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (ctas * sizeof(PagedJoin) + 255) / 256 * 256);
@@ -649,7 +635,7 @@ size_t paged_attn_scratch_bytes(int dim, int sms) {
     return dim == 64 ? std::max(scratch_of<64, 1>(sms), scratch_of<64, 2>(sms)) : std::max(scratch_of<128, 1>(sms), scratch_of<128, 2>(sms));
 }
 void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratch, int sms, cudaStream_t st) {
-    // Eight rows at a time where no request has more: half the products and registers of sixteen.
+    // Room for eight rows where no request has more: half the products and registers of sixteen.
     const bool eight = max_rows <= 8;
     if (dim == 64) eight ? launch_typed<64, 1>(a, max_rows, scratch, sms, st) : launch_typed<64, 2>(a, max_rows, scratch, sms, st);
     else eight ? launch_typed<128, 1>(a, max_rows, scratch, sms, st) : launch_typed<128, 2>(a, max_rows, scratch, sms, st);
