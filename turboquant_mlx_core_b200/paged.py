@@ -9,7 +9,8 @@ their lengths on the device.  A step:
         cache.append(layer, k, v)
         cache.attention(layer, q, out=out)
 
-Tensors are torch CUDA tensors; rows, counts and lengths may be int32 numpy arrays.  Everything runs in the CUDA library.
+Tensors are torch CUDA tensors; rows, counts and lengths may be int32 numpy arrays, counts and lengths any whole numbers that fit.  Everything runs in the
+CUDA library.
 """
 from __future__ import annotations
 
@@ -29,6 +30,24 @@ def _load_torch():
         import torch
         _torch = torch
     return _torch
+
+
+def _fits(n, what):
+    """(The C interface takes the low 32 bits of any number.)"""
+    if -0x80000000 <= n <= 0x7fffffff:
+        return n
+    raise ValueError(f"{what} must fit in 32 bits, got {n}")
+
+
+def _host_ints(x, what):
+    """Whole numbers in host memory, of any integer type, as contiguous int32."""
+    x = np.asarray(x)
+    if x.dtype != np.int32 and x.size:
+        if x.dtype.kind not in "iu":
+            raise TypeError(f"{what} must be whole numbers, got {x.dtype}")
+        _fits(int(x.min()), what)
+        _fits(int(x.max()), what)
+    return np.ascontiguousarray(x, np.int32)
 
 
 def _ints(x, what, n):
@@ -92,10 +111,10 @@ class PagedKVCache:
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, num_pages: int, page_tokens: int = 64, max_requests: int = 256,
                  max_pages_per_request: int | None = None, max_tokens: int = 8192):
         self._L = _lib.load()
-        self.num_layers, self.num_heads, self.head_dim = int(num_layers), int(num_heads), int(head_dim)
-        self.num_pages, self.page_tokens, self.max_requests = int(num_pages), int(page_tokens), int(max_requests)
-        self.max_pages_per_request = self.num_pages if max_pages_per_request is None else int(max_pages_per_request)
-        self.max_tokens = int(max_tokens)
+        self.num_layers, self.num_heads, self.head_dim = _fits(int(num_layers), "num_layers"), _fits(int(num_heads), "num_heads"), _fits(int(head_dim), "head_dim")
+        self.num_pages, self.page_tokens = _fits(int(num_pages), "num_pages"), _fits(int(page_tokens), "page_tokens")
+        self.max_requests, self.max_tokens = _fits(int(max_requests), "max_requests"), _fits(int(max_tokens), "max_tokens")
+        self.max_pages_per_request = self.num_pages if max_pages_per_request is None else _fits(int(max_pages_per_request), "max_pages_per_request")
         self._h = self._L.tq_paged_cache_create(self.num_layers, self.num_heads, self.head_dim, self.num_pages, self.page_tokens,
                                                 self.max_requests, self.max_pages_per_request, self.max_tokens)
         if not self._h:
@@ -109,15 +128,17 @@ class PagedKVCache:
     def plan(self, counts, tokens: int | None = None, max_count: int | None = None, rows=None, starts=None, lengths=None, slots=None,
              positions=None, tables=None, stream=None):
         """counts[i] new tokens for the request in row rows[i] (row i without rows).  `tokens` and `max_count`: the most that there can be in
-        all and for one request (taken from counts where that is a numpy array).  starts [n + 1], lengths [n], slots [tokens],
+        all and for one request (taken from counts where that is in host memory: a numpy array or a list).  starts [n + 1], lengths [n], slots [tokens],
         positions [tokens] and tables [n, width]: int32 tensors that are filled, each of them optional."""
         if not hasattr(counts, "data_ptr"):
-            counts = np.ascontiguousarray(counts, np.int32)
+            counts = _host_ints(counts, "counts")
             tokens = int(counts.sum()) if tokens is None else tokens
             max_count = int(counts.max(initial=0)) if max_count is None else max_count
         elif tokens is None or max_count is None:
             raise ValueError("plan: counts on the device need tokens and max_count")
         n, width = counts.shape[0], 0
+        _fits(tokens, "tokens")
+        _fits(max_count, "max_count")
         if tables is not None:
             if len(tables.shape) != 2 or tables.shape[0] != n:
                 raise ValueError("plan: tables must be [n, width]")
@@ -130,7 +151,7 @@ class PagedKVCache:
     def truncate(self, lengths, rows=None, stream=None):
         """The request in row rows[i] (row i without rows) keeps its first lengths[i] tokens; 0 releases it."""
         if not hasattr(lengths, "data_ptr"):
-            lengths = np.ascontiguousarray(lengths, np.int32)
+            lengths = _host_ints(lengths, "lengths")
         n = lengths.shape[0]
         if self._L.tq_paged_truncate(self._h, _ints(rows, "rows", n), _ints(lengths, "lengths", n), n, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.truncate")
@@ -141,7 +162,7 @@ class PagedKVCache:
         vp, more, _, vs = _rows(values, self.num_heads, self.head_dim, "values")
         if tokens != more or keys.dtype is not values.dtype:
             raise ValueError("keys and values must have the same number of tokens and type")
-        if self._L.tq_paged_append(self._h, layer, kp, vp, _tag(keys, "append"), tokens, ks, vs, None if stream is None else _stream_ptr(stream)):
+        if self._L.tq_paged_append(self._h, _fits(layer, "layer"), kp, vp, _tag(keys, "append"), tokens, ks, vs, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.append")
 
     def attention(self, layer: int, queries, window: int = 0, scale: float = 0.0, out=None, lse=None, stream=None):
@@ -161,7 +182,7 @@ class PagedKVCache:
             if lse.dtype is not _torch.float32 or lse.shape != (tokens, q_heads) or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous float32 [tokens, q_heads]")
             lp = lse.data_ptr()
-        if self._L.tq_paged_attention(self._h, layer, qp, tokens, q_heads, qs, window, scale, op, os_, lp, None if stream is None else _stream_ptr(stream)):
+        if self._L.tq_paged_attention(self._h, _fits(layer, "layer"), qp, tokens, q_heads, qs, _fits(window, "window"), scale, op, os_, lp, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.attention")
         return out
 
@@ -177,7 +198,7 @@ class PagedKVCache:
             if tag not in (None, _tag(x, "read_pages")):
                 raise ValueError("keys and values must have the same type")
             tag, at[i] = _tag(x, "read_pages"), x.data_ptr()
-        if self._L.tq_paged_read(self._h, layer, _ints(pages, "pages", n), n, *at, TQ_F16 if tag is None else tag,
+        if self._L.tq_paged_read(self._h, _fits(layer, "layer"), _ints(pages, "pages", n), n, *at, TQ_F16 if tag is None else tag,
                                  None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.read_pages")
 
