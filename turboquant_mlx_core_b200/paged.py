@@ -21,14 +21,14 @@ from ._lib import TQ_F16, TQ_F32, TQError, check
 from .api import _stream_ptr
 
 # A decode step's calls move microseconds of work each: their Python side is a handful of look-ups, and types are told by identity.
-_torch = None
+_torch = _int32 = _float16 = _float32 = None
 
 
 def _load_torch():
-    global _torch
+    global _torch, _int32, _float16, _float32
     if _torch is None:
         import torch
-        _torch = torch
+        _torch, _int32, _float16, _float32 = torch, torch.int32, torch.float16, torch.float32
     return _torch
 
 
@@ -50,12 +50,21 @@ def _host_ints(x, what):
     return np.ascontiguousarray(x, np.int32)
 
 
-def _ints(x, what, n):
+def _elsewhere(x, device, what):
+    """A tensor that is not on the cache's device: in host memory (the C interface takes or refuses it) or on another one."""
+    if x.get_device() >= 0:
+        raise ValueError(f"{what} is on cuda:{x.get_device()}, the cache on cuda:{device}")
+
+
+def _ints(x, what, n, device):
     """Address of n whole numbers of 32 bits, contiguous."""
     if x is None:
         return None
-    if hasattr(x, "data_ptr"):
-        fine, contiguous, size, at = x.dtype is _torch.int32, x.is_contiguous(), x.numel(), x.data_ptr()
+    its = getattr(x, "get_device", None)
+    if its is not None:
+        if its() != device:
+            _elsewhere(x, device, what)
+        fine, contiguous, size, at = x.dtype is _int32, x.is_contiguous(), x.numel(), x.data_ptr()
     else:
         fine, contiguous, size, at = x.dtype == np.int32, x.flags["C_CONTIGUOUS"], x.size, x.ctypes.data
     if not fine:
@@ -67,10 +76,13 @@ def _ints(x, what, n):
     return at
 
 
-def _rows(x, heads, dim, what):
+def _rows(x, heads, dim, what, device):
     """[tokens, heads, dim] with contiguous heads (`heads` 0: any number of them): address, tokens, heads, elements from token to token."""
-    if not hasattr(x, "data_ptr"):
+    its = getattr(x, "get_device", None)
+    if its is None:
         raise TypeError(f"{what} must be a torch CUDA tensor")
+    if its() != device:
+        _elsewhere(x, device, what)
     try:
         tokens, n, d = x.shape
         step, head, one = x.stride()
@@ -84,9 +96,9 @@ def _rows(x, heads, dim, what):
 
 
 def _tag(x, what):
-    if x.dtype is _torch.float16:
+    if x.dtype is _float16:
         return TQ_F16
-    if x.dtype is _torch.float32:
+    if x.dtype is _float32:
         return TQ_F32
     raise TypeError(f"{what}: expected float32 or float16, got {x.dtype}")
 
@@ -106,7 +118,9 @@ def _zeros_like(x, stream):
 
 class PagedKVCache:
     """Keys and values of up to `max_requests` requests in `num_pages` pages of `page_tokens` tokens, 8 bits each with a power of
-    two for each page and head."""
+    two for each page and head, on the device that is current here."""
+
+    _device = -1       # no CUDA device's number
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, num_pages: int, page_tokens: int = 64, max_requests: int = 256,
                  max_pages_per_request: int | None = None, max_tokens: int = 8192):
@@ -119,7 +133,7 @@ class PagedKVCache:
                                                 self.max_requests, self.max_pages_per_request, self.max_tokens)
         if not self._h:
             raise TQError("PagedKVCache: " + _lib.last_error())
-        _load_torch()
+        self._device = _load_torch().cuda.current_device()
 
     @property
     def handle(self):
@@ -137,15 +151,17 @@ class PagedKVCache:
         elif tokens is None or max_count is None:
             raise ValueError("plan: counts on the device need tokens and max_count")
         n, width = counts.shape[0], 0
-        _fits(tokens, "tokens")
-        _fits(max_count, "max_count")
+        if not 0 <= tokens <= 0x7fffffff or not 0 <= max_count <= 0x7fffffff:
+            _fits(tokens, "tokens")
+            _fits(max_count, "max_count")
         if tables is not None:
             if len(tables.shape) != 2 or tables.shape[0] != n:
                 raise ValueError("plan: tables must be [n, width]")
             width = tables.shape[1]
-        if self._L.tq_paged_plan(self._h, _ints(rows, "rows", n), _ints(counts, "counts", n), n, tokens, max_count, _ints(starts, "starts", n + 1),
-                                 _ints(lengths, "lengths", n), _ints(slots, "slots", tokens), _ints(positions, "positions", tokens),
-                                 _ints(tables, "tables", n * width), width, None if stream is None else _stream_ptr(stream)):
+        on = self._device
+        if self._L.tq_paged_plan(self._h, _ints(rows, "rows", n, on), _ints(counts, "counts", n, on), n, tokens, max_count, _ints(starts, "starts", n + 1, on),
+                                 _ints(lengths, "lengths", n, on), _ints(slots, "slots", tokens, on), _ints(positions, "positions", tokens, on),
+                                 _ints(tables, "tables", n * width, on), width, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.plan")
 
     def truncate(self, lengths, rows=None, stream=None):
@@ -153,36 +169,43 @@ class PagedKVCache:
         if not hasattr(lengths, "data_ptr"):
             lengths = _host_ints(lengths, "lengths")
         n = lengths.shape[0]
-        if self._L.tq_paged_truncate(self._h, _ints(rows, "rows", n), _ints(lengths, "lengths", n), n, None if stream is None else _stream_ptr(stream)):
+        on = self._device
+        if self._L.tq_paged_truncate(self._h, _ints(rows, "rows", n, on), _ints(lengths, "lengths", n, on), n, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.truncate")
 
     def append(self, layer: int, keys, values, stream=None):
         """Keys and values of the planned tokens, [tokens, heads, head_dim] fp32 or fp16; a token's heads are contiguous, tokens may be apart."""
-        kp, tokens, _, ks = _rows(keys, self.num_heads, self.head_dim, "keys")
-        vp, more, _, vs = _rows(values, self.num_heads, self.head_dim, "values")
+        kp, tokens, _, ks = _rows(keys, self.num_heads, self.head_dim, "keys", self._device)
+        vp, more, _, vs = _rows(values, self.num_heads, self.head_dim, "values", self._device)
         if tokens != more or keys.dtype is not values.dtype:
             raise ValueError("keys and values must have the same number of tokens and type")
-        if self._L.tq_paged_append(self._h, _fits(layer, "layer"), kp, vp, _tag(keys, "append"), tokens, ks, vs, None if stream is None else _stream_ptr(stream)):
+        if not 0 <= layer <= 0x7fffffff:
+            _fits(layer, "layer")
+        if self._L.tq_paged_append(self._h, layer, kp, vp, _tag(keys, "append"), tokens, ks, vs, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.append")
 
     def attention(self, layer: int, queries, window: int = 0, scale: float = 0.0, out=None, lse=None, stream=None):
         """Causal attention of the planned tokens' queries, fp16 [tokens, q_heads, head_dim], over their requests; returns out.  A `window` of w
         lets a token see itself and the w - 1 before it.  lse: fp32 [tokens, q_heads], filled with the log of the softmax denominators."""
-        qp, tokens, q_heads, qs = _rows(queries, 0, self.head_dim, "queries")
-        half = _torch.float16
-        if queries.dtype is not half:
+        qp, tokens, q_heads, qs = _rows(queries, 0, self.head_dim, "queries", self._device)
+        if queries.dtype is not _float16:
             raise TypeError("attention: queries must be float16")
         if out is None:
             out = _zeros_like(queries, stream)
-        op, more, _, os_ = _rows(out, q_heads, self.head_dim, "out")
-        if more != tokens or out.dtype is not half:
+        op, more, _, os_ = _rows(out, q_heads, self.head_dim, "out", self._device)
+        if more != tokens or out.dtype is not _float16:
             raise ValueError("out must be float16 of the queries' shape")
         lp = None
         if lse is not None:
-            if lse.dtype is not _torch.float32 or lse.shape != (tokens, q_heads) or not lse.is_contiguous():
+            if lse.dtype is not _float32 or lse.shape != (tokens, q_heads) or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous float32 [tokens, q_heads]")
+            if lse.get_device() != self._device:
+                _elsewhere(lse, self._device, "lse")
             lp = lse.data_ptr()
-        if self._L.tq_paged_attention(self._h, _fits(layer, "layer"), qp, tokens, q_heads, qs, _fits(window, "window"), scale, op, os_, lp, None if stream is None else _stream_ptr(stream)):
+        if not 0 <= layer <= 0x7fffffff or not 0 <= window <= 0x7fffffff:
+            _fits(layer, "layer")
+            _fits(window, "window")
+        if self._L.tq_paged_attention(self._h, layer, qp, tokens, q_heads, qs, window, scale, op, os_, lp, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.attention")
         return out
 
@@ -197,8 +220,10 @@ class PagedKVCache:
                 raise ValueError(f"keys and values must be contiguous {[n, self.page_tokens, self.num_heads, self.head_dim]}")
             if tag not in (None, _tag(x, "read_pages")):
                 raise ValueError("keys and values must have the same type")
+            if x.get_device() != self._device:
+                _elsewhere(x, self._device, "keys and values")
             tag, at[i] = _tag(x, "read_pages"), x.data_ptr()
-        if self._L.tq_paged_read(self._h, _fits(layer, "layer"), _ints(pages, "pages", n), n, *at, TQ_F16 if tag is None else tag,
+        if self._L.tq_paged_read(self._h, _fits(layer, "layer"), _ints(pages, "pages", n, self._device), n, *at, TQ_F16 if tag is None else tag,
                                  None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.read_pages")
 
