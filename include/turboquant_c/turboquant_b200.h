@@ -539,14 +539,20 @@ int tq_hybrid_attention(tq_kv_cache_t cache, tq_decode_buffer_t buf, int layer, 
  * Keys and values are held as whole numbers -127 .. 127 times a power of two for each page and KV head, keys and values apart: the
  * smallest 2^e, e >= -100, with which the largest magnitude does not round to more than 127 (to the nearest, ties to even).  Tokens
  * that join a page which holds older ones make its scale larger where they need to, never smaller, and the older numbers are then
- * rounded once more (truncation leaves scales as they are).  A NaN or an infinity makes the scale of its page and head NaN, and with it every row of the attention that
- * sees a token of that page and head, until the page is begun anew.
+ * rounded once more.  A NaN or an infinity makes the scale of its page and head NaN, and with it every row of the attention that sees a
+ * token of that page and head, until the page is begun anew.  Truncation leaves scales as they are: a token that is taken back again (a
+ * rejected draft) leaves the kept ones of its page at its coarser scale, or not numbers.
+ *
+ * A number that joins a page is off by half its scale at most, and by its largest magnitude's 127.5th part at most where the page's tokens
+ * come at once.  Normally distributed keys and values (pages of 64 tokens, 128 dims) are 1.4 % of their norm off, those of unequal
+ * strength from channel to channel and token to token (factors e^0.4 and e^0.5, normally distributed logarithms) 3 to 4 %; attention over
+ * 4096 such tokens 2.0 % and 2.9 %.  (The 3.5-bit cache, tq_kv_*, at the same numbers: 18 %, and 21 to 33 %.)
  *
  * A step is a plan, then an append and an attention per layer, in stream order.  All calls on a cache must be ordered (one stream, or
- * events between streams); they work on the cache's device whichever is current.  Data pointers are device pointers, except for rows, counts and
- * lengths, which may be host memory, read before the call returns, where the stream is not being captured.  A captured graph that appends or attends holds
- * its plan too, and ends the one in force: an append or attention behind a replay that was made for a plan of other sizes (n, tokens,
- * max_count) does nothing, and tq_paged_status tells. */
+ * events between streams); they work on the cache's device whichever is current.  Data pointers are device pointers that this device can
+ * use, except for rows, counts and lengths, which may be host memory, read before the call returns, where the stream is not being
+ * captured.  A captured graph that appends or attends holds its plan too, and ends the one in force: an append or attention behind a replay
+ * that was made for a plan of other sizes (n, tokens, max_count) does nothing, and tq_paged_status tells. */
 typedef struct tq_paged_cache_s* tq_paged_cache_t;
 
 /** head_dim 64 or 128; num_heads up to 65536; max_requests (rows of the block tables) up to 4096; max_tokens: new tokens of a plan at most.  All
@@ -581,9 +587,13 @@ int tq_paged_read(tq_paged_cache_t cache, int layer, const int* pages, int n, vo
  *  max(0, p - window + 1) .. p, all up to p with window 0.  q_heads is a multiple of the KV heads, whose groups are
  *  contiguous.  scale 0: 1 / sqrt(head_dim).  out fp16 of the queries' shape, strides in elements from token to token; lse
  *  (may be NULL): fp32 [tokens, q_heads], the log of each softmax denominator, with which parts merge
- *  (tq_exchange_merge_attention).  Rows behind the last request's are left as they are.  Results do not depend on the order in which CTAs run.  Where a
- *  request has more than 16 query rows (new tokens times the group), the pages of 64 tokens in a row are taken together: numbers of a page whose scale is 2^29 below the largest
- *  among them count as 0. */
+ *  (tq_exchange_merge_attention).  Rows behind the last request's are left as they are.  Results do not depend on the order in which
+ *  CTAs run.
+ *
+ *  Scores, softmax and sums are fp32 (a score beyond its range makes its row NaN); the weights are rounded to halves for their product
+ *  with the values: 2^-11 of each at most, and of small ones 2^-36 of the row's largest weight, times the largest scale among the values that the
+ *  row sees.  Where a request has more than 16 query rows (new tokens times the group) that is 2^-32, and the pages of 64 tokens in a row
+ *  are taken together: the numbers of a page whose scale is more than 2^29 below the largest among them, seen or not, count as 0. */
 int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window,
                        float scale, void* out_fp16, long out_stride, float* lse, void* stream);
 /** Non-zero, once, when a call that has finished found its batch impossible or another plan on the device than the one that it was made for, or a wait

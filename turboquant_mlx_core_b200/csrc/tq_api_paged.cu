@@ -178,9 +178,10 @@ public:
         a.page_shift = b_.page_tokens == 16 ? 4 : b_.page_tokens == 32 ? 5 : b_.page_tokens == 64 ? 6 : 7;
         a.scale_log2 = static_cast<float>((scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(dim_))) * 1.4426950408889634);
         a.status = d_status_;
-        // Up to kFewRows query rows of a request (new tokens times query heads to a KV head) go to the kernel for few rows.  Over 4096 tokens of 16 requests, there and in the kernel for
-        // many: 14 rows 30 and 49 us; in a form that took several times 16 rows of a request, 21 rows 48 and 48, 35 rows 67 and 49; 20 rows over 32768 tokens of 4 requests 132 and 132.
-        // The device finds the requests of each kernel; a batch of one has one.
+        // Up to kFewRows query rows of a request (new tokens times query heads to a KV head) go to the kernel for few rows.  Over 4096 tokens of 16
+        // requests, there and in the kernel for many: 14 rows 30 and 49 us; in a form that took several times 16 rows of a request, 21 rows 48 and
+        // 48, 35 rows 67 and 49; 20 rows over 32768 tokens of 4 requests 132 and 132. The device finds the requests of each kernel; a batch of one
+        // has one.
         const long max_rows = static_cast<long>(plan_.most) * a.group;
         const bool many = max_rows > tq::kFewRows;
         a.few_rows = many && plan_.n == 1 ? 0 : tq::kFewRows;

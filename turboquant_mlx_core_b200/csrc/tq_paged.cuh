@@ -173,8 +173,8 @@ void launch_paged_prompt(PagedAttnArgs a, int dim, long max_rows, void* scratch,
 // ---- what the attention kernels share -------------------------------------------------------------
 namespace paged_device {
 
-// Requests and pieces of the plan on the device; none, with a status, where it is of other sizes than the launch (a captured step came between a plan and the call): the launch's grid, its
-// choice of kernels and the caller's rows need not fit it.
+// Requests and pieces of the plan on the device; none, with a status, where it is of other sizes than the launch (a captured step came between a plan
+// and the call): the launch's grid, its choice of kernels and the caller's rows need not fit it.
 struct Planned {
     int requests, pieces;
 };

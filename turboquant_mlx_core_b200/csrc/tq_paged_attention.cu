@@ -1,25 +1,26 @@
-// Attention over the paged 8-bit KV cache: the new tokens' queries against all tokens of their request up to their own; here
-// requests of few query rows (tq_paged_prompt.cu: many).
+// Attention over the paged 8-bit KV cache: the new tokens' queries against all tokens of their request up to their own; here requests of few query
+// rows (tq_paged_prompt.cu: many).
 //
 //   s = q . k scale,  o = sum softmax(s) v          q [tokens, heads * group, D] fp16, k and v code * 2^e of a page and head
 //
-// The query rows of a request and KV head are its new tokens times the heads of the group, token-major; there are 16 at most here, and paged_attn_kernel has room for 8 or 16 (8 NT; eight
-// where no request has more): the decode step's kernel, bound by the bytes of the cache.  Every CTA streams an equal share of all (request, KV head, 64 tokens) units, whatever the
-// requests' lengths, which only the device knows: it sums them up first and finds its share by itself.  An item (request, KV head) that ends in another CTA than it begins in is added up
-// by paged_join_kernel, in order.
+// The query rows of a request and KV head are its new tokens times the heads of the group, token-major; there are 16 at most here, and
+// paged_attn_kernel has room for 8 or 16 (8 NT; eight where no request has more): the decode step's kernel, bound by the bytes of the cache.  Every
+// CTA streams an equal share of all (request, KV head, 64 tokens) units, whatever the requests' lengths, which only the device knows: it sums them up
+// first and finds its share by itself.  An item (request, KV head) that ends in another CTA than it begins in is added up by paged_join_kernel, in
+// order.
 //
-// One warp copies (bulk copies into a ring, an mbarrier per stage); four multiply, 16 tokens of a tile each, with a softmax of
-// their own, so that they meet only at an item's end.  Products are mma.sync.m16n8k16 on halves with the tokens (then the dims) as the 16 rows and the query rows as
-// the 8 columns, so that few query rows leave nothing idle; into the halves the codes go exactly:
-// a byte b = code + 128 becomes the half 1024 + b by a byte permutation, and 1152 is taken off.  The order of the dims inside a
-// product is free as long as both operands share it: a lane takes the 16 dims of one 16-byte chunk.  (tcgen05 would need the operands
-// in shared or tensor memory, behind a barrier for every tile, and 8 query rows leave most of its tile idle.)
+// One warp copies (bulk copies into a ring, an mbarrier per stage); four multiply, 16 tokens of a tile each, with a softmax of their own, so that
+// they meet only at an item's end.  Products are mma.sync.m16n8k16 on halves with the tokens (then the dims) as the 16 rows and the query rows as the
+// 8 columns, so that few query rows leave nothing idle; into the halves the codes go exactly: a byte b = code + 128 becomes the half 1024 + b by a
+// byte permutation, and 1152 is taken off.  The order of the dims inside a product is free as long as both operands share it: a lane takes the 16
+// dims of one 16-byte chunk.  (tcgen05 would need the operands in shared or tensor memory, behind a barrier for every tile, and 8 query rows leave
+// most of its tile idle.)
 //
-// Rounding: products of halves are exact and summed in fp32; the softmax is fp32; the weights are rounded to halves for the second product
-// (times 2^11, with a reference that lags by up to 2^4), their sum is taken before that.
+// Rounding: products of halves are exact and summed in fp32; the softmax is fp32; the weights are rounded to halves for the second product (times
+// 2^11, with a reference that lags by up to 2^4), their sum is taken before that.
 //
-// Measured, a new token each with 8 KV heads of 128 and a group of 5: 32 requests of 395 thousand tokens in all (809 MB) 148 us, 5.5 TB/s, 84 % of a copy's rate; two requests of 117 thousand in all
-// 48 us, 76 %.  (Query rows as the 16 rows of the product, most of them empty: 226 and 78 us.)
+// Measured, a new token each with 8 KV heads of 128 and a group of 5: 32 requests of 395 thousand tokens in all (809 MB) 148 us, 5.5 TB/s, 84 % of a
+// copy's rate; two requests of 117 thousand in all 48 us, 76 %.  (Query rows as the 16 rows of the product, most of them empty: 226 and 78 us.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -37,8 +38,8 @@ using namespace paged_device;
 constexpr int kTileTokens = 64;       // tokens of a unit
 constexpr int kMulWarps = 4;
 constexpr int kAttnThreads = 32 * (kMulWarps + 1);
-// The reference maximum of a row moves only when a score exceeds it by 2^kSlack: a vote instead of a reduction for most tiles.  Weights are held times 2^kOffset and at most
-// 2^15: halves that are normal numbers down to 2^-25 of the reference.
+// The reference maximum of a row moves only when a score exceeds it by 2^kSlack: a vote instead of a reduction for most tiles.  Weights are held
+// times 2^kOffset and at most 2^15: halves that are normal numbers down to 2^-25 of the reference.
 constexpr float kOffset = 11.f, kSlack = 4.f;
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -129,9 +130,9 @@ struct AttnShape {
     static constexpr int kPart = kRows * (D + 2);   // floats of a part: rows, then (maximum, sum) of each
 };
 
-// ONE: every request has one new token, so that its rows see the same and one unit of the values does for all of them.  Otherwise a window's or the drafts' end may lie between
-// rows, and each has its own.  (Its own for single tokens too: 32 requests of 197 thousand tokens in all, 16 rows to each of 4 heads, 71.3 us for 68.3; of 395 thousand, 5 rows to each of 8,
-// 135.6 for 134.3.)
+// ONE: every request has one new token, so that its rows see the same and one unit of the values does for all of them.  Otherwise a window's or the
+// drafts' end may lie between rows, and each has its own.  (Its own for single tokens too: 32 requests of 197 thousand tokens in all, 16 rows to
+// each of 4 heads, 69.1 us for 67.1; of 395 thousand, 5 rows to each of 8, 135.2 for 133.9.)
 template <int D, int NT, bool ONE>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     using S = AttnShape<D, NT>;
@@ -253,7 +254,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
                 raise_status(a.status, kPagedWait);
             }
         }
-        // Copies on their way land before the CTA's memory is another's: also where a multiplying warp gives up when all have been issued.  (The flag does not cut this short.)
+        // Copies on their way land before the CTA's memory is another's: also where a multiplying warp gives up when all have been issued.  (The flag
+        // does not cut this short.)
         unsigned int never = 0;
         for (int k = 0; k < issued; ++k) {
             if (s == 0) phase ^= 1;
@@ -273,7 +275,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
     while (more) {
         const int rows = at.w.count * a.group;
         const int first_pos = at.w.held - at.w.count;
-        // queries, the products' second operand: lane (g, qd) holds row g of each eight, of every 16-byte chunk c = qd + 4 j of codes the products 4 j .. 4 j + 3
+        // queries, the products' second operand: lane (g, qd) holds row g of each eight, of every 16-byte chunk c = qd + 4 j of codes the products 4
+        // j .. 4 j + 3
         uint32_t qf[NT][D / 16][2];
         int pos[NT][2];   // of the scores' rows 2 qd, 2 qd + 1
 #pragma unroll
@@ -301,7 +304,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
         const int pos_min = first_pos, pos_max = first_pos + (rows - 1) / a.group;
 
         float o[NT][D / 16][4], m[NT][2], l[NT][2];
-        // o is in units of the largest of the values' scales that its row has met: their exponents, a byte for each of the lane's rows (ONE: for all of them, the lowest byte).
+        // o is in units of the largest of the values' scales that its row has met: their exponents, a byte for each of the lane's rows (ONE: for all
+        // of them, the lowest byte).
         uint32_t units = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -537,9 +541,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<D, NT>::kCtas) paged_a
     }
 }
 
-// Parts of an item that several CTAs share, a CTA per item and row: eight warps take an eighth of the parts each, in the CTAs' order, and are added up in theirs.  It is bound by
-// the latency of one load behind another, of which 8 parts' of a warp are on their way at once.  (A CTA per item: what one SM fetches from the L2 cache bounds it, 65 parts of a
-// single request 13 -> 14.5 us.)
+// Parts of an item that several CTAs share, a CTA per item and row: eight warps take an eighth of the parts each, in the CTAs' order, and are added
+// up in theirs.  It is bound by the latency of one load behind another, of which 8 parts' of a warp are on their way at once.  (A CTA per item: what
+// one SM fetches from the L2 cache bounds it, 65 parts of a single request 13 -> 14.5 us.)
 constexpr int kJoinWarps = 8;
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {

@@ -78,11 +78,12 @@ __device__ __forceinline__ bool seen_before(unsigned int* seen, int row) {
     return (atomicOr(&seen[row >> 5], bit) & bit) != 0;
 }
 
-// Every CTA reads all requests and takes the sums over them (4096 at most, from the L2 cache), and the CTAs share the output: tokens, pieces, new pages and the
-// tables' copy, each element found by a binary search in the sums.  All or nothing: a batch that does not fit leaves the cache as it was, an empty plan and a
-// status.  COMMIT: one cluster, behind whose barrier nobody reads the lengths and the number of free pages any more, which then change.  It is bound by latency: a
-// launch, two dependent loads, the sums' barriers.  Much output is written by as many CTAs as there are SMs (OUTPUT), with no barrier between them, in front of a cluster that only
-// commits (61 prompts of up to 8192 tokens, 3 MB: 54 us with one cluster of eight for both, 13 so).
+// Every CTA reads all requests and takes the sums over them (4096 at most, from the L2 cache), and the CTAs share the output: tokens, pieces, new
+// pages and the tables' copy, each element found by a binary search in the sums.  All or nothing: a batch that does not fit leaves the cache as it
+// was, an empty plan and a status.  COMMIT: one cluster, behind whose barrier nobody reads the lengths and the number of free pages any more, which
+// then change.  It is bound by latency: a launch, two dependent loads, the sums' barriers.  Much output is written by as many CTAs as there are SMs
+// (OUTPUT), with no barrier between them, in front of a cluster that only commits (61 prompts of up to 8192 tokens, 3 MB: 54 us with one cluster of
+// eight for both, 13 so).
 template <bool OUTPUT, bool COMMIT>
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs a) {
     pdl_wait_release();
@@ -381,9 +382,9 @@ __device__ __forceinline__ void decode16(float (&v)[16], const uint4& c, float s
     for (int j = 0; j < 16; ++j) v[j] = static_cast<float>(static_cast<int>((w[j >> 2] >> (8 * (j & 3))) & 255u) - 128) * scale;
 }
 
-// A warp (for the few tokens of a decode step, four jobs to a CTA) or a CTA writes one piece's tokens of one head's keys or values: largest magnitude, scale, codes.  A thread takes 16
-// dims of ITER tokens, all asked for at once, which stay in registers (read twice, the second time from the caches, 67 thousand fp32 tokens of 8 heads took 145 us).
-// Older tokens of the page are read only where its scale grows.
+// A warp (for the few tokens of a decode step, four jobs to a CTA) or a CTA writes one piece's tokens of one head's keys or values: largest
+// magnitude, scale, codes.  A thread takes 16 dims of ITER tokens, all asked for at once, which stay in registers (read twice, the second time from
+// the caches, 67 thousand fp32 tokens of 8 heads took 145 us). Older tokens of the page are read only where its scale grows.
 template <int D, typename T, bool WIDE, bool WARP, int ITER>
 __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedAppendArgs a) {
     constexpr int kThreads = WARP ? 32 : 256, kChunks = D / 16, kRows = kThreads / kChunks;

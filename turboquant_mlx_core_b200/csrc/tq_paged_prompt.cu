@@ -1,35 +1,41 @@
-// Attention over the paged 8-bit KV cache for many query rows of a request: prompts, chunks of them, drafts of several
-// tokens.  The products are tcgen05.mma with S, P and O in tensor memory.
+// Attention over the paged 8-bit KV cache for many query rows of a request: prompts, chunks of them, drafts of several tokens.  The products are
+// tcgen05.mma with S, P and O in tensor memory.
 //
-// The rows of a request and KV head (new tokens times the heads of the group, token-major) go in items of 256: two tiles of 128, whose softmaxes run in
-// turn with each other's products.  The cache comes in tiles of 64 tokens.  As in tq_paged_attention.cu every CTA, one to an SM, takes an equal share of
-// all (request, KV head, 256 rows, 64 tokens) units, an item's beginning and end counted as kItemUnits more, and an item that ends in another CTA than it begins in is added up behind.
+// The rows of a request and KV head (new tokens times the heads of the group, token-major) go in items of 256: two tiles of 128, whose softmaxes run
+// in turn with each other's products.  The cache comes in tiles of 64 tokens.  As in tq_paged_attention.cu every CTA, one to an SM, takes an equal
+// share of all (request, KV head, 256 rows, 64 tokens) units, an item's beginning and end counted as kItemUnits more, and an item that ends in
+// another CTA than it begins in is added up behind.
 //
 //   S_t [128 x 64]   = Q_t [128 x D] (shared memory) . K [64 x D]^T (shared memory)         fp16 products, fp32 sums; two of them in turn for each t
 //   P_t              = 2^(S_t f - m + 7)  fp16, over S_t's own columns of tensor memory
 //   O_t [128 x D]   += P_t (tensor memory) . V (shared memory, transposed: rows are dims)
 //
-//   warps 0-3, 4-7   tile 0, tile 1: a thread per row reads its 64 scores once, keeps them in registers for the largest one and the weights, and writes its result
-//   warps 8, 9       one lane issues the scores' products, the values'; the commit behind P_t(j) V(j) also says that O_t may be rescaled, and that the scores of two tiles on may go where
-//                    P_t(j) was.  The products of the next item's first scores follow the last of this one's without a pause, while the softmax warps still write the results
+//   warps 0-3, 4-7   tile 0, tile 1: a thread per row reads its 64 scores once, keeps them in registers for the largest one and the weights, and
+//                    writes its result
+//   warps 8, 9       one lane issues the scores' products, the values'; the commit behind P_t(j) V(j) also says that O_t may be rescaled, and that
+//                    the scores of two tiles on may go where P_t(j) was.  The products of the next item's first scores follow the last of this one's
+//                    without a pause, while the softmax warps still write the results
 //   warp 10          walks the CTA's share and tells the others, item by item, what is next (four items ahead at most)
 //   warps 12-15      queries of tile 0, tile 1, of the next item as soon as the last scores of this one are there
 //   warps 16-23      keys: bytes to shared memory a tile ahead, then as halves (code * 2^(e - e_max + 5), exact) to their place for the products
 //   warps 24-31      values, transposed on the way; both in two groups that take every second tile
 //
-// Scales are powers of two: within a tile the pages' go into the halves without a rounding (but for codes 2^29 below the tile's largest scale), the tile's own goes into the
-// exponent's factor (keys) or, as an integer, into the exponent (values: P V is kept in units of the largest scale that the row has seen).  The reference maximum m
-// moves only when a score exceeds it by 2^8; weights are at most 2^15 then.  Where keys are of unequal strength one of a warp's 32 rows often has such a score (simulated, with norms spread by e^0.5: in 12 of
-// 63 tiles, in 19 with 2^4), and its O is then read, multiplied and written back, behind the weights, so that the products before it end meanwhile: 4096 such tokens 181 us, 190 with 2^4,
-// 199 with that and O in front of the weights; 175 where no row moves.
+// Scales are powers of two: within a tile the pages' go into the halves without a rounding (but for those of pages more than 2^29 below the tile's
+// largest), the tile's own goes into the exponent's factor (keys) or, as an integer, into the exponent (values: P V is kept in units of the largest
+// scale that the row has seen).  The reference maximum m moves only when a score exceeds it by 2^8; weights are at most 2^15 then.  Where keys are of
+// unequal strength one of a warp's 32 rows often has such a score (simulated, with norms spread by e^0.5: in 12 of 63 tiles, in 19 with 2^4), and its
+// O is then read, multiplied and written back, behind the weights, so that the products before it end meanwhile: 4096 such tokens 181 us, 190 with
+// 2^4, 199 with that and O in front of the weights; 175 where no row moves.
 //
-// What bounds it: 256 rows against 64 tokens (D = 128) take 2.7 thousand cycles.  A softmax warp is at work for 2.3 of them, waits for scores for 0.3 and writes results for 0.2; the products alone would take 1.24 (the scores'
-// 64 columns read 6 KB of shared memory in the 32 cycles that their arithmetic takes, 48 in fact), the exponentials alone 1.02, the softmax of both tiles with nothing beside it 1.17, all
-// roles' instructions fill 54 % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 175 us, 0.69 PFLOP/s of the
-// causal products, 41 % of a plain matrix product's rate.  Tried beside it, of the same prompt when it took 183: scores read twice in loops of 32 columns, a third less code, 191; two warps to a
-// row's 64 scores and half as many for the conversions 195; keys and values two tiles ahead 185.  Tiles of 128 tokens with one set of scores and one thread for all products: 699 for 8192 tokens, 668
-// with these.  Part of what the softmax takes longer here than alone is the supply of its instructions: copies of its step in a row, alone, 771 cycles each while the code is below 20 KB, 933 at 37 KB, 1100
-// at 68 KB and 2045 at 147 KB; the roles' loops here are some 30 KB together.
+// What bounds it: 256 rows against 64 tokens (D = 128) take 2.7 thousand cycles.  A softmax warp is at work for 2.3 of them, waits for scores for 0.3
+// and writes results for 0.2; the products alone would take 1.24 (the scores' 64 columns read 6 KB of shared memory in the 32 cycles that their
+// arithmetic takes, 48 in fact), the exponentials alone 1.02, the softmax of both tiles with nothing beside it 1.17, all roles' instructions fill 54
+// % of the issue slots and the tensor cores and the conversions together 75 % of shared memory's cycles.  4096 new tokens of 4 x 7 heads: 175 us,
+// 0.69 PFLOP/s of the causal products, 41 % of a plain matrix product's rate.  Tried beside it, of the same prompt when it took 183: scores read
+// twice in loops of 32 columns, a third less code, 191; two warps to a row's 64 scores and half as many for the conversions 195; keys and values two
+// tiles ahead 185.  Tiles of 128 tokens with one set of scores and one thread for all products: 699 for 8192 tokens, 668 with these.  Part of what
+// the softmax takes longer here than alone is the supply of its instructions: copies of its step in a row, alone, 771 cycles each while the code is
+// below 20 KB, 933 at 37 KB, 1100 at 68 KB and 2045 at 147 KB; the roles' loops here are some 30 KB together.
 //
 // Every wait is bounded; a warp that gives up flags it, all warps fall through to the end, where the tensor memory is freed.
 #include <algorithm>
@@ -57,10 +63,11 @@ constexpr int kWarpTokens = 16;      // of a tile's tokens that a warp turns int
 constexpr int kItemUnits = 4;        // what an item's beginning and end cost, in units
 constexpr int kStages = 4;           // of keys and of values, as halves
 constexpr int kRefs = 8;             // tiles whose scales are kept
-// Weights are held times 2^7, and at most 2^15: halves that are normal numbers down to 2^-21 of the reference, and 2^-32 of it off below: of 131072 tokens' values 2^-15 of the largest one
-// at the very worst, 1/16 of the result's rounding.
+// Weights are held times 2^7, and at most 2^15: halves that are normal numbers down to 2^-21 of the reference, and 2^-32 of it off below: of 131072
+// tokens' values 2^-15 of the largest one at the very worst, 1/16 of the result's rounding.
 constexpr float kOffset = 7.f, kSlack = 8.f;
-constexpr int kLeastLower = -60;     // of a tile's values against the largest so far: a weight times 2^-60 is 0 as a half, and their sum, which is taken of these, far from it
+// Of a tile's values against the largest so far: a weight times 2^-60 is 0 as a half, and their sum, which is taken of these, far from it
+constexpr int kLeastLower = -60;
 constexpr float kHeadroom = 32.f;    // largest factor of a code in the halves
 constexpr float kLeastFactor = 5.9604645e-8f;   // the least one, 2^-24: a half's last place
 constexpr uint32_t kTmemAll = 512;
@@ -68,7 +75,8 @@ constexpr uint32_t kTmemAll = 512;
 template <int D>
 struct Shape {
     static constexpr uint32_t kRowGroup = 16 * D;          // 8 rows of queries or keys: D / 8 core matrices of 128 bytes
-    static constexpr uint32_t kDimGroup = 16 * kTokens + 16;   // 8 dims of values, 16 core matrices; a warp's stores, 8 dims apart in pairs of lanes, would meet in the same banks without the 16
+    // 8 dims of values, 16 core matrices; a warp's stores, 8 dims apart in pairs of lanes, would meet in the same banks without the 16
+    static constexpr uint32_t kDimGroup = 16 * kTokens + 16;
     static constexpr uint32_t kQBytes = kRows / 8 * kRowGroup, kKBytes = kTokens / 8 * kRowGroup, kVBytes = D / 8 * kDimGroup;
     static constexpr uint32_t kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kKBytes, kRaw = kV + kStages * kVBytes;
     static constexpr uint32_t kRawWarp = kWarpTokens * D;   // bytes, for each of the sixteen warps that make them halves
@@ -390,9 +398,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const int token = at.start + in_row / a.group, hq = at.head * a.group + in_row % a.group, pos = at.first + in_row / a.group;
                 const bool live = row < at.rows;
                 const int oldest = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-                const bool idle = at.row0 + t * kRows + 32 * (warp & 3) >= at.rows;   // a warp without rows: it keeps the others' count (16 requests of 35 rows: 48 us, 56 with the softmax of what is not there)
-                // O is in units of vref: the largest of the values' scales that the row has seen (vseen), or the tile's where it sees only part of the tile and the rest is larger.  It comes down
-                // again behind such a tile: a window that begins there has all its other tokens in front.
+                // A warp without rows: it keeps the others' count (16 requests of 35 rows: 48 us, 56 with the softmax of what is not there)
+                const bool idle = at.row0 + t * kRows + 32 * (warp & 3) >= at.rows;
+                // O is in units of vref: the largest of the values' scales that the row has seen (vseen), or the tile's where it sees only part of
+                // the tile and the rest is larger.  It comes down again behind such a tile: a window that begins there has all its other tokens in
+                // front.
                 float m = -INFINITY, l = 0.f, vref = 0.f, vseen = 0.f;
                 for (int j = 0; j < tiles; ++j) {
                     const uint32_t ref = (count + j) & (kRefs - 1), n = done + j;
@@ -537,9 +547,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         give_registers<kMmaRegs>();
         constexpr uint32_t kIdescS = instr_desc(kTokens), kIdescO = instr_desc(D);
         if (warp < kScheduleWarp && elect_one()) {
-            // One thread for the scores, up to two tiles of the cache ahead, one for P V: a commit holds its thread up until the products in front are done, and what comes between it and
-            // the next product is beside the other thread's products then.  (One thread for all: 3.7 thousand cycles for 128 tokens with nothing else to do, of which the products take 2.1; one
-            // for each row tile, with 35 rows in one tile: 2.7 thousand cycles for 64 tokens.)
+            // One thread for the scores, up to two tiles of the cache ahead, one for P V: a commit holds its thread up until the products in front
+            // are done, and what comes between it and the next product is beside the other thread's products then.  (One thread for all: 3.7 thousand
+            // cycles for 128 tokens with nothing else to do, of which the products take 2.1; one for each row tile, with 35 rows in one tile: 2.7
+            // thousand cycles for 64 tokens.)
             const bool first = warp == kMmaWarp;
             bool go = true;
             auto until = [&](unsigned long long& b, uint32_t phase) {
@@ -550,7 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 return go;
             };
             const uint64_t q_desc = smem_desc(base + S::kQ, S::kRowGroup), k_desc = smem_desc(base + S::kK, S::kRowGroup), v_desc = smem_desc(base + S::kV, S::kDimGroup);
-            uint32_t turns = 0, items = 0, n0 = 0, n1 = 0;   // tiles of the cache; items of each row tile (a bit each, the parity); scores, or P V, of each row tile
+            // Tiles of the cache; items of each row tile (a bit each, the parity); scores, or P V, of each row tile
+            uint32_t turns = 0, items = 0, n0 = 0, n1 = 0;
             while (until(s_bar.seg_full[seg_n % kSegments], (seg_n / kSegments) & 1)) {
                 const int tiles = s_seg[seg_n % kSegments].tiles, pair = s_seg[seg_n % kSegments].two() ? 2 : 1;
                 if (tiles == 0) break;
@@ -604,13 +616,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const Segment& at = s_seg[seg_n % kSegments];
                 if (t == 1 && !at.two()) continue;
                 if (!wait(s_bar.q_empty[t], (q_n++ & 1) ^ 1)) break;
-                // Rows behind the last: zeros beside live ones of a softmax warp, what is there for warps without.  (With the last row in their place 148 CTAs asked the same place of the
-                // L2 cache for it a hundred times each, 20 us for a request of 35 rows.)
+                // Rows behind the last: zeros beside live ones of a softmax warp, what is there for warps without.  (With the last row in their place
+                // 148 CTAs asked the same place of the L2 cache for it a hundred times each, 20 us for a request of 35 rows.)
                 const int rows_here = min(kRows, at.rows - at.row0 - t * kRows), live = (rows_here + 7) / 8, groups = (rows_here + 31) / 32 * 4;
                 uint8_t* const dst = s_mem + S::kQ + t * S::kQBytes + (lane & 7) * 16 + (lane >> 3) * 128;
 #pragma unroll 1
                 for (int g = part; g < live; g += 2) {
-                    const int row = min(at.row0 + t * kRows + 8 * g + (lane & 7), at.rows - 1);   // (rows behind the last: the last again, nobody reads their results)
+                    // Rows behind the last: the last again, nobody reads their results
+                    const int row = min(at.row0 + t * kRows + 8 * g + (lane & 7), at.rows - 1);
                     const int token = row / a.group, hq = at.head * a.group + row - token * a.group;
                     const __half* const src = a.q + (at.start + token) * a.q_stride + static_cast<long>(hq) * D + 8 * (lane >> 3);
 #pragma unroll
@@ -676,8 +689,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         };
         int known_row = -1, known_first = -1, known = 0;   // 32 entries of a row of the tables, one per lane
         uint2 scales = make_uint2(0u, 0u);                 // of the fetched tile's pages, one per lane, as bits
-        // The 16 tokens' bytes on their way to this warp's part of shared memory, in an order in which eight rows' reads of a chunk meet in no bank.  (Tokens behind the request's last are
-        // read all the same, from its last page: their bytes are finite whatever was there, and no row sees them.)
+        // The 16 tokens' bytes on their way to this warp's part of shared memory, in an order in which eight rows' reads of a chunk meet in no bank.
+        // (Tokens behind the request's last are read all the same, from its last page: their bytes are finite whatever was there, and no row sees
+        // them.)
         auto fetch = [&](const Place& at) {
             const Segment& seg = s_seg[at.seg % kSegments];
             const int token = (seg.tile + at.j) * kTokens, first = token >> a.page_shift, pages = (min(kTokens, seg.held - token) + P - 1) >> a.page_shift;
@@ -796,9 +810,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     }
 }
 
-// Parts of the items that several CTAs share, in the CTAs' order: a thread takes four dims of ROWS rows, eight rows apart.  Bound by the latency of its loads (entry, parts, one behind
-// the other), so what a thread reads is on its way at once: two parts of four rows where items are full (a prompt, 148 items of two parts, 38 MB: 7 us less than a row at a
-// time), eight parts of a row where they are not (few rows over a long cache, cut into many).
+// Parts of the items that several CTAs share, in the CTAs' order: a thread takes four dims of ROWS rows, eight rows apart.  Bound by the latency of
+// its loads (entry, parts, one behind the other), so what a thread reads is on its way at once: two parts of four rows where items are full (a
+// prompt, 148 items of two parts, 38 MB: 7 us less than a row at a time), eight parts of a row where they are not (few rows over a long cache, cut
+// into many).
 constexpr int kJoinRows = 8;
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kJoinRows * D / 4) paged_prompt_join_kernel(const __grid_constant__ PagedAttnArgs a) {
