@@ -382,6 +382,33 @@ int tq_rope_f16(void* x_fp16, const int* positions, long rows, int heads, int he
 int tq_rope_qk_f16(void* q_fp16, void* k_fp16, const int* positions, long rows, int q_heads, int kv_heads, int head_dim, float theta,
                    void* stream);
 int tq_swiglu_f16(const void* gate_up_fp16, void* act_fp16, long rows, int intermediate, void* stream);
+/** The norm of each query and key head and its rotation in one pass, fp16: y = x * rsqrt(mean(x^2) + eps) * weight over a head's head_dim
+ *  elements, then y_i and y_{i + head_dim/2} turned by positions[row] * theta^(-2i/head_dim).  fp32 arithmetic with one rounding at the end;
+ *  angles as fractions of a turn in 64 bits, right at any position.  Row r's heads are contiguous, at r * stride elements (heads * head_dim or
+ *  more: a slice of a fused projection's result); results may go to where the rows are.  head_dim a multiple of 16, up to 512; weights [head_dim].
+ *  All pointers are device pointers of one device, whichever is current.  Fastest where pointers and strides are multiples of 16 bytes. */
+int tq_qk_norm_rope_f16(const void* q_fp16, const void* k_fp16, const void* q_weight_fp16, const void* k_weight_fp16, const int* positions, long rows,
+                        int q_heads, int kv_heads, int head_dim, long q_stride, long k_stride, float eps, float theta, void* q_out_fp16, void* k_out_fp16,
+                        long q_out_stride, long k_out_stride, void* stream);
+
+/** Which drafted tokens stay, and what follows them: speculative sampling on a tree of drafts for each of n requests.  Request i's nodes are the rows
+ *  starts[i] .. starts[i + 1] - 1 (of `rows`; as tq_paged_plan gives them); parents [rows] is a node's parent, counted from its request's first
+ *  node, which is in front of it.  Node 0 is no draft: the token that the last step ended with.  tokens [rows]; target [rows, vocab], what
+ *  the target gives to each token behind a node; draft [rows, vocab], what its children were drawn from, one after another with replacement, or
+ *  NULL: children that were chosen.  Both TQ_F32 or TQ_F16, probabilities that add up to one, strides in elements from row to row; what is no
+ *  positive number counts as 0.  uniforms [rows]: random numbers of [0, 1), each used once.
+ *
+ *  From node 0 on the children of the present node come in order; with p the target's row of the node, q the draft's, w = p and Z = 1, child c of
+ *  token x becomes the present node where uniforms[c] * Z * q(x) < w(x); otherwise w becomes max(w - Z q, 0) and Z its sum.  Without a draft: where
+ *  uniforms[c] * Z < w(x); otherwise Z becomes Z - w(x), w(x) 0.  Where none is accepted (or the path is full) the next token is the first
+ *  up to which the sum of w exceeds uniforms[0] times its whole sum; w is p again where nothing is left of it.  Sums and comparisons are in 64 bits.
+ *
+ *  path [n, width]: the nodes that stay, node 0 the first, -1 behind them; kept [n]: how many they are; next [n].  A request without nodes, or whose
+ *  rows are not inside the `rows`, keeps none and has next -1, as has one without a token that could be.  A node without a parent in front of it, or
+ *  with a token outside the vocabulary, is nobody's child.  Of a request's nodes the first 1024 are looked at; vocab up to 2^20, n up to 65536.
+ *  All pointers are device pointers of one device, whichever is current.  Fastest where pointers and strides are multiples of 16 bytes. */
+int tq_verify_drafts(const int* starts, const int* parents, const int* tokens, int n, int rows, const void* target, const void* draft, int dtype, int vocab,
+                     long target_stride, long draft_stride, const float* uniforms, int* path, int width, int* kept, int* next, void* stream);
 
 /** Waits for the device; non-zero if a wait of this exchange gave up. */
 int tq_exchange_status(tq_exchange_t ex);
@@ -575,6 +602,17 @@ int tq_paged_plan(tq_paged_cache_t cache, const int* rows, const int* counts, in
 /** The request in row rows[i] keeps its first lengths[i] tokens (0: it is gone); its other pages become free, to be taken in the same order
  *  again.  All or nothing, as above.  Ends the plan in force. */
 int tq_paged_truncate(tq_paged_cache_t cache, const int* rows, const int* lengths, int n, void* stream);
+/** The planned tokens as trees of drafts: parents [tokens] (device memory) is each token's parent, counted from its request's first new token and in
+ *  front of it, or -1: none; NULL: the token in front.  positions [tokens] (may be NULL): what the request held before and the token's depth, 0
+ *  behind the last.  A request whose new tokens are a chain may have any number of them, another one 256.  A request whose parents are no tree has
+ *  no attention (tq_paged_status tells); its positions are 0.  In force until the plan ends. */
+int tq_paged_tree(tq_paged_cache_t cache, const int* parents, int tokens, int* positions, void* stream);
+/** Of request i's new tokens the kept[i] ones path[i, 0 .. ] stay, ascending (as tq_verify_drafts gives them), all of them where kept[i] is below
+ *  0.  In all layers they move up to the places of the first new ones, and the pages behind become free.  A token that stays in its page keeps
+ *  its numbers; one that joins another page joins it as an append of its values would, and where the page's scale grows all that the page holds is
+ *  rounded once more.  path [n, width], kept [n] and lengths [n] (may be NULL; the tokens that each request holds then) are device memory, n is
+ *  the plan's.  A path that is none changes nothing (tq_paged_status tells).  Ends the plan in force. */
+int tq_paged_keep(tq_paged_cache_t cache, const int* path, int width, const int* kept, int n, int* lengths, void* stream);
 /** Keys and values [tokens, heads, head_dim] of the planned tokens (TQ_F32 or TQ_F16), token t at t * stride elements (heads * head_dim
  *  or more: a slice of a fused projection's result), into a layer.  `tokens` is the plan's; rows behind the last request's are not read.
  *  Fastest where pointers and strides are multiples of 16 bytes. */

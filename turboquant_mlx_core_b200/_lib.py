@@ -98,6 +98,8 @@ def load() -> C.CDLL:
     sig("tq_rope_f16", i, [vp, vp, C.c_long, i, i, C.c_float, vp])
     sig("tq_rope_qk_f16", i, [vp, vp, vp, C.c_long, i, i, i, C.c_float, vp])
     sig("tq_exchange_sum_f16_rmsnorm", i, [vp, i, C.c_long, C.c_long, i, vp, vp, vp, vp, C.c_float, vp])
+    sig("tq_qk_norm_rope_f16", i, [vp, vp, vp, vp, vp, C.c_long, i, i, i, C.c_long, C.c_long, C.c_float, C.c_float, vp, vp, C.c_long, C.c_long, vp])
+    sig("tq_verify_drafts", i, [vp, vp, vp, i, i, vp, vp, i, i, C.c_long, C.c_long, vp, vp, i, vp, vp, vp])
     sig("tq_swiglu_f16", i, [vp, vp, C.c_long, i, vp])
     sig("tq_exchange_merge_attention", i, [vp, vp, i, C.c_long, i, C.c_long, C.c_long, vp, vp])
     sig("tq_linear_forward_allgather", i, [vp, vp, vp, i, C.POINTER(C.c_void_p), i, C.c_long, C.c_long, C.POINTER(C.c_void_p), i,
@@ -166,6 +168,8 @@ def load() -> C.CDLL:
     sig("tq_paged_cache_free", None, [vp])
     sig("tq_paged_plan", i, [vp, vp, vp, i, i, i, vp, vp, vp, vp, vp, i, vp])
     sig("tq_paged_truncate", i, [vp, vp, vp, i, vp])
+    sig("tq_paged_tree", i, [vp, vp, i, vp, vp])
+    sig("tq_paged_keep", i, [vp, vp, i, vp, i, vp, vp])
     sig("tq_paged_append", i, [vp, i, vp, vp, i, i, C.c_long, C.c_long, vp])
     sig("tq_paged_read", i, [vp, i, vp, i, vp, vp, i, vp])
     sig("tq_paged_attention", i, [vp, i, vp, i, i, C.c_long, i, C.c_float, vp, C.c_long, vp, vp])

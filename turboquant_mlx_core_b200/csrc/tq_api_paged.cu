@@ -45,9 +45,11 @@ public:
         }
         // the arrays of a plan, 256-byte aligned in one block
         const size_t sizes[] = {sizeof(tq::PagedHeader), 4ul * max_requests, 4ul * max_requests * max_pages, 4ul * pages, 4ul * max_requests,
-                                4ul * max_requests + 4, 4ul * max_requests, sizeof(tq::PagedPiece) * b_.max_pieces, 8ul * max_requests};
-        size_t at[9], all = 0;
-        for (int i = 0; i < 9; ++i) {
+                                4ul * max_requests + 4, 4ul * max_requests, sizeof(tq::PagedPiece) * b_.max_pieces, 8ul * max_requests,
+                                sizeof(tq::PagedNode) * max_tokens, sizeof(uint8_t*) * layers};
+        constexpr int kArrays = sizeof(sizes) / sizeof(sizes[0]);
+        size_t at[kArrays], all = 0;
+        for (int i = 0; i < kArrays; ++i) {
             at[i] = all;
             all += (sizes[i] + 255) / 256 * 256;
         }
@@ -63,7 +65,12 @@ public:
         b_.held = reinterpret_cast<int*>(p + at[6]);
         b_.pieces = reinterpret_cast<tq::PagedPiece*>(p + at[7]);
         staged_ = reinterpret_cast<int*>(p + at[8]);
+        b_.nodes = reinterpret_cast<tq::PagedNode*>(p + at[9]);
+        b_.layers = reinterpret_cast<uint8_t* const*>(p + at[10]);
         TQ_CUDA(cudaMemset(p, 0, all));
+        std::vector<uint8_t*> bases;
+        for (const DeviceBuffer& l : layers_) bases.push_back(l.as<uint8_t>());
+        TQ_CUDA(cudaMemcpy(p + at[10], bases.data(), sizeof(uint8_t*) * bases.size(), cudaMemcpyHostToDevice));
         std::vector<int> stack(static_cast<size_t>(pages));
         for (int i = 0; i < pages; ++i) stack[static_cast<size_t>(i)] = pages - 1 - i;   // page 0 is the first to go
         TQ_CUDA(cudaMemcpy(b_.stack, stack.data(), 4ul * pages, cudaMemcpyHostToDevice));
@@ -105,6 +112,27 @@ public:
                             tables_width, d_status_, sms_};
         tq::launch_paged_plan(a, st);
         plan_ = {n, tokens, std::min(max_count, tokens)};
+        tree_ = false;
+    }
+    void tree(const int* parents, int tokens, int* positions, cudaStream_t st) {
+        TQ_REQUIRE(plan_.n >= 0, "paged tree: no plan in force");
+        TQ_REQUIRE(tokens == plan_.tokens, "paged tree: the plan is for " + std::to_string(plan_.tokens) + " tokens");
+        TQ_REQUIRE(!parents || tokens == 0 || tq::is_device_pointer(parents), "paged tree: parents must be a device pointer");
+        TQ_REQUIRE(!positions || tokens == 0 || tq::is_device_pointer(positions), "paged tree: positions must be a device pointer");
+        begin(st);
+        tq::launch_paged_tree({b_, parents, positions, plan_, d_status_}, st);
+        tree_ = true;
+    }
+    void keep(const int* path, int width, const int* kept, int n, int* lengths, cudaStream_t st) {
+        TQ_REQUIRE(plan_.n >= 0, "paged keep: no plan in force");
+        TQ_REQUIRE(n == plan_.n, "paged keep: the plan is for " + std::to_string(plan_.n) + " requests");
+        TQ_REQUIRE(width > 0, "paged keep: a path has room for one token at least");
+        if (n == 0) return;
+        TQ_REQUIRE(tq::is_device_pointer(path) && tq::is_device_pointer(kept) && (!lengths || tq::is_device_pointer(lengths)),
+                   "paged keep: paths, their lengths and results must be device pointers");
+        begin(st);
+        tq::launch_paged_keep({b_, path, kept, lengths, n, width, heads_, static_cast<int>(layers_.size()), plan_, d_status_, sms_}, dim_, st);
+        plan_.n = -1;
     }
     void truncate(const int* rows, const int* lengths, int n, cudaStream_t st) {
         TQ_REQUIRE(n >= 0 && n <= b_.max_requests, "paged truncate: more requests than the cache was made for");
@@ -192,13 +220,15 @@ public:
         const unsigned int code = *static_cast<volatile unsigned int*>(h_status_);
         if (code == tq::kPagedOk) return;
         *static_cast<volatile unsigned int*>(h_status_) = tq::kPagedOk;
-        static const char* const what[] = {"", "a row outside the tables, or twice in a batch",
+        static const std::string what[] = {"", "a row outside the tables, or twice in a batch",
                                            "a negative count, one above max_count, or more tokens in all than announced",
                                            "a request would be longer than max_pages_per_request pages", "not enough free pages",
                                            "truncation to a length that the request does not have", "a page number outside the cache",
                                            "a wait on the device ran out",
-                                           "the plan on the device is not the one that a call was made for"};
-        throw tq::Error(std::string("paged cache: ") + what[code < 9 ? code : 0]);
+                                           "the plan on the device is not the one that a call was made for",
+                                           "parents that make no tree, or a tree of more than " + std::to_string(tq::kPagedTreeNodes) + " nodes",
+                                           "a path that is not an ascending list of a request's new tokens"};
+        throw tq::Error("paged cache: " + what[code < 11 ? code : 0]);
     }
     int free_pages() {
         tq::ensure_device(device_);
@@ -226,6 +256,7 @@ private:
 
     int heads_, dim_, max_tokens_, device_ = 0, sms_ = 0;
     tq::PagedSizes plan_{-1, 0, 0};   // of the plan in force (n < 0: none)
+    bool tree_ = false;               // its tokens are trees
     size_t prompt_scratch_ = 0;
     tq::StreamUse use_;
     std::vector<DeviceBuffer> layers_;
@@ -274,6 +305,18 @@ int tq_paged_plan(tq_paged_cache_t cache, const int* rows, const int* counts, in
 int tq_paged_truncate(tq_paged_cache_t cache, const int* rows, const int* lengths, int n, void* stream) {
     return guarded<int>(0, -1, [&]() {
         paged(cache)->truncate(rows, lengths, n, cuda_stream(stream));
+        return 0;
+    });
+}
+int tq_paged_tree(tq_paged_cache_t cache, const int* parents, int tokens, int* positions, void* stream) {
+    return guarded<int>(0, -1, [&]() {
+        paged(cache)->tree(parents, tokens, positions, cuda_stream(stream));
+        return 0;
+    });
+}
+int tq_paged_keep(tq_paged_cache_t cache, const int* path, int width, const int* kept, int n, int* lengths, void* stream) {
+    return guarded<int>(0, -1, [&]() {
+        paged(cache)->keep(path, width, kept, n, lengths, cuda_stream(stream));
         return 0;
     });
 }

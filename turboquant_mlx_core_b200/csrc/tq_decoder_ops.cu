@@ -4,6 +4,7 @@
 // so that a whole tensor-parallel decode step can be timed.  fp16 in and out, fp32 arithmetic;
 // every kernel is memory-bound (a few bytes per element) and carries the programmatic-launch wait
 // so that it can follow the kernels of this library without a launch gap.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -85,6 +86,131 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(__half* __restr
         }
         *reinterpret_cast<uint4*>(v) = pack_halves(lo);
         *reinterpret_cast<uint4*>(v + half) = pack_halves(hi);
+    }
+}
+
+// The norm of each query and key head and its rotation in one pass:
+//
+//   y = x rsqrt(mean(x^2) + eps) w,  (y_i, y_{i + D/2}) turned by position * theta^(-2 i / D)
+//
+// fp32 from the sum of squares to the rotation, one rounding at the end.  The angle is a fraction of a turn: position times the frequency in units
+// of 2^-64 turns, of which a 64-bit product keeps the fraction, 2^-34 off at most whatever the position (in fp32 it is a hundredth off at
+// position 131072).
+//
+// A thread takes eight pairs of a head, 16 bytes from either half, so that the rotation stays in its registers; `lanes` threads, the next power
+// of two above D / 16, share a head and its sum of squares.  It is bound by memory (few rows: by latency): 16 bytes in and out for eight
+// elements, asked for in front of the sines and cosines, which D / 2 threads take for all heads of a row.
+constexpr int kHeadHalfMax = 256;
+struct QkNormArgs {
+    const __half* x[2];       // queries, keys
+    const __half* w[2];
+    __half* y[2];
+    long x_stride[2], y_stride[2];   // elements from row to row
+    const int* positions;
+    long rows;
+    int heads[2], dim, lanes, rows_per_cta;
+    float eps;
+    unsigned long long turns[kHeadHalfMax];   // frequencies in 2^-64 turns
+};
+template <bool WIDE>
+__device__ __forceinline__ uint4 load_head(const __half* p) {
+    if constexpr (WIDE) {
+        return *reinterpret_cast<const uint4*>(p);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __half_as_ushort(p[2 * k]) | static_cast<uint32_t>(__half_as_ushort(p[2 * k + 1])) << 16;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_head(__half* p, const uint4& v) {
+    if constexpr (WIDE) {
+        *reinterpret_cast<uint4*>(p) = v;
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            p[2 * k] = __ushort_as_half(static_cast<unsigned short>(w[k]));
+            p[2 * k + 1] = __ushort_as_half(static_cast<unsigned short>(w[k] >> 16));
+        }
+    }
+}
+template <bool WIDE>
+__global__ void __launch_bounds__(512) qk_norm_rope_kernel(const __grid_constant__ QkNormArgs a) {
+    ops_dependency_sync();
+    extern __shared__ float2 s_turn[];   // [rows_per_cta][dim / 2] cosine, sine
+    const int half = a.dim >> 1, per_row = (a.heads[0] + a.heads[1]) * a.lanes;
+    const long row0 = static_cast<long>(blockIdx.x) * a.rows_per_cta;
+    const int rows = static_cast<int>(min(static_cast<long>(a.rows_per_cta), a.rows - row0)), items = rows * per_row;
+    struct Item {
+        const __half* x;
+        __half* y;
+        int which, row, at;   // queries or keys; row of the CTA's; its first pair
+        bool live;
+    };
+    auto item = [&](int i) {
+        Item it;
+        it.row = min(i / per_row, rows - 1);
+        const int in = i - it.row * per_row, h = in / a.lanes, t = in - h * a.lanes;
+        it.which = h >= a.heads[0] ? 1 : 0;
+        it.at = 8 * t;
+        it.live = i < items && it.at < half;
+        const long row = row0 + it.row, off = static_cast<long>(it.which ? h - a.heads[0] : h) * a.dim + it.at;
+        it.x = a.x[it.which] + row * a.x_stride[it.which] + off;
+        it.y = a.y[it.which] + row * a.y_stride[it.which] + off;
+        return it;
+    };
+    auto load = [&](const Item& it, uint4& lo, uint4& hi) {
+        lo = hi = make_uint4(0u, 0u, 0u, 0u);
+        if (it.live) {
+            lo = load_head<WIDE>(it.x);
+            hi = load_head<WIDE>(it.x + half);
+        }
+    };
+    Item it = item(threadIdx.x);
+    uint4 lo, hi;
+    load(it, lo, hi);
+    for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
+        const int r = i / half, p = i - r * half;
+        const unsigned long long turn = static_cast<unsigned long long>(static_cast<long long>(a.positions[row0 + r])) * a.turns[p];
+        const float t = static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f;   // half turns, -1 .. 1
+        float s, c;
+        sincospif(t, &s, &c);
+        s_turn[i] = make_float2(c, s);
+    }
+    __syncthreads();
+    // (all lanes of a warp go round as often: the sums' shuffles)
+    for (int i = threadIdx.x; i - static_cast<int>(threadIdx.x & 31) < items;) {
+        float u[8], v[8];
+        unpack_halves(lo, u);
+        unpack_halves(hi, v);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(u[j], u[j], fmaf(v[j], v[j], sum));
+        for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const Item now = it;
+        i += blockDim.x;
+        if (i - static_cast<int>(threadIdx.x & 31) < items) {
+            it = item(i);
+            load(it, lo, hi);
+        }
+        if (!now.live) continue;
+        const float scale = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+        float g[8], k[8];
+        const __half* const w = a.w[now.which] + now.at;
+        unpack_halves(load_head<WIDE>(w), g);
+        unpack_halves(load_head<WIDE>(w + half), k);
+        const float2* const turn = s_turn + now.row * half + now.at;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 cs = turn[j];
+            const float p = u[j] * scale * g[j], q = v[j] * scale * k[j];
+            u[j] = p * cs.x - q * cs.y;
+            v[j] = q * cs.x + p * cs.y;
+        }
+        store_head<WIDE>(now.y, pack_halves(u));
+        store_head<WIDE>(now.y + half, pack_halves(v));
     }
 }
 
@@ -181,6 +307,43 @@ void launch_rope_qk_f16(__half* q, __half* k, const int* positions, long rows, i
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = ops_config(static_cast<unsigned>(blocks), 128, stream, attr);
     TQ_CUDA(cudaLaunchKernelEx(&cfg, rope_kernel, q, positions, q_heads, dim, std::log2(theta), pairs_q, k, kv_heads, pairs_k));
+}
+
+void launch_qk_norm_rope_f16(const __half* q, const __half* k, const __half* q_weight, const __half* k_weight, const int* positions, long rows, int q_heads,
+                             int kv_heads, int dim, long q_stride, long k_stride, float eps, float theta, __half* q_out, __half* k_out, long q_out_stride,
+                             long k_out_stride, cudaStream_t stream) {
+    QkNormArgs a{};
+    a.x[0] = q;
+    a.x[1] = k;
+    a.w[0] = q_weight;
+    a.w[1] = k_weight;
+    a.y[0] = q_out;
+    a.y[1] = k_out;
+    a.x_stride[0] = q_stride;
+    a.x_stride[1] = k_stride;
+    a.y_stride[0] = q_out_stride;
+    a.y_stride[1] = k_out_stride;
+    a.positions = positions;
+    a.rows = rows;
+    a.heads[0] = q_heads;
+    a.heads[1] = kv_heads;
+    a.dim = dim;
+    a.eps = eps;
+    a.lanes = 1;
+    while (a.lanes * 16 < dim) a.lanes *= 2;
+    constexpr double kTwoPi = 6.283185307179586476925286766559;
+    for (int i = 0; i < dim / 2; ++i) a.turns[i] = static_cast<unsigned long long>(std::llrint(std::pow(static_cast<double>(theta), -2.0 * i / dim) / kTwoPi * 18446744073709551616.0));
+    uintptr_t all = 0;
+    for (int i = 0; i < 2; ++i)
+        all |= reinterpret_cast<uintptr_t>(a.x[i]) | reinterpret_cast<uintptr_t>(a.w[i]) | reinterpret_cast<uintptr_t>(a.y[i]) | static_cast<uintptr_t>(2 * (a.x_stride[i] | a.y_stride[i]));
+    // Threads of a row, and rows to a CTA of some 256 threads where a row has fewer.
+    const int per_row = (q_heads + kv_heads) * a.lanes, turns = (per_row + 511) / 512;
+    a.rows_per_cta = static_cast<int>(std::min<long>(std::max(1, 256 / per_row), rows));
+    const int threads = std::min(512, (a.rows_per_cta * ((per_row + turns - 1) / turns) + 31) / 32 * 32);
+    const dim3 grid(static_cast<unsigned>((rows + a.rows_per_cta - 1) / a.rows_per_cta)), block(static_cast<unsigned>(threads));
+    const size_t smem = static_cast<size_t>(a.rows_per_cta) * (dim / 2) * sizeof(float2);
+    if (all % 16 == 0) launch_pdl(qk_norm_rope_kernel<true>, grid, block, smem, stream, a);
+    else launch_pdl(qk_norm_rope_kernel<false>, grid, block, smem, stream, a);
 }
 
 void launch_swiglu_f16(const __half* gate_up, __half* act, long rows, int inter, cudaStream_t stream) {

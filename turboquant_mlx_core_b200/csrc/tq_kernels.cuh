@@ -207,6 +207,9 @@ void launch_rope_f16(__half* x, const int* positions, long rows, int heads, int 
 // queries [rows, q_heads, dim] and keys [rows, kv_heads, dim] in one launch
 void launch_rope_qk_f16(__half* q, __half* k, const int* positions, long rows, int q_heads, int kv_heads, int dim, float theta,
                         cudaStream_t stream);
+void launch_qk_norm_rope_f16(const __half* q, const __half* k, const __half* q_weight, const __half* k_weight, const int* positions, long rows, int q_heads,
+                             int kv_heads, int dim, long q_stride, long k_stride, float eps, float theta, __half* q_out, __half* k_out, long q_out_stride,
+                             long k_out_stride, cudaStream_t stream);
 void launch_swiglu_f16(const __half* gate_up, __half* act, long rows, int inter, cudaStream_t stream);
 
 // tq_misc.cu — small element-wise helpers.

@@ -50,7 +50,14 @@ struct __align__(16) PagedHeader {
     int free_pages;      // pages on the stack
     int requests, tokens, pieces;   // of the plan (all 0 where it was refused)
     PagedSizes sizes;    // n below 0: a truncation came behind it
-    int unused;
+    int state;           // PagedState
+};
+enum PagedState { kPagedPlain = 0, kPagedTree = 1 /* the plan's tokens are trees */, kPagedKept = 2 /* a branch of each is to be kept */ };
+// A new token as a node of its request's tree.  Nodes are numbered as a walk meets them that goes down from each node, one child after another, before
+// it goes on: those below a node, and itself, are pre .. last, so that i is an ancestor of j, or j, where pre_i <= pre_j <= last_i.
+struct __align__(16) PagedNode {
+    int pre, last, depth;
+    int good;            // of a request whose parents make a tree
 };
 // A run of new tokens in one page.
 struct PagedPiece {
@@ -66,6 +73,8 @@ struct PagedBatch {
     int* starts;           // (+ 1)
     int* held;
     PagedPiece* pieces;
+    PagedNode* nodes;      // [max_tokens]
+    uint8_t* const* layers;   // [num_layers]
     int max_requests, max_pages, num_pages, page_tokens, max_pieces;
 };
 
@@ -79,7 +88,9 @@ enum PagedStatus : unsigned int {
     kPagedBadLength = 5,   // truncation to a length that the request does not have
     kPagedBadPage = 6,     // a page number outside the cache
     kPagedWait = 7,        // a bounded wait ran out
-    kPagedOtherPlan = 8    // the plan on the device is not the one that a launch was made for
+    kPagedOtherPlan = 8,   // the plan on the device is not the one that a launch was made for
+    kPagedBadTree = 9,     // parents that make no tree
+    kPagedBadPath = 10     // a path that is not an ascending list of new tokens
 };
 
 // Lets a kernel have so much dynamic shared memory, once for each device (`set`: those that have been).
@@ -125,6 +136,29 @@ struct PagedAppendArgs {
     unsigned int* status;
 };
 void launch_paged_append(const PagedAppendArgs& a, int dim, bool half, cudaStream_t st);
+
+// The parents of the plan's tokens (or null: each token's is the one in front).  A tree that is not a chain has kPagedTreeNodes nodes at most.
+constexpr int kPagedTreeNodes = 256;
+struct PagedTreeArgs {
+    PagedBatch b;
+    const int* parents;
+    int* positions;       // or null
+    PagedSizes sizes;
+    unsigned int* status;
+};
+void launch_paged_tree(const PagedTreeArgs& a, cudaStream_t st);
+// path [n][width]: of each request the new tokens that stay, kept[i] of them (all where that is below 0).
+struct PagedKeepArgs {
+    PagedBatch b;
+    const int* path;
+    const int* kept;
+    int* lengths;         // or null
+    int n, width, heads, layers;
+    PagedSizes sizes;
+    unsigned int* status;
+    int sms;
+};
+void launch_paged_keep(const PagedKeepArgs& a, int dim, cudaStream_t st);
 
 struct PagedReadArgs {
     const uint8_t* layer;

@@ -286,9 +286,156 @@ __global__ void __launch_bounds__(kPlanThreads) paged_truncate_kernel(PagedPlanA
     }
 }
 
+// The parents of a plan's tokens to numbers, depths and positions: a CTA for each request.  A chain, of any length, is told by its parents alone.  In
+// another tree each node walks up, counts itself at its ancestors and learns its depth; what its elder siblings hold comes from a look at all
+// nodes in front, and its number from a second walk.  It is bound by the walks' and the looks' reads of shared memory (a thread for each of 256 nodes at most).
+constexpr int kTreeThreads = 256;
+__global__ void __launch_bounds__(kTreeThreads) paged_tree_kernel(PagedTreeArgs a) {
+    pdl_wait_release();
+    behind_wait(a.parents, a.b.starts, a.b.held, a.b.header);
+    static_assert(kTreeThreads >= kPagedTreeNodes);
+    __shared__ int s_parent[kPagedTreeNodes], s_size[kPagedTreeNodes], s_off[kPagedTreeNodes];
+    const int tid = threadIdx.x, requests = paged_device::planned(a.b.header, a.sizes, a.status).requests;
+    if (blockIdx.x == 0) {
+        if (tid == 0 && requests > 0) a.b.header->state = kPagedTree;
+        if (a.positions && requests == 0)
+            for (int t = tid; t < a.sizes.tokens; t += kTreeThreads) a.positions[t] = 0;
+    }
+    for (int i = blockIdx.x; i < requests; i += gridDim.x) {
+        const int start = a.b.starts[i], count = a.b.starts[i + 1] - start, first = a.b.held[i] - count;
+        if (a.positions && i == requests - 1)
+            for (int t = start + count + tid; t < a.sizes.tokens; t += kTreeThreads) a.positions[t] = 0;
+        bool chain = true, tree = count <= kPagedTreeNodes;
+        for (int j = tid; j < count; j += kTreeThreads) {
+            const int p = a.parents ? a.parents[start + j] : j - 1;
+            chain = chain && p == j - 1;
+            tree = tree && p >= -1 && p < j;
+            if (count <= kPagedTreeNodes) {
+                s_parent[j] = p;
+                s_size[j] = 1;
+            }
+        }
+        chain = __syncthreads_and(chain);
+        tree = __syncthreads_and(tree);
+        PagedNode* const nodes = a.b.nodes + start;
+        if (chain || !tree) {
+            if (!chain && tid == 0) raise_status(a.status, kPagedBadTree);
+            for (int j = tid; j < count; j += kTreeThreads) {
+                nodes[j] = {j, count - 1, j, chain ? 1 : 0};
+                if (a.positions) a.positions[start + j] = chain ? first + j : 0;
+            }
+            continue;   // (nothing of it is in shared memory that the next one would meet)
+        }
+        const int j = tid;
+        int depth = 0;
+        if (j < count)
+            for (int p = s_parent[j]; p >= 0; p = s_parent[p]) {
+                atomicAdd(&s_size[p], 1);
+                ++depth;
+            }
+        __syncthreads();
+        if (j < count) {
+            int off = s_parent[j] >= 0 ? 1 : 0;
+            for (int k = 0; k < j; ++k)
+                if (s_parent[k] == s_parent[j]) off += s_size[k];
+            s_off[j] = off;
+        }
+        __syncthreads();
+        if (j < count) {
+            int pre = 0;
+            for (int p = j; p >= 0; p = s_parent[p]) pre += s_off[p];
+            nodes[j] = {pre, pre + s_size[j] - 1, depth, 1};
+            if (a.positions) a.positions[start + j] = first + depth;
+        }
+        __syncthreads();
+    }
+}
+
+// The bookkeeping of a kept branch: request i's length is what it held in front of the plan and kept[i] (all of the new ones where that is below 0), and
+// its pages behind that become free, as a truncation has it; the plan ends.  Every path is looked at before anything changes.  The tables' rows stay as
+// they are for the kernel behind, which moves tokens.
+__global__ void __launch_bounds__(kPlanThreads) paged_keep_plan_kernel(PagedKeepArgs a) {
+    pdl_wait_release();
+    behind_wait(a.path, a.kept, a.b.header);
+    extern __shared__ int s_plan[];
+    __shared__ unsigned int s_error;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+    const int n = a.n, P = a.b.page_tokens, tid = threadIdx.x;
+    int* const s_keep = s_plan;           // [n] tokens that stay
+    int* const s_page = s_keep + n;       // [n + 1] freed pages in front of the request's
+    if (tid == 0) s_error = kPagedOk;
+    const PagedHeader header = *const_cast<const PagedHeader*>(a.b.header);
+    const bool other = header.sizes.n != a.sizes.n || header.sizes.tokens != a.sizes.tokens || header.sizes.most != a.sizes.most;
+    // (a plan that was refused has no requests, and its lengths are as they were)
+    const bool refused = header.requests == 0;
+    __syncthreads();
+    const int per = (n + kPlanThreads - 1) / kPlanThreads, i0 = tid * per;
+    int held[kPlanPerThread], keep[kPlanPerThread];
+    long long sums[3] = {0, 0, 0}, all[3];
+#pragma unroll
+    for (int k = 0; k < kPlanPerThread; ++k) {
+        held[k] = keep[k] = 0;
+        if (k >= per || i0 + k >= n || other) continue;
+        const int i = i0 + k;
+        held[k] = a.b.held[i];
+        const int count = refused ? 0 : a.b.starts[i + 1] - a.b.starts[i];
+        int kept = a.kept[i];
+        if (refused) kept = 0;
+        else if (kept > count || kept > a.width) {
+            atomicMax(&s_error, static_cast<unsigned int>(kPagedBadPath));
+            kept = 0;
+        } else if (kept < 0) kept = count;
+        keep[k] = held[k] - count + kept;
+        sums[0] += (held[k] + P - 1) / P - (keep[k] + P - 1) / P;
+    }
+    if (!other && !refused) {
+        for (long t = tid; t < static_cast<long>(n) * a.width; t += kPlanThreads) {
+            const int i = static_cast<int>(t / a.width), k = static_cast<int>(t - static_cast<long>(i) * a.width), kept = a.kept[i];
+            if (k >= kept) continue;
+            const int token = a.path[t], count = a.b.starts[i + 1] - a.b.starts[i];
+            if (token < 0 || token >= count || (k > 0 && a.path[t - 1] >= token)) atomicMax(&s_error, static_cast<unsigned int>(kPagedBadPath));
+        }
+    }
+    block_sums(sums, all);   // (its barriers publish s_error)
+    const bool ok = s_error == kPagedOk && !other && !refused;
+    const int pages = ok ? static_cast<int>(all[0]) : 0, free_before = header.free_pages;
+    int page = static_cast<int>(sums[0]);
+#pragma unroll
+    for (int k = 0; k < kPlanPerThread; ++k) {
+        const int i = i0 + k;
+        if (k >= per || i >= n) continue;
+        s_keep[i] = ok || other ? keep[k] : held[k];
+        s_page[i] = ok ? page : 0;
+        page += (held[k] + P - 1) / P - (keep[k] + P - 1) / P;
+    }
+    if (tid == 0) s_page[n] = pages;
+    cluster.sync();   // every CTA has read the header
+    const int t0 = rank * kPlanThreads + tid, step = ctas * kPlanThreads;
+    if (!other) {
+        for (int t = t0; t < n; t += step) {
+            if (ok) a.b.lengths[a.b.rows[t]] = s_keep[t];
+            if (a.lengths) a.lengths[t] = s_keep[t];
+        }
+    }
+    if (ok) {
+        for (int t = t0; t < pages; t += step) {
+            const int i = owner_of(s_page, n, t), idx = (s_keep[i] + P - 1) / P + t - s_page[i];
+            a.b.stack[free_before + pages - 1 - t] = a.b.tables[static_cast<size_t>(a.b.rows[i]) * a.b.max_pages + idx];
+        }
+    }
+    if (t0 == 0) {
+        if (other) raise_status(a.status, kPagedOtherPlan);
+        else {
+            *a.b.header = {free_before + pages, 0, 0, 0, {-1, 0, 0}, ok ? kPagedKept : kPagedPlain};
+            if (s_error != kPagedOk) raise_status(a.status, s_error);
+        }
+    }
+}
+
 // `ctas` CTAs, a cluster where there are 2 .. 8 of them and they are to be one.
-template <typename Kernel>
-void launch_cluster(Kernel kernel, int ctas, bool cluster, size_t smem, const PagedPlanArgs& a, cudaStream_t st, std::atomic<unsigned long long>& set) {
+template <typename Kernel, typename Args>
+void launch_cluster(Kernel kernel, int ctas, bool cluster, size_t smem, const Args& a, cudaStream_t st, std::atomic<unsigned long long>& set) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -456,6 +603,122 @@ __global__ void __launch_bounds__(WARP ? 128 : 256) paged_append_kernel(PagedApp
     }
 }
 
+// ---- kept branches ------------------------------------------------------------------------------------
+
+// v * 2^k as a whole number of -127 .. 127 that it is near to (ties to even); the caller knows that it is one.
+__device__ __forceinline__ uint4 rescaled16(const uint4& codes, float ratio) {
+    float v[16];
+    decode16(v, codes, 1.f);
+    return encode16(v, ratio);
+}
+// from / to, powers of two: where it is above 2^30 the codes are zeros.
+__device__ __forceinline__ float scale_ratio(unsigned int from, unsigned int to) {
+    const int e = static_cast<int>(from >> 23) - static_cast<int>(to >> 23);
+    return e < -120 ? 0.f : __uint_as_float(static_cast<unsigned int>(min(e, 30) + 127) << 23);
+}
+
+// The tokens of a path move to the places of the first new ones: a warp for each (layer, request, KV head), keys or values.  Places are below, or
+// at, what moves there and both ascend, so that a batch of tokens may be written when it has been read.  Within a page the codes move as they are.
+// A token from another page joins as its value, and the page's scale grows where it must; all that the page holds is rounded again then.  The pages
+// are done in ascending order: what one takes from those behind it is read before they change.  It is bound by latency, of five loads behind one
+// another (kept, path, table, codes and scales).
+template <int D>
+__global__ void __launch_bounds__(128) paged_keep_kernel(PagedKeepArgs a) {
+    constexpr int kChunks = D / 16, kTokens = 32 / kChunks;   // a lane's chunk of a token, tokens at a time
+    pdl_wait_release();
+    behind_wait(a.path, a.kept, a.b.header, a.b.layers);
+    if (a.b.header->state != kPagedKept) return;
+    const int lane = threadIdx.x & 31, P = a.b.page_tokens, c = lane % kChunks, r = lane / kChunks;
+    const size_t block = paged_block_bytes(P, D);
+    const long jobs = static_cast<long>(a.layers) * a.n * a.heads * 2;
+    for (long job = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 5); job < jobs; job += static_cast<long>(gridDim.x) * 4) {
+        const bool second = (job & 1) != 0;
+        long rest = job >> 1;
+        const int head = static_cast<int>(rest % a.heads);
+        rest /= a.heads;
+        const int i = static_cast<int>(rest % a.n), kept = a.kept[i];
+        const int* const path = a.path + static_cast<long>(i) * a.width;
+        // tokens in front of the first one that moves stay
+        int stay = 0;
+        for (bool all = true; all && stay < kept; stay += all ? 32 : 0) {
+            const unsigned int moves = __ballot_sync(0xffffffffu, stay + lane < kept && path[stay + lane] != stay + lane);
+            if (moves) {
+                stay += __ffs(static_cast<int>(moves)) - 1;
+                all = false;
+            }
+        }
+        if (stay >= kept) continue;
+        uint8_t* const layer = a.b.layers[rest / a.n];
+        const int first = a.b.held[i] - (a.b.starts[i + 1] - a.b.starts[i]);
+        const int* const table = a.b.tables + static_cast<size_t>(a.b.rows[i]) * a.b.max_pages;
+        auto codes_of = [&](int page) { return layer + (static_cast<size_t>(page) * a.heads + head) * block + (second ? static_cast<size_t>(P) * D : 0); };
+        auto scale_of = [&](int page) {
+            return reinterpret_cast<unsigned int*>(layer + (static_cast<size_t>(page) * a.heads + head) * block + 2 * static_cast<size_t>(P) * D) + (second ? 1 : 0);
+        };
+        auto chunk = [&](uint8_t* codes, int place) {
+            return reinterpret_cast<uint4*>(codes + static_cast<size_t>(place) * D + 16 * (second ? value_chunk<D>(place, c) : key_chunk<D>(place, c)));
+        };
+        for (int k = stay; k < kept;) {
+            const int idx = (first + k) / P, page = table[idx], upto = min(kept, (idx + 1) * P - first);
+            uint8_t* const codes = codes_of(page);
+            // from within the page
+            int near = k;   // behind the last of them (ascending: a prefix)
+            for (bool more = true; more && near < upto;) {
+                const int t = near + r, from = t < upto ? first + path[t] : 0;
+                const bool mine = t < upto && from / P == idx;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (mine) v = *chunk(codes, from % P);
+                __syncwarp();
+                if (mine) *chunk(codes, (first + t) % P) = v;
+                __syncwarp();
+                const int moved = __popc(__ballot_sync(0xffffffffu, mine && c == 0));
+                near += moved;
+                more = moved == kTokens;
+            }
+            if (near < upto) {   // from others
+                unsigned int* const scale_at = scale_of(page);
+                const unsigned int held = *scale_at;
+                unsigned int top = 0u;
+                for (int base = near; base < upto; base += kTokens) {
+                    const int t = base + r;
+                    if (t >= upto) continue;
+                    const int from = first + path[t], other = table[from / P];
+                    const unsigned int scale = *scale_of(other);
+                    const uint4 raw = *chunk(codes_of(other), from % P);
+                    if (scale >= 0x7f800000u) {
+                        top = scale;
+                        continue;
+                    }
+                    float v[16];
+                    decode16(v, raw, __uint_as_float(scale));
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                const unsigned int scale = max(scale_bits(top), held);   // (as bits: NaN is above the finite ones, and stays)
+                const bool finite = scale < 0x7f800000u;
+                if (finite && scale != held) {
+                    const float ratio = scale_ratio(held, scale);
+                    for (int t = r; t < P; t += kTokens) *chunk(codes, t) = rescaled16(*chunk(codes, t), ratio);
+                }
+                __syncwarp();
+                for (int base = near; base < upto; base += kTokens) {
+                    const int t = base + r;
+                    if (t >= upto) continue;
+                    const int from = first + path[t], other = table[from / P];
+                    uint4 v = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                    if (finite) v = rescaled16(*chunk(codes_of(other), from % P), scale_ratio(*scale_of(other), scale));
+                    *chunk(codes, (first + t) % P) = v;
+                }
+                __syncwarp();
+                if (lane == 0) *scale_at = scale;
+            }
+            __syncwarp();
+            k = upto;
+        }
+    }
+}
+
 template <int D, typename T, bool WIDE>
 void launch_append_typed(const PagedAppendArgs& a, cudaStream_t st) {
     // pieces that the plan can have: each of the requests begins and ends in a page of its own
@@ -530,6 +793,18 @@ void launch_paged_truncate(const PagedPlanArgs& a, cudaStream_t st) {
     static std::atomic<unsigned long long> set{0};
     launch_cluster(paged_truncate_kernel, plan_ctas(std::min<long>(static_cast<long>(a.n) * a.b.max_pages, a.b.num_pages)), true,
                    (3 * static_cast<size_t>(a.n) + 1) * sizeof(int), a, st, set);
+}
+void launch_paged_tree(const PagedTreeArgs& a, cudaStream_t st) {
+    launch_pdl(paged_tree_kernel, dim3(static_cast<unsigned int>(std::max(1, a.sizes.n))), dim3(kTreeThreads), 0, st, a);
+}
+void launch_paged_keep(const PagedKeepArgs& a, int dim, cudaStream_t st) {
+    static std::atomic<unsigned long long> set{0};
+    launch_cluster(paged_keep_plan_kernel, plan_ctas(std::min<long>(static_cast<long>(a.n) * a.b.max_pages, a.sizes.tokens / a.b.page_tokens + 2L * a.n)), true,
+                   (2 * static_cast<size_t>(a.n) + 1) * sizeof(int), a, st, set);
+    const long warps = static_cast<long>(a.layers) * a.n * a.heads * 2;
+    const dim3 grid(static_cast<unsigned int>(std::min<long>((warps + 3) / 4, 1 << 20)));
+    if (dim == 64) launch_pdl(paged_keep_kernel<64>, grid, dim3(128), 0, st, a);
+    else launch_pdl(paged_keep_kernel<128>, grid, dim3(128), 0, st, a);
 }
 void launch_paged_init(uint8_t* layer, size_t blocks, size_t block_bytes, cudaStream_t st) {
     paged_init_kernel<<<static_cast<unsigned int>(std::min<size_t>(blocks, 4096)), 256, 0, st>>>(layer, blocks, block_bytes);

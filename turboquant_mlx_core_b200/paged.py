@@ -95,6 +95,12 @@ def _rows(x, heads, dim, what, device):
     return x.data_ptr(), tokens, n, step if tokens > 1 else max(n * dim, step)
 
 
+def _number(x, what):
+    if len(x.shape) != 1:
+        raise ValueError(f"{what} must have one dimension")
+    return x.shape[0]
+
+
 def _tag(x, what):
     if x.dtype is _float16:
         return TQ_F16
@@ -121,6 +127,7 @@ class PagedKVCache:
     two for each page and head, on the device that is current here."""
 
     _device = -1       # no CUDA device's number
+    _planned = 0       # tokens of the last plan
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, num_pages: int, page_tokens: int = 64, max_requests: int = 256,
                  max_pages_per_request: int | None = None, max_tokens: int = 8192):
@@ -163,6 +170,30 @@ class PagedKVCache:
                                  _ints(lengths, "lengths", n, on), _ints(slots, "slots", tokens, on), _ints(positions, "positions", tokens, on),
                                  _ints(tables, "tables", n * width, on), width, None if stream is None else _stream_ptr(stream)):
             check(-1, "PagedKVCache.plan")
+        self._planned = tokens
+
+    def tree(self, parents=None, positions=None, stream=None):
+        """The planned tokens are trees of drafts: parents, an int32 tensor [tokens], is each token's parent, counted from its request's first new
+        token and in front of it, or -1; None: chains.  positions: int32 [tokens], filled with what a request held before and the token's depth."""
+        if parents is None and positions is None:
+            tokens = self._planned
+        else:
+            tokens = _number(parents if parents is not None else positions, "parents and positions")
+        if self._L.tq_paged_tree(self._h, _ints(parents, "parents", tokens, self._device), tokens, _ints(positions, "positions", tokens, self._device),
+                                 None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.tree")
+
+    def keep(self, path, kept, lengths=None, stream=None):
+        """Of each request's new tokens kept[i] stay, those that path[i] lists in ascending order (all of them where kept[i] is below 0), as
+        `verify_drafts` gives them; they move up in all layers, and the pages behind become free.  path [n, width], kept [n] and lengths [n] (filled with
+        the tokens that each request holds then) are int32 tensors."""
+        if len(path.shape) != 2:
+            raise ValueError("keep: path must be [n, width]")
+        n, width = path.shape
+        on = self._device
+        if self._L.tq_paged_keep(self._h, _ints(path, "path", n * width, on), width, _ints(kept, "kept", n, on), n, _ints(lengths, "lengths", n, on),
+                                 None if stream is None else _stream_ptr(stream)):
+            check(-1, "PagedKVCache.keep")
 
     def truncate(self, lengths, rows=None, stream=None):
         """The request in row rows[i] (row i without rows) keeps its first lengths[i] tokens; 0 releases it."""
@@ -249,3 +280,77 @@ class PagedKVCache:
             self.close()
         except Exception:
             pass
+
+
+def _device_of(x, what):
+    its = getattr(x, "get_device", None)
+    if its is None:
+        raise TypeError(f"{what} must be a torch CUDA tensor")
+    return its()
+
+
+def qk_norm_rope(queries, keys, query_weight, key_weight, positions, theta: float = 10000.0, eps: float = 1e-6, out=None, stream=None):
+    """The norm of each head of queries and keys, fp16 [tokens, heads, head_dim], and its rotation by `positions` (int32 [tokens]; what `plan` and `tree`
+    give) in one pass; a token's heads are contiguous, tokens may be apart.  The weights are fp16 [head_dim].  out: a pair of tensors, None: in
+    place.  Returns the pair."""
+    _load_torch()
+    on = _device_of(queries, "queries")
+    if len(queries.shape) != 3:
+        raise ValueError("queries must be [tokens, heads, head_dim]")
+    dim, out = queries.shape[2], (queries, keys) if out is None else out
+    at = []
+    for x, y, what in ((queries, out[0], "queries"), (keys, out[1], "keys")):
+        xp, n, heads, step = _rows(x, 0, dim, what, on)
+        yp, m, _, to = _rows(y, heads, dim, "out", on)
+        if x.dtype is not _float16 or y.dtype is not _float16:
+            raise TypeError(f"{what} and out must be float16")
+        if n != m or n != queries.shape[0]:
+            raise ValueError("queries, keys and out must have the same number of tokens")
+        at.append((xp, heads, step, yp, to))
+    weights = []
+    for w in (query_weight, key_weight):
+        if w.dtype is not _float16:
+            raise TypeError(f"weights must be float16, got {w.dtype}")
+        if w.shape != (dim,) or not w.is_contiguous():
+            raise ValueError(f"weights must be contiguous, [{dim}]")
+        if w.get_device() != on:
+            raise ValueError("weights are on another device than the queries")
+        weights.append(w.data_ptr())
+    tokens = queries.shape[0]
+    (qp, q_heads, qs, qo, qt), (kp, kv_heads, ks, ko, kt) = at
+    if _lib.load().tq_qk_norm_rope_f16(qp, kp, *weights, _ints(positions, "positions", tokens, on), tokens, q_heads, kv_heads, dim, qs, ks, eps, theta, qo, ko, qt, kt,
+                                       None if stream is None else _stream_ptr(stream)):
+        check(-1, "qk_norm_rope")
+    return out
+
+
+def verify_drafts(starts, parents, tokens, target, draft, uniforms, path, kept, next, stream=None):
+    """Which drafts stay: a walk down each request's tree that tests children against the target's probabilities with the given random numbers
+    (include/turboquant_c/turboquant_b200.h, tq_verify_drafts).  starts int32 [n + 1] (what `plan` gives), parents and tokens int32 [rows], target and
+    draft (or None: chosen drafts) fp32 or fp16 [rows, vocab], uniforms fp32 [rows].  Fills path [n, width], kept [n] and next [n], int32: what
+    `PagedKVCache.keep` takes, and the tokens that follow."""
+    _load_torch()
+    on = _device_of(starts, "starts")
+    if len(path.shape) != 2 or _number(starts, "starts") != path.shape[0] + 1:
+        raise ValueError("verify_drafts: path must be [n, width], starts [n + 1]")
+    (n, width), rows = path.shape, _number(tokens, "tokens")
+    at = []
+    for x, what in ((target, "target"), (draft, "draft")):
+        if x is None:
+            at += [None, 0]
+            continue
+        if x.shape != target.shape or len(x.shape) != 2 or x.shape[0] != rows or (x.shape[1] > 1 and x.stride(1) != 1):
+            raise ValueError(f"{what} must be [{rows}, vocab] with contiguous rows")
+        if x.dtype is not target.dtype:
+            raise ValueError("target and draft must have the same type")
+        if _device_of(x, what) != on:
+            raise ValueError(f"{what} is on another device than starts")
+        at += [x.data_ptr(), x.stride(0) if rows > 1 else max(x.stride(0), x.shape[1])]
+    if uniforms.dtype is not _float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous():
+        raise ValueError(f"uniforms must be contiguous float32 [{rows}]")
+    if _device_of(uniforms, "uniforms") != on:
+        raise ValueError("uniforms are on another device than starts")
+    if _lib.load().tq_verify_drafts(_ints(starts, "starts", n + 1, on), _ints(parents, "parents", rows, on), _ints(tokens, "tokens", rows, on), n, rows, at[0], at[2],
+                                    _tag(target, "verify_drafts"), _fits(target.shape[1], "vocab"), at[1], at[3], uniforms.data_ptr(), _ints(path, "path", n * width, on),
+                                    width, _ints(kept, "kept", n, on), _ints(next, "next", n, on), None if stream is None else _stream_ptr(stream)):
+        check(-1, "verify_drafts")
