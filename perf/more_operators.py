@@ -468,6 +468,8 @@ def _prepare_cache(case, seed):
             s["pages"] = torch.cat([tables[i, r.start:r.stop] for i, r in enumerate(spots)])
             size = (s["pages"].shape[0], page, case["kv_heads"], case["dim"])
             s["values"] = [[torch.empty(size, dtype=torch.float16, device=DEV) for _ in range(2)] for _ in layers]
+            rest = [c - len(p) for c, p in zip(counts, paths)]
+            s |= {"rest": torch.tensor(rest, **ints), "rest_sizes": (sum(rest), max(rest))}
     else:
         old = torch.tensor(held, device=DEV)
         request = torch.repeat_interleave(torch.arange(n, device=DEV), torch.tensor(counts, device=DEV))
@@ -531,6 +533,7 @@ def run(s):
         cache.keep(s["path"], s["kept"], lengths=s["lengths"])
         for i, kv in enumerate(s["values"]):
             cache.read_pages(i, s["pages"], *kv)
+        cache.plan(s["rest"], *s["rest_sizes"])      # (each request's pages again, so that the next pass takes them in this one's order)
         cache.truncate(s["held"])
         return s["positions"], s["lengths"], s["values"]
     total, page, held = s["total"], s["page"], s["held"]
