@@ -173,6 +173,7 @@ def load() -> C.CDLL:
     sig("tq_paged_append", i, [vp, i, vp, vp, i, i, C.c_long, C.c_long, vp])
     sig("tq_paged_read", i, [vp, i, vp, i, vp, vp, i, vp])
     sig("tq_paged_attention", i, [vp, i, vp, i, i, C.c_long, i, C.c_float, vp, C.c_long, vp, vp])
+    sig("tq_paged_tree_attention", i, [vp, i, vp, i, i, C.c_long, i, C.c_float, vp, C.c_long, vp, vp])
     sig("tq_paged_status", i, [vp])
     sig("tq_paged_free_pages", i, [vp])
 

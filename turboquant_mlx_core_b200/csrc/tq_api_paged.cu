@@ -177,9 +177,10 @@ public:
         tq::PagedReadArgs a{layers_[static_cast<size_t>(layer)].as<uint8_t>(), pages, keys, values, n, heads_, b_.page_tokens, b_.num_pages, d_status_};
         tq::launch_paged_read(a, dim_, dtype == TQ_F16, st);
     }
-    void attention(int layer, const void* q, int tokens, int q_heads, long q_stride, int window, float scale, void* out, long out_stride, float* lse, cudaStream_t st) {
+    void attention(int layer, const void* q, int tokens, int q_heads, long q_stride, int window, float scale, void* out, long out_stride, float* lse, bool tree, cudaStream_t st) {
         check_layer(layer);
         TQ_REQUIRE(plan_.n >= 0, "paged attention: no plan in force");
+        TQ_REQUIRE(!tree || tree_, "paged tree attention: the plan in force has no trees");
         TQ_REQUIRE(tokens == plan_.tokens, "paged attention: the plan is for " + std::to_string(plan_.tokens) + " tokens");
         TQ_REQUIRE(q_heads > 0 && q_heads % heads_ == 0, "paged attention: query heads must be a multiple of KV heads");
         TQ_REQUIRE(q_heads / heads_ <= 1024, "paged attention: more than 1024 query heads to a KV head");
@@ -206,6 +207,10 @@ public:
         a.page_shift = b_.page_tokens == 16 ? 4 : b_.page_tokens == 32 ? 5 : b_.page_tokens == 64 ? 6 : 7;
         a.scale_log2 = static_cast<float>((scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(dim_))) * 1.4426950408889634);
         a.status = d_status_;
+        if (tree) {
+            tq::launch_paged_tree_attention(a, dim_, static_cast<long>(plan_.most) * a.group, scratch_.as<char>() + prompt_scratch_, sms_, st);
+            return;
+        }
         // Up to kFewRows query rows of a request (new tokens times query heads to a KV head) go to the kernel for few rows.  Over 4096 tokens of 16
         // requests, there and in the kernel for many: 14 rows 30 and 49 us; in a form that took several times 16 rows of a request, 21 rows 48 and
         // 48, 35 rows 67 and 49; 20 rows over 32768 tokens of 4 requests 132 and 132. The device finds the requests of each kernel; a batch of one
@@ -336,7 +341,14 @@ int tq_paged_read(tq_paged_cache_t cache, int layer, const int* pages, int n, vo
 int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window, float scale,
                        void* out_fp16, long out_stride, float* lse, void* stream) {
     return guarded<int>(0, -1, [&]() {
-        paged(cache)->attention(layer, queries_fp16, tokens, q_heads, q_stride, window, scale, out_fp16, out_stride, lse, cuda_stream(stream));
+        paged(cache)->attention(layer, queries_fp16, tokens, q_heads, q_stride, window, scale, out_fp16, out_stride, lse, false, cuda_stream(stream));
+        return 0;
+    });
+}
+int tq_paged_tree_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window, float scale,
+                            void* out_fp16, long out_stride, float* lse, void* stream) {
+    return guarded<int>(0, -1, [&]() {
+        paged(cache)->attention(layer, queries_fp16, tokens, q_heads, q_stride, window, scale, out_fp16, out_stride, lse, true, cuda_stream(stream));
         return 0;
     });
 }
