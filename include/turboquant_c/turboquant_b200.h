@@ -636,8 +636,8 @@ int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp
                        float scale, void* out_fp16, long out_stride, float* lse, void* stream);
 /** The same for planned tokens that are trees (tq_paged_tree): a token sees those in front of its request's new ones, its ancestors and itself, with
  *  a window those of them whose positions are above its own less the window.  Rows of a request whose parents make no tree are left as they
- *  are.  Weights are rounded to halves: 2^-11 of each at most, and of small ones 2^-32 of the largest product of a weight and its value's
- *  scale that the row sees; values of scales below 2^-60 count as 0. */
+ *  are.  Weights are rounded to halves: 2^-11 of each at most, and of small ones 2^-32 of the row's largest weight, times the largest scale among
+ *  the values that the row sees. */
 int tq_paged_tree_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window,
                             float scale, void* out_fp16, long out_stride, float* lse, void* stream);
 /** Non-zero, once, when a call that has finished found its batch impossible or another plan on the device than the one that it was made for, or a wait

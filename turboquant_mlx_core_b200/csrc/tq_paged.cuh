@@ -204,7 +204,7 @@ void launch_paged_attention(PagedAttnArgs a, int dim, int max_rows, void* scratc
 size_t paged_prompt_scratch_bytes(int dim, int sms);
 void launch_paged_prompt(PagedAttnArgs a, int dim, long max_rows, void* scratch, int sms, cudaStream_t st);
 
-// Trees of drafts, of any number of rows (tq_paged_tree.cu); its scratch is the prompts'.
+// Trees of drafts, of any number of rows (tq_paged_prompt.cu; its scratch is the prompts').
 void launch_paged_tree_attention(PagedAttnArgs a, int dim, long max_rows, void* scratch, int sms, cudaStream_t st);
 
 // ---- what the attention kernels share -------------------------------------------------------------

@@ -7,17 +7,11 @@ namespace tq {
 
 namespace paged_device {
 
-// instruction descriptor: D fp32, A and B fp16, M = 128, N = n; A and B K-major, or (mn) with M and N in rows
-__host__ __device__ constexpr uint32_t instr_desc(uint32_t n, bool mn = false) {
-    return (1u << 4) | (mn ? 3u << 15 : 0u) | ((n >> 3) << 17) | (128u >> 4 << 24);
-}
+// instruction descriptor: D fp32, A and B fp16, both K-major, M = 128, N = n
+__host__ __device__ constexpr uint32_t instr_desc(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | (128u >> 4 << 24); }
 // shared-memory descriptor: K-major, no swizzle, 128 bytes from core matrix to core matrix along K, `group` from 8 rows to the next 8
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t group) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 16) | (static_cast<uint64_t>(group >> 4) << 32) | (1ull << 46);
-}
-// ... no swizzle, `along` bytes from 8 elements to the next 8 along K, `across` along M or N; K-major: `along` is of two core matrices of 8 x 16 bytes
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t along, uint32_t across) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(along >> 4) << 16) | (static_cast<uint64_t>(across >> 4) << 32) | (1ull << 46);
 }
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n  tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p; }"
@@ -64,6 +58,11 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[16]) {
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
                    "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                  :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 : : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 // Waits for this thread's loads; the registers of one of them go through it, so that nothing that uses them comes earlier.

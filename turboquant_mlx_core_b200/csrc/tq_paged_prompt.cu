@@ -91,13 +91,20 @@ struct Request {
     __device__ __forceinline__ int first() const { return held - count; }
     __device__ __forceinline__ int pairs() const { return (rows + kPairRows - 1) / kPairRows; }
     // tiles of the cache that the rows of a pair see
+    template <bool TREE>
     __device__ __forceinline__ void tiles(const PagedAttnArgs& a, int pair, int& lo, int& hi) const {
+        if constexpr (TREE) {   // (any row may see any place)
+            lo = a.window > 0 ? max(0, first() - a.window + 1) / kTokens : 0;
+            hi = (held - 1) / kTokens + 1;
+            return;
+        }
         const int last = first() + (min(rows, (pair + 1) * kPairRows) - 1) / a.group;
         hi = last / kTokens + 1;
         lo = a.window > 0 ? max(0, first() + pair * kPairRows / a.group - a.window + 1) / kTokens : 0;
     }
 };
 // The first request of many rows from i on (lanes look at 32 at a time); n if there is none.
+template <bool TREE>
 __device__ __forceinline__ int next_request(const PagedAttnArgs& a, int i, int n, int lane, Request& r) {
     for (int base = i; base < n; base += 32) {
         const int mine = min(base + lane, n - 1);
@@ -106,7 +113,8 @@ __device__ __forceinline__ int next_request(const PagedAttnArgs& a, int i, int n
         x.start = a.b.starts[mine];
         x.count = a.b.starts[mine + 1] - x.start;
         x.held = a.b.held[mine];
-        const bool many = base + lane < n && x.count * a.group > a.few_rows;
+        bool many = base + lane < n && x.count * a.group > a.few_rows;
+        if constexpr (TREE) many = many && a.b.nodes[x.start].good;
         const unsigned int found = __ballot_sync(0xffffffffu, many);
         if (found) {
             const int src = __ffs(static_cast<int>(found)) - 1;
@@ -121,11 +129,12 @@ __device__ __forceinline__ int next_request(const PagedAttnArgs& a, int i, int n
     return n;
 }
 // Tiles of all pairs of a request (the lanes take pairs in turn).
+template <bool TREE>
 __device__ __forceinline__ long long request_tiles(const PagedAttnArgs& a, const Request& r, int lane) {
     long long sum = 0;
     for (int p = lane; p < r.pairs(); p += 32) {
         int lo, hi;
-        r.tiles(a, p, lo, hi);
+        r.tiles<TREE>(a, p, lo, hi);
         sum += hi - lo + kItemUnits;
     }
 #pragma unroll
@@ -134,6 +143,7 @@ __device__ __forceinline__ long long request_tiles(const PagedAttnArgs& a, const
 }
 
 // A CTA's share of the units: (request, KV head, pair, tile), the tile running fastest.
+template <bool TREE>
 struct Walker {
     Request r;
     int i, n, head, pair, lo, hi, tile;
@@ -142,11 +152,11 @@ struct Walker {
     __device__ __forceinline__ void place(const PagedAttnArgs& a, int request, int requests, long long skip, long long units, int lane) {
         n = requests;
         left = units;
-        i = next_request(a, request, n, lane, r);
+        i = next_request<TREE>(a, request, n, lane, r);
         long long sum;
-        while (i < n && skip >= (sum = request_tiles(a, r, lane)) * a.heads) {
+        while (i < n && skip >= (sum = request_tiles<TREE>(a, r, lane)) * a.heads) {
             skip -= sum * a.heads;
-            i = next_request(a, i + 1, n, lane, r);
+            i = next_request<TREE>(a, i + 1, n, lane, r);
         }
         if (i >= n) {   // (not with a share of units that exist)
             left = 0;
@@ -156,7 +166,7 @@ struct Walker {
         skip -= head * sum;
         for (int base = 0;; base += 32) {   // the pair in which the rest lies
             int l = 0, h = 0;
-            if (base + lane < r.pairs()) r.tiles(a, base + lane, l, h);
+            if (base + lane < r.pairs()) r.template tiles<TREE>(a, base + lane, l, h);
             int upto = base + lane < r.pairs() ? h - l + kItemUnits : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -186,11 +196,11 @@ struct Walker {
             pair = 0;
             if (++head == a.heads) {
                 head = 0;
-                i = next_request(a, i + 1, n, lane, r);
+                i = next_request<TREE>(a, i + 1, n, lane, r);
                 if (i >= n) return false;
             }
         }
-        r.tiles(a, pair, lo, hi);
+        r.template tiles<TREE>(a, pair, lo, hi);
         tile = lo;
         before = kItemUnits;
         return left > before;
@@ -204,12 +214,17 @@ struct Segment {
     int begins, ends;              // whether it holds the item's first and last tile
     int last;                      // the CTA in which the item ends
     __device__ __forceinline__ bool two() const { return rows - row0 > kRows; }
+    // Row tiles that are at work; tiles of the cache that one takes, and the first of them
+    template <bool TREE>
+    __device__ __forceinline__ int teams() const { return two() || (TREE && tiles > 1) ? 2 : 1; }
+    template <bool TREE>
+    __device__ __forceinline__ bool split() const { return TREE && !two(); }
 };
 constexpr int kSegments = 4;
 constexpr int kSegmentReaders = 30;   // warps: softmax, products, queries, keys, values
 
 struct Bars {
-    unsigned long long q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], o_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], seg_full[kSegments], seg_empty[kSegments], done[2];
+    unsigned long long q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], o_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], merge, seg_full[kSegments], seg_empty[kSegments], done[2];
 };
 
 // The larger of powers of two and zeros by their bits, of those that are numbers.
@@ -233,12 +248,85 @@ __device__ __forceinline__ uint32_t scaled_halves(uint32_t w, uint32_t which, __
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int D>
+// The columns of a tile from token tb on that hold new tokens which the row of node `number` at position pos sees, as bits (by all lanes).
+__device__ __noinline__ uint64_t seen_nodes(const PagedAttnArgs& a, const Segment& at, int tb, int number, int pos, int lane) {
+    uint64_t seen = 0;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        const int token = tb + 32 * h + lane;
+        int lo = static_cast<int>(0x80000000u), place = 0;   // (no number is in there)
+        unsigned int span = 0;
+        if (token >= at.first && token < at.held) {
+            const PagedNode node = a.b.nodes[at.start + token - at.first];
+            lo = node.pre;
+            span = static_cast<unsigned int>(node.last - node.pre);
+            place = at.first + node.depth;
+        }
+        uint32_t bits = 0;
+#pragma unroll 8
+        for (int e = 0; e < 32; ++e) {
+            const int lo_e = __shfl_sync(0xffffffffu, lo, e), place_e = __shfl_sync(0xffffffffu, place, e);
+            const unsigned int span_e = __shfl_sync(0xffffffffu, span, e);
+            if (static_cast<unsigned int>(number - lo_e) <= span_e && (a.window <= 0 || place_e > pos - a.window)) bits |= 1u << e;
+        }
+        seen |= static_cast<uint64_t>(bits) << (32 * h);
+    }
+    return seen;
+}
+// The weights of a tile whose pages' values lie so far apart that their codes went into the product alone: sixteen columns of one page at a time, its
+// scale against the row's unit in the exponents.  Returns their sum, without the scales.  (Out of the way: its scores come from tensor memory again.)
+__device__ __noinline__ float apart_weights(uint32_t t_s, uint64_t seen, float f, float m, float4 parts, float vref) {
+    float all = 0.f;
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g) {
+        const float part = g == 0 ? parts.x : g == 1 ? parts.y : g == 2 ? parts.z : parts.w;
+        const float lower = part > 0.f ? static_cast<float>(max((static_cast<int>(__float_as_uint(part)) - static_cast<int>(__float_as_uint(vref))) >> 23, kLeastLower)) : 0.f;
+        const float shift = m - kOffset - lower;
+        uint32_t x[16], p[8];
+        tmem_ld(t_s + 16 * g, x);
+        tmem_ld_wait(x);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float w = seen >> (16 * g + e) & 1 ? exp2_approx(fmaf(__uint_as_float(x[e]), f, -shift)) : 0.f;
+            sum += w;
+            x[e] = __float_as_uint(w);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = pack_half2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        tmem_st(t_s + 8 * g, p);   // (columns that have been read)
+        all = fmaf(sum, exp2_approx(-lower), all);
+    }
+    return all;
+}
+// 32 dims of a row of the first team, and of the second's, in their units.
+__device__ __forceinline__ void add_second(uint32_t (&x)[32], uint32_t taddr, float first, float second) {
+    uint32_t y[32];
+    tmem_ld(taddr, y);
+    tmem_ld_wait(y);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(fmaf(__uint_as_float(y[e]), second, __uint_as_float(x[e]) * first));
+}
+
+// TREE: trees of drafts (paged_tree_kernel in tq_paged_plan.cu numbers the nodes): a row sees the tokens in front of the new ones, its ancestors and
+// itself.  A request has some tens to some hundreds of rows there, so that many items have no second row tile; its warps then take every second
+// tile of the cache for the first one's rows, with a maximum, a sum and an O of their own, and the two are added up at the item's end (both read the
+// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 64 thousand tokens of 4 heads: 48 us; a team's step takes 2.8 thousand
+// cycles there, 0.9 of which it waits for scores, whose keys' conversion takes 3.4 for every second tile.  Tried beside it, in the same case: the
+// products turned around (tokens as their 128 rows, query rows as 32, 64 or 128 columns, a softmax thread per token), which takes a tile's products as
+// long as there are rows: 90 us, since each thread then keeps a sum for every row and four warps have to agree on every reference; keys and values
+// from memory through registers to their place, without the bytes in shared memory: 58, with 24 words spilled.
+template <int D, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_constant__ PagedAttnArgs a) {
     using S = Shape<D>;
     extern __shared__ __align__(1024) uint8_t s_mem[];
     __shared__ __align__(8) Bars s_bar;
-    __shared__ long long s_sum[kWarps];
+    // units of each warp's requests; later the second team's maximum, sum and unit (its exponent) of each row: there is no more room
+    __shared__ __align__(16) uint8_t s_room[TREE ? 9 * kRows : kWarps * 8];
+    long long* const s_sum = reinterpret_cast<long long*>(s_room);
+    float* const s_top2 = reinterpret_cast<float*>(s_room);
+    float* const s_sum2 = s_top2 + (TREE ? kRows : 0);
+    uint8_t* const s_unit2 = s_room + (TREE ? 8 * kRows : 0);
     __shared__ float s_kref[kRefs], s_vref[kRefs];
     __shared__ __align__(16) float s_vpart[kRefs][kTokens / kWarpTokens];   // the values' scales of a tile's parts, of one page each
     __shared__ __align__(16) Segment s_seg[kSegments];
@@ -264,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             bar_init(bar(s_bar.v_full[k]), 4);
             bar_init(bar(s_bar.v_empty[k]), 1);
         }
+        bar_init(bar(s_bar.merge), 4);
         for (int k = 0; k < kSegments; ++k) {
             bar_init(bar(s_bar.seg_full[k]), 1);
             bar_init(bar(s_bar.seg_empty[k]), kSegmentReaders);
@@ -272,13 +361,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait_release();
-    const int n = planned(a.b.header, a.sizes, a.status).requests;
+    int n = planned(a.b.header, a.sizes, a.status).requests;
+    if constexpr (TREE) {
+        if (n > 0 && a.b.header->state != kPagedTree) {   // (a plan of the same sizes that has no trees)
+            if (blockIdx.x == 0 && tid == 0) raise_status(a.status, kPagedOtherPlan);
+            n = 0;
+        }
+    }
     const int per = (n + kWarps - 1) / kWarps;
     {
         const int end = min(n, (warp + 1) * per);
         long long mine = 0;
         Request r;
-        for (int i = next_request(a, warp * per, end, lane, r); i < end; i = next_request(a, i + 1, end, lane, r)) mine += request_tiles(a, r, lane) * a.heads;
+        for (int i = next_request<TREE>(a, warp * per, end, lane, r); i < end; i = next_request<TREE>(a, i + 1, end, lane, r)) mine += request_tiles<TREE>(a, r, lane) * a.heads;
         if (lane == 0) s_sum[warp] = mine;
     }
     __syncthreads();
@@ -324,22 +419,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         const uint32_t t_s0 = tmem + lanes + t * 2 * kTokens, t_o = tmem + lanes + 4 * kTokens + t * D;
         const bool out_wide = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * 2)) & 15) == 0;
         uint32_t done = 0, count = 0;   // tiles of this thread's so far, and of the share (their scales' place)
+        uint32_t merged = 0;            // items that two teams shared
         while (next_segment()) {
             const Segment& at = s_seg[seg_n % kSegments];
             const int tiles = at.tiles, tile0 = at.tile;
-            if (t == 0 || at.two()) {
-                const int row = at.row0 + t * kRows + r_in, in_row = min(row, at.rows - 1);
-                const int token = at.start + in_row / a.group, hq = at.head * a.group + in_row % a.group, pos = at.first + in_row / a.group;
+            if (t < at.teams<TREE>()) {
+                const bool split = at.split<TREE>();
+                const int row = at.row0 + (split ? 0 : t * kRows) + r_in, in_row = min(row, at.rows - 1);
+                const int token = at.start + in_row / a.group, hq = at.head * a.group + in_row % a.group;
+                int pos = at.first + in_row / a.group, number = 0;   // (TREE: by the node's depth; its number)
+                if constexpr (TREE) {
+                    const PagedNode node = a.b.nodes[token];
+                    pos = at.first + node.depth;
+                    number = node.pre;
+                }
                 const bool live = row < at.rows;
                 const int oldest = a.window > 0 ? max(0, pos - a.window + 1) : 0;
                 // A warp without rows: it keeps the others' count (16 requests of 35 rows: 48 us, 56 with the softmax of what is not there)
-                const bool idle = at.row0 + t * kRows + 32 * (warp & 3) >= at.rows;
+                const bool idle = at.row0 + (split ? 0 : t * kRows) + 32 * (warp & 3) >= at.rows;
                 // O is in units of vref: the largest of the values' scales that the row has seen (vseen), or the tile's where it sees only part of
                 // the tile and the rest is larger.  It comes down again behind such a tile: a window that begins there has all its other tokens in
                 // front.
                 float m = -INFINITY, l = 0.f, vref = 0.f, vseen = 0.f;
-                for (int j = 0; j < tiles; ++j) {
-                    const uint32_t ref = (count + j) & (kRefs - 1), n = done + j;
+                const int step = split ? 2 : 1, j0 = split ? t : 0;
+                uint32_t n = done;
+                for (int j = j0; j < tiles; j += step, ++n) {
+                    const uint32_t ref = (count + j) & (kRefs - 1);
                     if (!wait(s_bar.s_full[t][n & 1], (n >> 1) & 1)) break;
                     if (idle) {
                         if (lane == 0) bar_arrive(bar(s_bar.p_full[t][n & 1]));
@@ -348,19 +453,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     fence_after();
                     const uint32_t t_s = t_s0 + (n & 1) * kTokens;
                     uint32_t x[32], y[32];
-                    const float kref = s_kref[ref], vref_here = s_vref[ref];
+                    const float kref = s_kref[ref], vref_here = TREE ? fabsf(s_vref[ref]) : s_vref[ref];
+                    const bool apart = TREE && s_vref[ref] < 0.f;   // the codes are there alone
                     tmem_ld(t_s, x);
                     tmem_ld(t_s + 32, y);
                     const int tb = (tile0 + j) * kTokens;
                     const float f = fmaxf(kref * a.scale_log2, 1.1754944e-38f);   // (not 0: minus infinity times it)
-                    const int newest = pos - tb, eldest = oldest - tb;   // columns eldest .. newest are seen
-                    float vt = newest >= 0 && eldest < kTokens ? vref_here : 0.f, vpart = vt;   // (what a row does not see leaves its unit alone)
+                    // columns eldest .. newest are seen (TREE: and new tokens by their nodes)
+                    const int newest = (TREE ? at.first - 1 : pos) - tb, eldest = oldest - tb;
+                    float vt = TREE || (newest >= 0 && eldest < kTokens) ? vref_here : 0.f, vpart = vt;   // (what a row does not see leaves its unit alone)
+                    uint64_t all_seen = ~0ull;   // (TREE)
                     tmem_ld_wait(x);
                     tmem_ld_wait(y);
                     if (__any_sync(0xffffffffu, newest < kTokens - 1 || eldest > 0)) {
                         // a bit for each column
-                        const uint64_t seen = (newest >= 63 ? ~0ull : newest < 0 ? 0ull : (2ull << newest) - 1) & (eldest <= 0 ? ~0ull : eldest > 63 ? 0ull : ~0ull << eldest);
+                        uint64_t seen = (newest >= 63 ? ~0ull : newest < 0 ? 0ull : (2ull << newest) - 1) & (eldest <= 0 ? ~0ull : eldest > 63 ? 0ull : ~0ull << eldest);
+                        if constexpr (TREE) seen |= seen_nodes(a, at, tb, number, pos, lane);
                         const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+                        if constexpr (TREE) all_seen = seen;
                         const float4 parts = *reinterpret_cast<const float4*>(s_vpart[ref]);
                         vpart = fmaxf(fmaxf(lo & 0xffffu ? parts.x : 0.f, lo >> 16 ? parts.y : 0.f), fmaxf(hi & 0xffffu ? parts.z : 0.f, hi >> 16 ? parts.w : 0.f));
                         if (code_factor(__float_as_uint(vpart), __float_as_uint(vt)) < kLeastFactor) vt = 0.f;   // (all that it sees counts as 0)
@@ -375,6 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     for (int e = 0; e < 32; ++e) tops[e & 3] = fmaxf(fmaxf(tops[e & 3], __uint_as_float(x[e])), __uint_as_float(y[e]));
                     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     top *= f;   // (f is positive; NaN columns do not count)
+                    float4 parts = make_float4(0.f, 0.f, 0.f, 0.f);   // (apart) the scales of what the row sees, sixteen columns each
+                    if (apart) {
+                        parts = *reinterpret_cast<const float4*>(s_vpart[ref]);
+                        parts.x = all_seen & 0xffffu ? parts.x : 0.f;
+                        parts.y = all_seen & 0xffff0000u ? parts.y : 0.f;
+                        parts.z = all_seen & 0xffff00000000u ? parts.z : 0.f;
+                        parts.w = all_seen >> 48 ? parts.w : 0.f;
+                        vt = vpart = fmaxf(fmaxf(parts.x, parts.y), fmaxf(parts.z, parts.w));
+                    }
                     const bool jump = top > m + kSlack || (m == -INFINITY && top > m);
                     float both = 1.f;
                     vseen = fmaxf(vseen, vpart);
@@ -405,12 +524,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         }
                         tmem_st16(to, p);
                     };
-                    weights(x, t_s);
-                    weights(y, t_s + 16);
-                    const float2 both_sums = unpack2(add2(sums[0], sums[1]));
-                    const float sum = both_sums.x + both_sums.y;
-                    l = fmaf(sum, exp2_approx(-lower), l);
-                    if (moves && j > 0) {   // O to the new reference: behind the weights, which take as long as the products that it waits for
+                    if (apart) {
+                        l += apart_weights(t_s, all_seen, f, m == -INFINITY ? 0.f : m, parts, vref);
+                    } else {
+                        weights(x, t_s);
+                        weights(y, t_s + 16);
+                        const float2 both_sums = unpack2(add2(sums[0], sums[1]));
+                        const float sum = both_sums.x + both_sums.y;
+                        l = fmaf(sum, exp2_approx(-lower), l);
+                    }
+                    if (moves && j > j0) {   // O to the new reference: behind the weights, which take as long as the products that it waits for
                         if (!wait(s_bar.o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1)) break;
                         fence_after();
 #pragma unroll 1
@@ -427,11 +550,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     __syncwarp();
                     if (lane == 0) bar_arrive(bar(s_bar.p_full[t][n & 1]));
                 }
-                done += tiles;
-                if (wait(s_bar.o_done[t][(done - 1) & 1], ((done - 1) >> 1) & 1)) {
+                done += (tiles - j0 + step - 1) / step;
+                bool last = wait(s_bar.o_done[t][(done - 1) & 1], ((done - 1) >> 1) & 1);
+                const bool shared = split && tiles > 1;
+                float second = 0.f;   // the second team's unit, against this one's reference
+                if constexpr (TREE) {
+                    if (last && shared) {
+                        if (t == 1) {
+                            s_top2[r_in] = m;
+                            s_sum2[r_in] = l;
+                            s_unit2[r_in] = static_cast<uint8_t>(__float_as_uint(vref) >> 23);
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(bar(s_bar.merge));
+                            last = false;   // (the first team does the rest)
+                        } else {
+                            last = wait(s_bar.merge, merged++ & 1);
+                            const float m1 = s_top2[r_in], top = fmaxf(m, m1);
+                            const float x0 = m == top || m == -INFINITY ? 1.f : exp2_approx(m - top), x1 = m1 == top || m1 == -INFINITY ? 1.f : exp2_approx(m1 - top);
+                            l = fmaf(l, x0, s_sum2[r_in] * x1);
+                            vref *= x0;
+                            second = __uint_as_float(static_cast<uint32_t>(s_unit2[r_in]) << 23) * x1 * (1.f / kHeadroom);
+                            m = top;
+                        }
+                    }
+                }
+                if (last) {
                     fence_after();
                     const bool begins = at.begins, ends = at.ends;
-                    const float unit = vref * (1.f / kHeadroom);
+                    float unit = vref * (1.f / kHeadroom), one = unit;
+                    if (shared) unit = 1.f;
                     uint32_t x[32];
                     if (begins && ends) {
                         const float inv = unit / l;
@@ -440,6 +588,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         for (int q = 0; q < D / 32; ++q) {
                             tmem_ld(t_o + 32 * q, x);
                             tmem_ld_wait(x);
+                            if constexpr (TREE) {
+                                if (shared) add_second(x, t_o + D + 32 * q, one, second);
+                            }
                             if (!live) continue;
 #pragma unroll
                             for (int e = 0; e < 32; e += 8) {
@@ -458,6 +609,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         for (int q = 0; q < D / 32; ++q) {
                             tmem_ld(t_o + 32 * q, x);
                             tmem_ld_wait(x);
+                            if constexpr (TREE) {
+                                if (shared) add_second(x, t_o + D + 32 * q, one, second);
+                            }
 #pragma unroll
                             for (int e = 0; e < 32; e += 4)
                                 *reinterpret_cast<float4*>(part + ((8 * q + e / 4) * kPairRows + pr) * 4) =
@@ -470,7 +624,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     }
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(bar(s_bar.o_empty[t]));
+                    if (lane == 0) {
+                        bar_arrive(bar(s_bar.o_empty[t]));
+                        if (TREE && shared) bar_arrive(bar(s_bar.o_empty[1]));
+                    }
                 }
             }
             count += tiles;
@@ -500,30 +657,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             while (until(s_bar.seg_full[seg_n % kSegments], (seg_n / kSegments) & 1)) {
                 const int tiles = s_seg[seg_n % kSegments].tiles, pair = s_seg[seg_n % kSegments].two() ? 2 : 1;
                 if (tiles == 0) break;
+                const bool split = s_seg[seg_n % kSegments].split<TREE>();   // (row tile t takes the tiles t, t + 2, ... with the first one's queries)
 #pragma unroll 1
                 for (int j = 0; j < tiles; ++j, ++turns) {
                     const uint32_t stage = turns % kStages, turn = (turns / kStages) & 1;
                     if (!until(first ? s_bar.k_full[stage] : s_bar.v_full[stage], turn)) break;
 #pragma unroll 1
-                    for (int t = 0; t < pair; ++t) {
+                    for (int t = split ? j & 1 : 0; t < (split ? (j & 1) + 1 : pair); ++t) {
                         const uint32_t nt = t ? n1 : n0, place = nt & 1, t_s = tmem + (2 * t + place) * kTokens;
                         if (first) {
-                            if (j == 0 && !until(s_bar.q_full[t], (items >> t) & 1)) break;
+                            if (j == 0 && !until(s_bar.q_full[split ? 0 : t], (items >> t) & 1)) break;
                             // P of two tiles before was where these scores go
                             if (nt >= 2 && !until(s_bar.o_done[t][place], ((nt >> 1) - 1) & 1)) break;
                             fence_after();
-                            const uint64_t q = q_desc + t * (S::kQBytes >> 4), k = k_desc + stage * (S::kKBytes >> 4);
+                            const uint64_t q = q_desc + (split ? 0 : t) * (S::kQBytes >> 4), k = k_desc + stage * (S::kKBytes >> 4);
 #pragma unroll
                             for (int s = 0; s < D / 16; ++s) umma_ss(t_s, q + 16 * s, k + 16 * s, kIdescS, s > 0);
                             umma_commit(bar(s_bar.s_full[t][place]));
-                            if (j + 1 == tiles) umma_commit(bar(s_bar.q_empty[t]));
+                            if (j + 1 == tiles) umma_commit(bar(s_bar.q_empty[split ? 0 : t]));
                         } else {
-                            if (j == 0 && !until(s_bar.o_empty[t], ((items >> t) & 1) ^ 1)) break;
+                            const bool begins = j == (split ? t : 0);
+                            if (begins && !until(s_bar.o_empty[t], ((items >> t) & 1) ^ 1)) break;
                             if (!until(s_bar.p_full[t][place], (nt >> 1) & 1)) break;
                             fence_after();
                             const uint64_t v = v_desc + stage * (S::kVBytes >> 4);
 #pragma unroll
-                            for (int s = 0; s < kTokens / 16; ++s) umma_ts(tmem + 4 * kTokens + t * D, t_s + 8 * s, v + 16 * s, kIdescO, j > 0 || s > 0);
+                            for (int s = 0; s < kTokens / 16; ++s) umma_ts(tmem + 4 * kTokens + t * D, t_s + 8 * s, v + 16 * s, kIdescO, !begins || s > 0);
                             umma_commit(bar(s_bar.o_done[t][place]));
                         }
                         if (t) ++n1; else ++n0;
@@ -531,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     if (!go) break;
                     umma_commit(bar(first ? s_bar.k_empty[stage] : s_bar.v_empty[stage]));
                 }
-                items ^= pair == 2 ? 3u : 1u;
+                items ^= pair == 2 || (!first && split && tiles > 1) ? 3u : 1u;
                 bar_arrive(bar(s_bar.seg_empty[seg_n % kSegments]));
                 ++seg_n;
             }
@@ -580,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         }
         if (warp == kScheduleWarp) {
             const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
-            Walker at;
+            Walker<TREE> at;
             long long front = 0;
             int w = 0;
             while (w + 1 < kWarps && front + s_sum[w] <= u0) front += s_sum[w++];
@@ -665,12 +824,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             // a page whose values are not numbers is one whose keys are not: its tokens' columns become NaN
             const uint32_t key_bits = here.y < 0x7f800000u ? here.x : 0x7fc00000u, value_bits = here.y < 0x7f800000u ? here.y : 0u;
             const uint32_t value_ref = largest_scale(value_bits);
+            // (TREE) Pages whose values would not be exact in the largest one's unit, which may be one that hardly any row sees: the codes go there alone, and
+            // the weights have the scales.
+            const bool apart = TREE && __any_sync(0xffffffffu, value_bits != 0u && code_factor(value_bits, value_ref) < kLeastFactor);
             if (keys) {
                 // lane = (row of 8, chunk of 4)
                 const uint32_t ref = largest_scale(key_bits);
                 const __half2 fa = __float2half2_rn(code_factor(__shfl_sync(0xffffffffu, key_bits, page), ref)), off = __hmul2(fa, __float2half2_rn(-1152.f));
                 uint8_t* const dst = s_mem + S::kK + stage * S::kKBytes + 2 * w * S::kRowGroup + (lane & 7) * 16;
-#pragma unroll 1
+#pragma unroll(TREE ? 2 : 1)
                 for (int s = 0; s < D / 32; ++s) {
                     const int r = 8 * (s & 1) + (lane & 7), c0 = (lane >> 3) + 2 * (s & 2);
                     const uint4 b4 = *reinterpret_cast<const uint4*>(raw + r * D + 16 * raw_chunk<D>(r, key_chunk<D>(r, c0)));
@@ -690,14 +852,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     if (lane < kTokens / kWarpTokens) s_vpart[now.n & (kRefs - 1)][lane] = __uint_as_float(part);
                     if (lane == 0) {
                         s_kref[now.n & (kRefs - 1)] = ref > 0u ? __uint_as_float(ref) * (1.f / kHeadroom) : 1.f;
-                        s_vref[now.n & (kRefs - 1)] = __uint_as_float(value_ref);
+                        s_vref[now.n & (kRefs - 1)] = apart ? -__uint_as_float(value_ref) : __uint_as_float(value_ref);
                     }
                 }
             } else {
                 // a lane takes four dims of eight tokens
                 constexpr int kLanes = D / 4, kGroups = 32 / kLanes;   // groups of 8 tokens side by side in a warp
                 const int d4 = lane % kLanes;
-                const __half2 fa = __float2half2_rn(code_factor(__shfl_sync(0xffffffffu, value_bits, page), value_ref)), off = __hmul2(fa, __float2half2_rn(-1152.f));
+                const __half2 fa = __float2half2_rn(apart ? kHeadroom : code_factor(__shfl_sync(0xffffffffu, value_bits, page), value_ref)), off = __hmul2(fa, __float2half2_rn(-1152.f));
                 uint8_t* const dst = s_mem + S::kV + stage * S::kVBytes + (d4 >> 1) * S::kDimGroup + (d4 & 1) * 64 + 2 * w * 128;
 #pragma unroll 1
                 for (int s = 0; s < 2; s += kGroups) {
@@ -825,13 +987,13 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) paged_prompt_join_kernel(co
     }
 }
 
-template <int D>
+template <int D, bool TREE>
 void launch_typed(PagedAttnArgs a, long max_rows, void* scratch, int sms, cudaStream_t st) {
     a.joins = static_cast<PagedJoin*>(scratch);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(scratch) + (sms * sizeof(PagedJoin) + 255) / 256 * 256);
     static std::atomic<unsigned long long> set{0};
-    allow_shared_memory(paged_prompt_kernel<D>, Shape<D>::kSmem, set);
-    launch_pdl_carved(paged_prompt_kernel<D>, dim3(static_cast<unsigned int>(sms)), dim3(kThreads), Shape<D>::kSmem, 100, st, a);
+    allow_shared_memory(paged_prompt_kernel<D, TREE>, Shape<D>::kSmem, set);
+    launch_pdl_carved(paged_prompt_kernel<D, TREE>, dim3(static_cast<unsigned int>(sms)), dim3(kThreads), Shape<D>::kSmem, 100, st, a);
     const auto join = [&](auto kernel, int rows) {
         launch_pdl_carved(kernel, dim3(static_cast<unsigned int>(sms), static_cast<unsigned int>((std::min<long>(kPairRows, max_rows) + rows - 1) / rows)), dim3(kJoinRows * D / 4), 0, 100, st, a);
     };
@@ -845,8 +1007,13 @@ size_t paged_prompt_scratch_bytes(int dim, int sms) {
     return (sms * sizeof(PagedJoin) + 255) / 256 * 256 + static_cast<size_t>(sms) * 2 * kPairRows * (static_cast<size_t>(dim) + 2) * sizeof(float);
 }
 void launch_paged_prompt(PagedAttnArgs a, int dim, long max_rows, void* scratch, int sms, cudaStream_t st) {
-    if (dim == 64) launch_typed<64>(a, max_rows, scratch, sms, st);
-    else launch_typed<128>(a, max_rows, scratch, sms, st);
+    if (dim == 64) launch_typed<64, false>(a, max_rows, scratch, sms, st);
+    else launch_typed<128, false>(a, max_rows, scratch, sms, st);
+}
+void launch_paged_tree_attention(PagedAttnArgs a, int dim, long max_rows, void* scratch, int sms, cudaStream_t st) {
+    a.few_rows = 0;
+    if (dim == 64) launch_typed<64, true>(a, max_rows, scratch, sms, st);
+    else launch_typed<128, true>(a, max_rows, scratch, sms, st);
 }
 
 }  // namespace tq
