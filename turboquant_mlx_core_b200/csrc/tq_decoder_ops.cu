@@ -9,6 +9,7 @@
 #include <cstdint>
 
 #include "tq_common.cuh"
+#include "tq_host.hpp"
 #include "tq_kernels.cuh"
 
 namespace tq {
@@ -97,9 +98,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(__half* __restr
 // of 2^-64 turns, of which a 64-bit product keeps the fraction, 2^-34 off at most whatever the position (in fp32 it is a hundredth off at
 // position 131072).
 //
-// A thread takes eight pairs of a head, 16 bytes from either half, so that the rotation stays in its registers; `lanes` threads, the next power
-// of two above D / 16, share a head and its sum of squares.  It is bound by memory (few rows: by latency): 16 bytes in and out for eight
-// elements, asked for in front of the sines and cosines, which D / 2 threads take for all heads of a row.
+// A thread takes eight pairs of a head, 16 bytes from either half, so that the rotation stays in its registers, and the same pairs of the same head
+// in several rows, so that it keeps the weights and finds its place once; `lanes` threads, the next power of two above D / 16, share a head and its sum
+// of squares.  It is bound by memory, 16 bytes in and out for eight elements (few rows: by latency, 2.6 us): a row's values are asked for while the one
+// before is at work, the first one's in front of the sines and cosines, which D / 2 threads take for all heads of a row.  8192 rows of 40 + 8 heads of
+// 128: 44.6 us, 4.5 TB/s, 69 % of a plain copy's rate (52 with a row to a CTA, whose threads find head and pair anew for each 64 bytes; 44.8 with three
+// CTAs to an SM instead of two, in 56 registers): some 200 instructions for 64 bytes are what is left beside memory.
 constexpr int kHeadHalfMax = 256;
 struct QkNormArgs {
     const __half* x[2];       // queries, keys
@@ -108,7 +112,8 @@ struct QkNormArgs {
     long x_stride[2], y_stride[2];   // elements from row to row
     const int* positions;
     long rows;
-    int heads[2], dim, lanes, rows_per_cta;
+    int heads[2], dim, lanes;
+    int width, rounds, beside, rows_each;   // threads of a row, and their rounds; rows side by side in a CTA, and one behind the other
     float eps;
     unsigned long long turns[kHeadHalfMax];   // frequencies in 2^-64 turns
 };
@@ -139,78 +144,71 @@ __device__ __forceinline__ void store_head(__half* p, const uint4& v) {
 template <bool WIDE>
 __global__ void __launch_bounds__(512) qk_norm_rope_kernel(const __grid_constant__ QkNormArgs a) {
     ops_dependency_sync();
-    extern __shared__ float2 s_turn[];   // [rows_per_cta][dim / 2] cosine, sine
-    const int half = a.dim >> 1, per_row = (a.heads[0] + a.heads[1]) * a.lanes;
-    const long row0 = static_cast<long>(blockIdx.x) * a.rows_per_cta;
-    const int rows = static_cast<int>(min(static_cast<long>(a.rows_per_cta), a.rows - row0)), items = rows * per_row;
-    struct Item {
-        const __half* x;
-        __half* y;
-        int which, row, at;   // queries or keys; row of the CTA's; its first pair
-        bool live;
-    };
-    auto item = [&](int i) {
-        Item it;
-        it.row = min(i / per_row, rows - 1);
-        const int in = i - it.row * per_row, h = in / a.lanes, t = in - h * a.lanes;
-        it.which = h >= a.heads[0] ? 1 : 0;
-        it.at = 8 * t;
-        it.live = i < items && it.at < half;
-        const long row = row0 + it.row, off = static_cast<long>(it.which ? h - a.heads[0] : h) * a.dim + it.at;
-        it.x = a.x[it.which] + row * a.x_stride[it.which] + off;
-        it.y = a.y[it.which] + row * a.y_stride[it.which] + off;
-        return it;
-    };
-    auto load = [&](const Item& it, uint4& lo, uint4& hi) {
-        lo = hi = make_uint4(0u, 0u, 0u, 0u);
-        if (it.live) {
-            lo = load_head<WIDE>(it.x);
-            hi = load_head<WIDE>(it.x + half);
+    extern __shared__ __align__(16) float2 s_turn[];   // [rows of the CTA][dim / 2] cosine, sine
+    const int half = a.dim >> 1, all = (a.heads[0] + a.heads[1]) * a.lanes, rows_cta = a.beside * a.rows_each;
+    const long row0 = static_cast<long>(blockIdx.x) * rows_cta;
+    const int rows = static_cast<int>(min(static_cast<long>(rows_cta), a.rows - row0));
+    const int mine = a.beside > 1 ? static_cast<int>(threadIdx.x) / a.width : 0, place = static_cast<int>(threadIdx.x) - mine * a.width;
+    for (int round = 0; round < a.rounds; ++round) {   // (by all threads: the barrier, the sums' shuffles)
+        const int i = min(place + round * a.width, all - 1), h = i / a.lanes, t = 8 * (i - h * a.lanes), which = h >= a.heads[0] ? 1 : 0;
+        const bool live = t < half && mine < a.beside && place + round * a.width < all;
+        const long at = static_cast<long>(which ? h - a.heads[0] : h) * a.dim + t;
+        const __half* x = a.x[which] + (row0 + mine) * a.x_stride[which] + at;
+        __half* y = a.y[which] + (row0 + mine) * a.y_stride[which] + at;
+        const long x_step = a.beside * a.x_stride[which], y_step = a.beside * a.y_stride[which];
+        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo, wl = lo, wh = lo;
+        if (live && mine < rows) {
+            lo = load_head<WIDE>(x);
+            hi = load_head<WIDE>(x + half);
         }
-    };
-    Item it = item(threadIdx.x);
-    uint4 lo, hi;
-    load(it, lo, hi);
-    for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
-        const int r = i / half, p = i - r * half;
-        const unsigned long long turn = static_cast<unsigned long long>(static_cast<long long>(a.positions[row0 + r])) * a.turns[p];
-        const float t = static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f;   // half turns, -1 .. 1
-        float s, c;
-        sincospif(t, &s, &c);
-        s_turn[i] = make_float2(c, s);
-    }
-    __syncthreads();
-    // (all lanes of a warp go round as often: the sums' shuffles)
-    for (int i = threadIdx.x; i - static_cast<int>(threadIdx.x & 31) < items;) {
-        float u[8], v[8];
-        unpack_halves(lo, u);
-        unpack_halves(hi, v);
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(u[j], u[j], fmaf(v[j], v[j], sum));
-        for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const Item now = it;
-        i += blockDim.x;
-        if (i - static_cast<int>(threadIdx.x & 31) < items) {
-            it = item(i);
-            load(it, lo, hi);
+        if (live) {
+            wl = load_head<WIDE>(a.w[which] + t);
+            wh = load_head<WIDE>(a.w[which] + t + half);
         }
-        if (!now.live) continue;
-        const float scale = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+        if (round == 0) {
+            for (int k = threadIdx.x; k < rows * half; k += blockDim.x) {
+                const int r = k / half, p = k - r * half;
+                const unsigned long long turn = static_cast<unsigned long long>(static_cast<long long>(a.positions[row0 + r])) * a.turns[p];
+                const float angle = static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f;   // half turns, -1 .. 1
+                float s, c;
+                sincospif(angle, &s, &c);
+                s_turn[k] = make_float2(c, s);
+            }
+            __syncthreads();
+        }
         float g[8], k[8];
-        const __half* const w = a.w[now.which] + now.at;
-        unpack_halves(load_head<WIDE>(w), g);
-        unpack_halves(load_head<WIDE>(w + half), k);
-        const float2* const turn = s_turn + now.row * half + now.at;
+        unpack_halves(wl, g);
+        unpack_halves(wh, k);
+        for (int r = mine; r - mine < rows; r += a.beside) {   // (warps stay together: rows that are not there are zeros)
+            float u[8], v[8];
+            unpack_halves(lo, u);
+            unpack_halves(hi, v);
+            float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 cs = turn[j];
-            const float p = u[j] * scale * g[j], q = v[j] * scale * k[j];
-            u[j] = p * cs.x - q * cs.y;
-            v[j] = q * cs.x + p * cs.y;
+            for (int j = 0; j < 8; ++j) sum = fmaf(u[j], u[j], fmaf(v[j], v[j], sum));
+            __half* const to = y;
+            x += x_step;
+            y += y_step;
+            if (live && r + a.beside < rows) {
+                lo = load_head<WIDE>(x);
+                hi = load_head<WIDE>(x + half);
+            }
+            for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (!live || r >= rows) continue;
+            const float scale = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+            const float4* const turn = reinterpret_cast<const float4*>(s_turn + r * half + t);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float4 two = turn[j >> 1];
+                const float p0 = u[j] * scale * g[j], q0 = v[j] * scale * k[j], p1 = u[j + 1] * scale * g[j + 1], q1 = v[j + 1] * scale * k[j + 1];
+                u[j] = p0 * two.x - q0 * two.y;
+                v[j] = q0 * two.x + p0 * two.y;
+                u[j + 1] = p1 * two.z - q1 * two.w;
+                v[j + 1] = q1 * two.z + p1 * two.w;
+            }
+            store_head<WIDE>(to, pack_halves(u));
+            store_head<WIDE>(to + half, pack_halves(v));
         }
-        store_head<WIDE>(now.y, pack_halves(u));
-        store_head<WIDE>(now.y + half, pack_halves(v));
     }
 }
 
@@ -336,12 +334,16 @@ void launch_qk_norm_rope_f16(const __half* q, const __half* k, const __half* q_w
     uintptr_t all = 0;
     for (int i = 0; i < 2; ++i)
         all |= reinterpret_cast<uintptr_t>(a.x[i]) | reinterpret_cast<uintptr_t>(a.w[i]) | reinterpret_cast<uintptr_t>(a.y[i]) | static_cast<uintptr_t>(2 * (a.x_stride[i] | a.y_stride[i]));
-    // Threads of a row, and rows to a CTA of some 256 threads where a row has fewer.
-    const int per_row = (q_heads + kv_heads) * a.lanes, turns = (per_row + 511) / 512;
-    a.rows_per_cta = static_cast<int>(std::min<long>(std::max(1, 256 / per_row), rows));
-    const int threads = std::min(512, (a.rows_per_cta * ((per_row + turns - 1) / turns) + 31) / 32 * 32);
-    const dim3 grid(static_cast<unsigned>((rows + a.rows_per_cta - 1) / a.rows_per_cta)), block(static_cast<unsigned>(threads));
-    const size_t smem = static_cast<size_t>(a.rows_per_cta) * (dim / 2) * sizeof(float2);
+    // Threads of a row (in several rounds above 512, then of whole warps); rows side by side where a row has few, and as many behind one another, up to
+    // four, as leave four CTAs to each SM.
+    const int per_row = (q_heads + kv_heads) * a.lanes;
+    a.rounds = (per_row + 511) / 512;
+    a.width = a.rounds == 1 ? per_row : ((per_row + a.rounds - 1) / a.rounds + 31) / 32 * 32;
+    a.beside = static_cast<int>(std::min<long>(std::max(1, 256 / a.width), rows));
+    a.rows_each = static_cast<int>(std::min<long>(4, std::max<long>(1, rows / (a.beside * 4L * sm_count(current_device())))));
+    const int rows_cta = a.beside * a.rows_each, threads = (a.beside * a.width + 31) / 32 * 32;
+    const dim3 grid(static_cast<unsigned>((rows + rows_cta - 1) / rows_cta)), block(static_cast<unsigned>(threads));
+    const size_t smem = static_cast<size_t>(rows_cta) * (dim / 2) * sizeof(float2);
     if (all % 16 == 0) launch_pdl(qk_norm_rope_kernel<true>, grid, block, smem, stream, a);
     else launch_pdl(qk_norm_rope_kernel<false>, grid, block, smem, stream, a);
 }

@@ -15,8 +15,9 @@
 // order.  The warp in whose part the sum passes u0 Z goes over it once more.  Sums, products and comparisons are in 64 bits: a token is a whole
 // number, and a comparison of sums in 32 bits would go wrong next to a border, of which there are as many as tokens.
 //
-// It is bound by the two rows that a request's walk ends at (few requests: by the latency of three loads behind one another, a pass, the
-// cluster's barriers).
+// What bounds it: few requests, latency (three loads behind one another, a pass, the cluster's barriers, the last part once more: 10 us for one); many,
+// the passes, each of them two conversions to 64 bits for every token, of which an SM makes 16 a cycle: 64 requests of 16 nodes in 39 us, 2 TB/s of
+// the rows that walks end at.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -31,6 +32,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCtas = 8;
+constexpr int kAtOnce = 2;   // 16-byte pieces of a row that a lane asks for at once (four, and one CTA to an SM: 52 us instead of 39 below)
 
 template <typename T>
 __device__ __forceinline__ float probability(const T* row, int x) {
@@ -38,29 +40,61 @@ __device__ __forceinline__ float probability(const T* row, int x) {
     return p > 0.f ? p : 0.f;   // (NaN too)
 }
 
-// Elements e .. e + VEC - 1 of a row, 0 beyond its end and for what is no positive number.
-template <typename T, int VEC, bool WIDE>
-__device__ __forceinline__ void load_row(float (&v)[VEC], const T* row, int e, int vocab) {
-    if (WIDE && e + VEC <= vocab) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(row + e);
-        if constexpr (sizeof(T) == 2) {
-            unpack_halves(raw, v);
+// 16 bytes of a row, elements e and on; zeros beyond its end.
+template <typename T, bool WIDE>
+__device__ __forceinline__ uint4 load_row(const T* row, int e, int end) {
+    constexpr int VEC = 16 / sizeof(T);
+    if (WIDE && e + VEC <= end) return *reinterpret_cast<const uint4*>(row + e);
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+            w[k] = e + k < end ? __float_as_uint(row[e + k]) : 0u;
         } else {
-            v[0] = __uint_as_float(raw.x);
-            v[1] = __uint_as_float(raw.y);
-            v[2] = __uint_as_float(raw.z);
-            v[3] = __uint_as_float(raw.w);
+            const uint32_t lo = e + 2 * k < end ? __half_as_ushort(row[e + 2 * k]) : 0u, hi = e + 2 * k + 1 < end ? __half_as_ushort(row[e + 2 * k + 1]) : 0u;
+            w[k] = lo | hi << 16;
         }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = v[k] > 0.f ? v[k] : 0.f;
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = e + k < vocab ? probability(row, e + k) : 0.f;
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// They as numbers, 0 for what is no positive one.
+template <typename T>
+__device__ __forceinline__ void numbers(float (&v)[16 / sizeof(T)], const uint4& raw) {
+    if constexpr (sizeof(T) == 2) {
+        unpack_halves(raw, v);
+    } else {
+        v[0] = __uint_as_float(raw.x);
+        v[1] = __uint_as_float(raw.y);
+        v[2] = __uint_as_float(raw.z);
+        v[3] = __uint_as_float(raw.w);
+    }
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) v[k] = v[k] > 0.f ? v[k] : 0.f;
 }
 
+// The parts' sums, four (or fewer) to a lane, in the lanes' order: the lane's and all in front of it.
+struct PartSums {
+    double each[kMaxCtas * kWarps / 32], upto, total;
+    __device__ __forceinline__ void load(const double* sums, int parts, int lane) {
+        constexpr int kEach = kMaxCtas * kWarps / 32;
+        const int per = (parts + 31) / 32;
+        upto = 0.;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            each[k] = k < per && lane * per + k < parts ? sums[lane * per + k] : 0.;
+            upto += each[k];
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31);
+    }
+};
+
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs a) {
     constexpr int VEC = 16 / sizeof(T), kGroup = 32 * VEC;
     pdl_wait_release();
     extern __shared__ uint32_t s_gone[];   // without q: tokens of this CTA's part of the vocabulary that were rejected, a bit each
@@ -74,6 +108,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     const cg::cluster_group cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank()), i = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    cluster.barrier_arrive();
     const bool drawn = a.draft != nullptr;
     const int start = a.starts[i], end = a.starts[i + 1];
     // (a request without nodes, or one that is not inside the rows, has none)
@@ -86,6 +121,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
                 a.next[i] = -1;
             }
         }
+        cluster.barrier_wait();
         return;   // (the whole cluster)
     }
     const T* const target = static_cast<const T*>(a.target) + start * a.target_stride;
@@ -104,14 +140,46 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     if (!drawn)
         for (int k = tid; k < words; k += kThreads) s_gone[k] = 0u;
     __syncthreads();
-    cluster.sync();   // every CTA of it runs: its shared memory may be written
+    cluster.barrier_wait();   // every CTA of it runs: its shared memory may be written
 
     const int mine0 = (rank * kWarps + warp) * a.segment;   // this warp's part of the vocabulary
     int now = 0, at = 1, kept = 1, rejected = 0, turn = 0;
     double subtract = 0., left = 1.;
     if (tid == 0) s_path[0] = 0;
+    // The sum of this warp's part of w = max(p - s q, 0) (without q: of p, but for tokens that are gone).
+    auto part_sum = [&](const T* p_row, const T* q_row, double s, bool gaps) {
+        double sum = 0.;
+        const int part_end = min(mine0 + a.segment, a.vocab);
+        for (int e0 = mine0; e0 < part_end; e0 += kAtOnce * kGroup) {
+            uint4 p[kAtOnce], q[kAtOnce];
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b) {
+                const int e = e0 + b * kGroup + lane * VEC;
+                p[b] = load_row<T, WIDE>(p_row, e, part_end);
+                if (q_row) q[b] = load_row<T, WIDE>(q_row, e, part_end);
+            }
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b) {
+                const int at = e0 + b * kGroup + lane * VEC - rank * kWarps * a.segment;
+                const uint32_t gone = gaps && at < kWarps * a.segment ? s_gone[at >> 5] >> (at & 31) : 0u;
+                float v[VEC], u[VEC];
+                numbers<T>(v, p[b]);
+                if (q_row) {
+                    numbers<T>(u, q[b]);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) sum += fmax(static_cast<double>(v[k]) - s * u[k], 0.);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) sum += gone >> k & 1u ? 0. : static_cast<double>(v[k]);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        return sum;
+    };
     bool fresh = true, over = false;   // no rejection at this node; the walk is over
-    double total = 0., before = 0.;
+    double total = 0.;
     for (;;) {
         // ---- the walk, by the first warp of each CTA, up to the next pass ----
         if (warp == 0) {
@@ -184,28 +252,12 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
         const T* const p_row = target + s_now * a.target_stride;
         const T* const q_row = drawn && s_subtract > 0. ? draft + s_now * a.draft_stride : nullptr;
         const double s = s_subtract;
-        double sum = 0.;
-        for (int e0 = mine0; e0 < min(mine0 + a.segment, a.vocab); e0 += kGroup) {
-            const int e = e0 + lane * VEC;
-            float p[VEC], q[VEC];
-            load_row<T, VEC, WIDE>(p, p_row, e, a.vocab);
-            if (q_row) {
-                load_row<T, VEC, WIDE>(q, q_row, e, a.vocab);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) sum += fmax(static_cast<double>(p[k]) - s * q[k], 0.);
-            } else {
-                uint32_t gone = 0u;
-                if (!drawn) gone = s_gone[(e - rank * kWarps * a.segment) >> 5] >> ((e - rank * kWarps * a.segment) & 31);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) sum += gone >> k & 1u ? 0. : static_cast<double>(p[k]);
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double sum = part_sum(p_row, q_row, s, !drawn);
         if (lane < ctas) *cluster.map_shared_rank(&s_sum[turn & 1][rank * kWarps + warp], lane) = sum;
         cluster.sync();
-        total = 0.;
-        for (int k = 0; k < ctas * kWarps; ++k) total += s_sum[turn & 1][k];
+        PartSums parts;
+        parts.load(s_sum[turn & 1], ctas * kWarps, lane);
+        total = parts.total;
         ++turn;
         left = total;
         if (state == 1) break;
@@ -220,82 +272,112 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
         // Nothing is left (a target that its draft covers but for roundings): the target's row as it is.
         whole = true;
         s = 0.;
-        double sum = 0.;
-        for (int e0 = mine0; e0 < min(mine0 + a.segment, a.vocab); e0 += kGroup) {
-            float p[VEC];
-            load_row<T, VEC, WIDE>(p, target + now * a.target_stride, e0 + lane * VEC, a.vocab);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) sum += static_cast<double>(p[k]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double sum = part_sum(target + now * a.target_stride, nullptr, 0., false);
         if (lane < ctas) *cluster.map_shared_rank(&s_sum[last_turn ^ 1][rank * kWarps + warp], lane) = sum;
         cluster.sync();
-        total = 0.;
-        for (int k = 0; k < ctas * kWarps; ++k) total += s_sum[last_turn ^ 1][k];
     }
-    const double* const sums = s_sum[whole ? last_turn ^ 1 : last_turn];
+    PartSums parts;
+    parts.load(s_sum[whole ? last_turn ^ 1 : last_turn], ctas * kWarps, lane);
     // the part in which the sum passes u total: the last one with anything where none does
+    const double limit = u * parts.total;
     int owner = -1;
+    double before = 0.;
     {
-        const double limit = u * total;
-        double running = 0.;
-        for (int k = 0; k < ctas * kWarps; ++k) {
-            if (sums[k] > 0.) {
-                owner = k;
-                before = running;
-            }
-            running += sums[k];
-            if (owner == k && running > limit) break;
-        }
-        if (rank == 0) {
-            for (int k = tid; k < a.width; k += kThreads) a.path[static_cast<long>(i) * a.width + k] = k < s_kept ? s_path[k] : -1;
-            if (tid == 0) {
-                a.kept[i] = s_kept;
-                if (owner < 0) a.next[i] = -1;
+        constexpr int kEach = kMaxCtas * kWarps / 32;
+        const int per = (ctas * kWarps + 31) / 32;
+        int last = -1, passing = -1;   // of the lane's parts
+        double at[kEach], upto = __shfl_up_sync(0xffffffffu, parts.upto, 1);
+        if (lane == 0) upto = 0.;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            at[k] = upto;
+            upto += parts.each[k];
+            if (parts.each[k] > 0.) {
+                last = k;
+                if (passing < 0 && upto > limit) passing = k;
             }
         }
-        if (owner == rank * kWarps + warp) {
-            int found = -1, positive = -1;   // the token; the last one so far that could be
-            double sum = before;
-            for (int e0 = mine0; found < 0 && e0 < min(mine0 + a.segment, a.vocab); e0 += kGroup) {
-                const int e = e0 + lane * VEC;
-                float p[VEC], q[VEC];
-                double w[VEC], own = 0.;
-                load_row<T, VEC, WIDE>(p, target + now * a.target_stride, e, a.vocab);
-                if (s > 0.) load_row<T, VEC, WIDE>(q, draft + now * a.draft_stride, e, a.vocab);
-                uint32_t gone = 0u;
-                if (!drawn && !whole) gone = s_gone[(e - rank * kWarps * a.segment) >> 5] >> ((e - rank * kWarps * a.segment) & 31);
+        const unsigned int some = __ballot_sync(0xffffffffu, last >= 0), beyond = __ballot_sync(0xffffffffu, passing >= 0);
+        const int src = beyond ? __ffs(static_cast<int>(beyond)) - 1 : some ? 31 - __clz(static_cast<int>(some)) : 0;
+        const int k = __shfl_sync(0xffffffffu, beyond ? passing : last, src);
+        if (some) owner = src * per + k;
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    w[k] = s > 0. ? fmax(static_cast<double>(p[k]) - s * q[k], 0.) : gone >> k & 1u ? 0. : static_cast<double>(p[k]);
-                    own += w[k];
-                }
-                double upto = own;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double t = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += t;
-                }
-                const unsigned int some = __ballot_sync(0xffffffffu, own > 0.), beyond = __ballot_sync(0xffffffffu, own > 0. && sum + upto > limit);
-                int token = -1, last = -1;
-                double running = sum + (upto - own);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    running += w[k];
-                    if (w[k] > 0.) {
-                        last = e + k;
-                        if (token < 0 && running > limit) token = e + k;
-                    }
-                }
-                if (token < 0) token = last;   // (the lane's own sum rounded otherwise)
-                if (beyond) found = __shfl_sync(0xffffffffu, token, __ffs(static_cast<int>(beyond)) - 1);
-                else if (some) positive = __shfl_sync(0xffffffffu, last, 31 - __clz(static_cast<int>(some)));
-                sum += __shfl_sync(0xffffffffu, upto, 31);
-            }
-            if (lane == 0) a.next[i] = found >= 0 ? found : positive;
+        for (int i = 0; i < kEach; ++i)
+            if (i == k) before = at[i];
+        before = __shfl_sync(0xffffffffu, before, src);
+    }
+    if (rank == 0) {
+        for (int k = tid; k < a.width; k += kThreads) a.path[static_cast<long>(i) * a.width + k] = k < s_kept ? s_path[k] : -1;
+        if (tid == 0) {
+            a.kept[i] = s_kept;
+            if (owner < 0) a.next[i] = -1;
         }
     }
+    if (owner != rank * kWarps + warp) return;
+    int found = -1, positive = -1;   // the token; the last one so far that could be
+    double sum = before;
+    const int part_end = min(mine0 + a.segment, a.vocab);
+    for (int e0 = mine0; found < 0 && e0 < part_end; e0 += kAtOnce * kGroup) {
+        uint4 p[kAtOnce], q[kAtOnce];
+#pragma unroll
+        for (int b = 0; b < kAtOnce; ++b) {
+            const int e = e0 + b * kGroup + lane * VEC;
+            p[b] = load_row<T, WIDE>(target + now * a.target_stride, e, part_end);
+            if (s > 0.) q[b] = load_row<T, WIDE>(draft + now * a.draft_stride, e, part_end);
+        }
+        auto weights = [&](double (&w)[VEC], int b) {
+            float v[VEC], u[VEC];
+            numbers<T>(v, p[b]);
+            if (s > 0.) {
+                numbers<T>(u, q[b]);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) w[k] = fmax(static_cast<double>(v[k]) - s * u[k], 0.);
+            } else {
+                const int at = e0 + b * kGroup + lane * VEC - rank * kWarps * a.segment;
+                const uint32_t gone = !drawn && !whole && at < kWarps * a.segment ? s_gone[at >> 5] >> (at & 31) : 0u;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) w[k] = gone >> k & 1u ? 0. : static_cast<double>(v[k]);
+            }
+        };
+        double own[kAtOnce], upto[kAtOnce];
+#pragma unroll
+        for (int b = 0; b < kAtOnce; ++b) {
+            double w[VEC];
+            weights(w, b);
+            own[b] = 0.;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) own[b] += w[k];
+            upto[b] = own[b];
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b) {
+                const double t = __shfl_up_sync(0xffffffffu, upto[b], o);
+                if (lane >= o) upto[b] += t;
+            }
+#pragma unroll
+        for (int b = 0; b < kAtOnce; ++b) {
+            if (found >= 0) continue;
+            const unsigned int some = __ballot_sync(0xffffffffu, own[b] > 0.), beyond = __ballot_sync(0xffffffffu, own[b] > 0. && sum + upto[b] > limit);
+            int token = -1, last = -1;
+            double running = sum + (upto[b] - own[b]), w[VEC];
+            weights(w, b);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                running += w[k];
+                if (w[k] > 0.) {
+                    last = e0 + b * kGroup + lane * VEC + k;
+                    if (token < 0 && running > limit) token = last;
+                }
+            }
+            if (token < 0) token = last;   // (the lane's own sum rounded otherwise)
+            if (beyond) found = __shfl_sync(0xffffffffu, token, __ffs(static_cast<int>(beyond)) - 1);
+            else if (some) positive = __shfl_sync(0xffffffffu, last, 31 - __clz(static_cast<int>(some)));
+            sum += __shfl_sync(0xffffffffu, upto[b], 31);
+        }
+    }
+    if (lane == 0) a.next[i] = found >= 0 ? found : positive;
 }
 
 }  // namespace
@@ -303,6 +385,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 void launch_verify_drafts(VerifyArgs a, int n, bool half, cudaStream_t st) {
     if (n == 0) return;
     const int es = half ? 2 : 4, group = 32 * 16 / es;
+    // CTAs to a request: as many as there are pieces for, up to 8 (the portable most), however many requests there are: they take one to many passes, and
+    // the ones behind fill up (64 requests of 16 nodes, 151936 tokens: 39 us; with two CTAs each, which run all at once, 56, with four 44).
     int ctas = 1;
     while (ctas < kMaxCtas && ctas * kWarps * group < a.vocab) ctas *= 2;
     a.segment = ((a.vocab + ctas * kWarps - 1) / (ctas * kWarps) + group - 1) / group * group;
