@@ -330,7 +330,12 @@ void launch_qk_norm_rope_f16(const __half* q, const __half* k, const __half* q_w
     a.lanes = 1;
     while (a.lanes * 16 < dim) a.lanes *= 2;
     constexpr double kTwoPi = 6.283185307179586476925286766559;
-    for (int i = 0; i < dim / 2; ++i) a.turns[i] = static_cast<unsigned long long>(std::llrint(std::pow(static_cast<double>(theta), -2.0 * i / dim) / kTwoPi * 18446744073709551616.0));
+    // (a power for every eighth, the others eight products of it at most: 2^-50 off, where a power each took two thirds of the call)
+    const double ratio = std::pow(static_cast<double>(theta), -2.0 / dim);
+    for (int i = 0; i < dim / 2; i += 8) {
+        double turn = std::pow(static_cast<double>(theta), -2.0 * i / dim) / kTwoPi * 18446744073709551616.0;
+        for (int k = i; k < i + 8; ++k, turn *= ratio) a.turns[k] = static_cast<unsigned long long>(std::llrint(turn));
+    }
     uintptr_t all = 0;
     for (int i = 0; i < 2; ++i)
         all |= reinterpret_cast<uintptr_t>(a.x[i]) | reinterpret_cast<uintptr_t>(a.w[i]) | reinterpret_cast<uintptr_t>(a.y[i]) | static_cast<uintptr_t>(2 * (a.x_stride[i] | a.y_stride[i]));

@@ -304,29 +304,26 @@ def qk_norm_rope(queries, keys, query_weight, key_weight, positions, theta: floa
     on = _device_of(queries, "queries")
     if len(queries.shape) != 3:
         raise ValueError("queries must be [tokens, heads, head_dim]")
-    dim, out = queries.shape[2], (queries, keys) if out is None else out
-    at = []
-    for x, y, what in ((queries, out[0], "queries"), (keys, out[1], "keys")):
-        xp, n, heads, step = _rows(x, 0, dim, what, on)
-        yp, m, _, to = _rows(y, heads, dim, "out", on)
-        if x.dtype is not _float16 or y.dtype is not _float16:
-            raise TypeError(f"{what} and out must be float16")
-        if n != m or n != queries.shape[0]:
-            raise ValueError("queries, keys and out must have the same number of tokens")
-        at.append((xp, heads, step, yp, to))
-    weights = []
+    dim = queries.shape[2]
+    qp, tokens, q_heads, qs = _rows(queries, 0, dim, "queries", on)
+    kp, more, kv_heads, ks = _rows(keys, 0, dim, "keys", on)
+    if out is None:
+        out, qo, qt, ko, kt, qn, kn = (queries, keys), qp, qs, kp, ks, tokens, tokens
+    else:
+        qo, qn, _, qt = _rows(out[0], q_heads, dim, "out", on)
+        ko, kn, _, kt = _rows(out[1], kv_heads, dim, "out", on)
+    if not tokens == more == qn == kn:
+        raise ValueError("queries, keys and out must have the same number of tokens")
+    half = _float16
+    if not (queries.dtype is half and keys.dtype is half and out[0].dtype is half and out[1].dtype is half and query_weight.dtype is half and key_weight.dtype is half):
+        raise TypeError("queries, keys, weights and out must be float16")
     for w in (query_weight, key_weight):
-        if w.dtype is not _float16:
-            raise TypeError(f"weights must be float16, got {w.dtype}")
         if w.shape != (dim,) or not w.is_contiguous():
             raise ValueError(f"weights must be contiguous, [{dim}]")
         if w.get_device() != on:
             raise ValueError("weights are on another device than the queries")
-        weights.append(w.data_ptr())
-    tokens = queries.shape[0]
-    (qp, q_heads, qs, qo, qt), (kp, kv_heads, ks, ko, kt) = at
-    if _lib.load().tq_qk_norm_rope_f16(qp, kp, *weights, _ints(positions, "positions", tokens, on), tokens, q_heads, kv_heads, dim, qs, ks, eps, theta, qo, ko, qt, kt,
-                                       None if stream is None else _stream_ptr(stream)):
+    if _lib.load().tq_qk_norm_rope_f16(qp, kp, query_weight.data_ptr(), key_weight.data_ptr(), _ints(positions, "positions", tokens, on), tokens, q_heads, kv_heads, dim,
+                                       qs, ks, eps, theta, qo, ko, qt, kt, None if stream is None else _stream_ptr(stream)):
         check(-1, "qk_norm_rope")
     return out
 
