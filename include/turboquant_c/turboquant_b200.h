@@ -406,7 +406,8 @@ int tq_qk_norm_rope_f16(const void* q_fp16, const void* k_fp16, const void* q_we
  *  path [n, width]: the nodes that stay, node 0 the first, -1 behind them; kept [n]: how many they are; next [n].  A request without nodes, or whose
  *  rows are not inside the `rows`, keeps none and has next -1, as has one without a token that could be.  A node without a parent in front of it, or
  *  with a token outside the vocabulary, is nobody's child.  Of a request's nodes the first 1024 are looked at; vocab up to 2^20, n up to 65536.
- *  All pointers are device pointers of one device, whichever is current.  Fastest where pointers and strides are multiples of 16 bytes. */
+ *  All pointers are device pointers of one device, whichever is current; results must not be where an argument or another result is.  Fastest where
+ *  pointers and strides are multiples of 16 bytes. */
 int tq_verify_drafts(const int* starts, const int* parents, const int* tokens, int n, int rows, const void* target, const void* draft, int dtype, int vocab,
                      long target_stride, long draft_stride, const float* uniforms, int* path, int width, int* kept, int* next, void* stream);
 
@@ -611,7 +612,7 @@ int tq_paged_tree(tq_paged_cache_t cache, const int* parents, int tokens, int* p
  *  0.  In all layers they move up to the places of the first new ones, and the pages behind become free.  A token that stays in its page keeps
  *  its numbers; one that joins another page joins it as an append of its values would, and where the page's scale grows all that the page holds is
  *  rounded once more.  path [n, width], kept [n] and lengths [n] (may be NULL; the tokens that each request holds then) are device memory, n is
- *  the plan's.  A path that is none changes nothing (tq_paged_status tells).  Ends the plan in force. */
+ *  the plan's; lengths must not be where the other two are.  A path that is none changes nothing (tq_paged_status tells).  Ends the plan in force. */
 int tq_paged_keep(tq_paged_cache_t cache, const int* path, int width, const int* kept, int n, int* lengths, void* stream);
 /** Keys and values [tokens, heads, head_dim] of the planned tokens (TQ_F32 or TQ_F16), token t at t * stride elements (heads * head_dim
  *  or more: a slice of a fused projection's result), into a layer.  `tokens` is the plan's; rows behind the last request's are not read.

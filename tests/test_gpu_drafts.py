@@ -276,3 +276,13 @@ def test_a_large_vocabulary_on_another_stream_and_replayed(tq):
             for i, rows in enumerate((slice(0, 3), slice(3, 5))):
                 path, token = drafts_model.verify(s[0][i], s[1][rows], s[2][rows], None if s[3] is None else s[3][rows], s[4][rows], 3)
                 assert out["path"][i].tolist()[:len(path)] == path and int(out["kept"][i]) == len(path) and int(out["next"][i]) == token
+
+
+def test_results_where_arguments_are(tq):
+    rng = np.random.default_rng(12)
+    parents, tokens, target, draft, u = batch(rng, [5, 6], 40, 2, True)
+    starts, drafted, uniforms = ints([0, 5, 11]), ints(tokens), torch.from_numpy(u).cuda()
+    out = outputs(2, 4)
+    for change in ({"next": drafted[3:5]}, {"kept": starts[1:]}, {"next": out["kept"]}, {"kept": out["path"].view(-1)[6:]}, {"path": uniforms.view(torch.int32)[:8].view(2, 4)}):
+        with pytest.raises(tq.TQError, match="must not be where"):
+            tq.verify_drafts(starts, ints(np.concatenate(parents)), drafted, on_device(target), on_device(draft), uniforms, **{**out, **change})

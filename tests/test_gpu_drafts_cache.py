@@ -314,3 +314,70 @@ def test_a_captured_step(tq):
         assert lengths.tolist() == want
         p.compare(pages)
     p.c.close()
+
+
+def test_a_branch_is_kept_once(tq):
+    """A captured keep that is replayed again without a plan moves nothing more, and the status tells."""
+    rng = np.random.default_rng(9)
+    p = Pair(tq, 2, 64, 16, 2, 20)
+    p.step(rng, [20, 10], [0, 1])
+    path, kept, lengths = ints([[1, 3, 4], [0, 2, -1]]), ints([3, 2]), torch.full((2,), 9, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    p.step(rng, [5, 5], [0, 1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        p.c.keep(path, kept, lengths=lengths, stream=side)
+    graph.replay()
+    for m in p.m:
+        for which in (0, 1):
+            drafts_model.keep(m, which, [[1, 3, 4], [0, 2]])
+        m.truncate([23, 12], [0, 1])
+    assert lengths.tolist() == [23, 12]
+    p.compare(20)
+    for _ in range(2):
+        lengths.fill_(9)
+        graph.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(tq.TQError, match="plan on the device"):
+            p.c.check_status()
+        assert lengths.tolist() == [9, 9]
+        p.compare(20)
+    p.c.close()
+
+
+def test_results_where_the_paths_are(tq):
+    """Refused: the moves read the paths and their lengths behind the bookkeeping.  Next to them they may be."""
+    rng = np.random.default_rng(10)
+    p = Pair(tq, 1, 64, 16, 2, 20)
+    p.step(rng, [20, 10], [0, 1])
+    p.step(rng, [5, 5], [0, 1])
+    block = ints([0, 4, 1, 2, 2, 2, 77, 77])
+    path, kept = block[:4].view(2, 2), block[4:6]
+    for lengths in (kept, block[5:7], block[3:5], block[:2]):
+        with pytest.raises(tq.TQError, match="must not be where"):
+            p.c.keep(path, kept, lengths=lengths)
+    p.c.keep(path, kept, lengths=block[6:])
+    for which in (0, 1):
+        drafts_model.keep(p.m[0], which, [[0, 4], [1, 2]])
+    p.m[0].truncate([22, 12], [0, 1])
+    assert block.tolist() == [0, 4, 1, 2, 2, 2, 22, 12]
+    p.compare(20)
+    p.c.close()
+
+
+def test_paths_in_wide_rows(tq):
+    """A path's row may be longer than any request's new tokens; what is behind it is not looked at."""
+    rng = np.random.default_rng(11)
+    p = Pair(tq, 1, 64, 16, 2, 20)
+    p.step(rng, [20, 10], [0, 1])
+    p.step(rng, [5, 3], [0, 1])
+    path = torch.full((2, 70000), 1 << 30, dtype=torch.int32, device="cuda")
+    path[0, :2], path[1, :3] = ints([2, 4]), ints([0, 1, 2])
+    p.c.keep(path, ints([2, 3]))
+    for which in (0, 1):
+        drafts_model.keep(p.m[0], which, [[2, 4], [0, 1, 2]])
+    p.m[0].truncate([22, 13], [0, 1])
+    p.compare(20)
+    p.c.close()

@@ -130,6 +130,9 @@ public:
         if (n == 0) return;
         TQ_REQUIRE(tq::is_device_pointer(path) && tq::is_device_pointer(kept) && (!lengths || tq::is_device_pointer(lengths)),
                    "paged keep: paths, their lengths and results must be device pointers");
+        // (the kernel behind the bookkeeping reads both again)
+        TQ_REQUIRE(tq::ranges_apart(lengths, 4ul * n, kept, 4ul * n) && tq::ranges_apart(lengths, 4ul * n, path, 4ul * n * width),
+                   "paged keep: lengths must not be where the paths or their lengths are");
         begin(st);
         tq::launch_paged_keep({b_, path, kept, lengths, n, width, heads_, static_cast<int>(layers_.size()), plan_, d_status_, sms_}, dim_, st);
         plan_.n = -1;

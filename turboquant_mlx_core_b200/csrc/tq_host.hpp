@@ -56,6 +56,12 @@ inline bool is_device_pointer(const void* p) {
     return attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged;
 }
 
+// True when two ranges have no byte in common.
+inline bool ranges_apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return !a || !b || x + a_bytes <= y || y + b_bytes <= x;
+}
+
 // For page-locked host memory (cudaHostAlloc / cudaHostRegister, mapped as usual under unified
 // addressing) returns the address a kernel can use for it, else NULL.
 inline void* pinned_host_device_alias(const void* p) {

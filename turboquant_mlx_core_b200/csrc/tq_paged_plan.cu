@@ -390,11 +390,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_keep_plan_kernel(PagedKeep
         sums[0] += (held[k] + P - 1) / P - (keep[k] + P - 1) / P;
     }
     if (!other && !refused) {
-        for (long t = tid; t < static_cast<long>(n) * a.width; t += kPlanThreads) {
-            const int i = static_cast<int>(t / a.width), k = static_cast<int>(t - static_cast<long>(i) * a.width), kept = a.kept[i];
+        const int width = min(a.width, max(1, a.sizes.most));   // (no path is longer)
+        for (long t = tid; t < static_cast<long>(n) * width; t += kPlanThreads) {
+            const int i = static_cast<int>(t / width), k = static_cast<int>(t - static_cast<long>(i) * width), kept = a.kept[i];
             if (k >= kept) continue;
-            const int token = a.path[t], count = a.b.starts[i + 1] - a.b.starts[i];
-            if (token < 0 || token >= count || (k > 0 && a.path[t - 1] >= token)) atomicMax(&s_error, static_cast<unsigned int>(kPagedBadPath));
+            const int* const at = a.path + static_cast<long>(i) * a.width + k;
+            const int token = *at, count = a.b.starts[i + 1] - a.b.starts[i];
+            if (token < 0 || token >= count || (k > 0 && at[-1] >= token)) atomicMax(&s_error, static_cast<unsigned int>(kPagedBadPath));
         }
     }
     block_sums(sums, all);   // (its barriers publish s_error)
@@ -425,8 +427,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_keep_plan_kernel(PagedKeep
         }
     }
     if (t0 == 0) {
-        if (other) raise_status(a.status, kPagedOtherPlan);
-        else {
+        if (other) {
+            if (header.state == kPagedKept) a.b.header->state = kPagedPlain;   // (a replay behind another call: nothing to move again)
+            raise_status(a.status, kPagedOtherPlan);
+        } else {
             *a.b.header = {free_before + pages, 0, 0, 0, {-1, 0, 0}, ok ? kPagedKept : kPagedPlain};
             if (s_error != kPagedOk) raise_status(a.status, s_error);
         }
