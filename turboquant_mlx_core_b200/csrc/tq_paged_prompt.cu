@@ -142,6 +142,15 @@ __device__ __forceinline__ long long request_tiles(const PagedAttnArgs& a, const
     return sum;
 }
 
+// Of numbers that are not negative.  TREE: where 32 bits hold both the division is a quarter as long, and four of them are in front of a CTA's first
+// product (a tree of 8 nodes over 4096 tokens: 20.7 us, 19.0 with this and what else comes sooner below).  In a prompt of 4096 tokens the same
+// changes take 4 us more of 171 than they save, by where they put the other warps' code.
+template <bool TREE>
+__device__ __forceinline__ long long quotient(long long x, long long by) {
+    if constexpr (!TREE) return x / by;
+    return (x | by) >> 32 ? x / by : static_cast<long long>(static_cast<unsigned int>(x) / static_cast<unsigned int>(by));
+}
+
 // A CTA's share of the units: (request, KV head, pair, tile), the tile running fastest.
 template <bool TREE>
 struct Walker {
@@ -162,7 +171,7 @@ struct Walker {
             left = 0;
             return;
         }
-        head = static_cast<int>(skip / sum);
+        head = static_cast<int>(quotient<TREE>(skip, sum));
         skip -= head * sum;
         for (int base = 0;; base += 32) {   // the pair in which the rest lies
             int l = 0, h = 0;
@@ -254,20 +263,26 @@ __device__ __noinline__ uint64_t seen_nodes(const PagedAttnArgs& a, const Segmen
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
         const int token = tb + 32 * h + lane;
+        const bool there = token >= at.first && token < at.held;
         int lo = static_cast<int>(0x80000000u), place = 0;   // (no number is in there)
         unsigned int span = 0;
-        if (token >= at.first && token < at.held) {
+        if (there) {
             const PagedNode node = a.b.nodes[at.start + token - at.first];
             lo = node.pre;
             span = static_cast<unsigned int>(node.last - node.pre);
             place = at.first + node.depth;
         }
+        const uint32_t some = __ballot_sync(0xffffffffu, there);
         uint32_t bits = 0;
-#pragma unroll 8
-        for (int e = 0; e < 32; ++e) {
-            const int lo_e = __shfl_sync(0xffffffffu, lo, e), place_e = __shfl_sync(0xffffffffu, place, e);
-            const unsigned int span_e = __shfl_sync(0xffffffffu, span, e);
-            if (static_cast<unsigned int>(number - lo_e) <= span_e && (a.window <= 0 || place_e > pos - a.window)) bits |= 1u << e;
+#pragma unroll 1
+        for (int e0 = 0; e0 < 32; e0 += 4) {   // (most tiles hold few new tokens, or none)
+            if (!(some >> e0 & 0xfu)) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = e0 + k, lo_e = __shfl_sync(0xffffffffu, lo, e), place_e = __shfl_sync(0xffffffffu, place, e);
+                const unsigned int span_e = __shfl_sync(0xffffffffu, span, e);
+                if (static_cast<unsigned int>(number - lo_e) <= span_e && (a.window <= 0 || place_e > pos - a.window)) bits |= 1u << e;
+            }
         }
         seen |= static_cast<uint64_t>(bits) << (32 * h);
     }
@@ -311,11 +326,14 @@ __device__ __forceinline__ void add_second(uint32_t (&x)[32], uint32_t taddr, fl
 // TREE: trees of drafts (paged_tree_kernel in tq_paged_plan.cu numbers the nodes): a row sees the tokens in front of the new ones, its ancestors and
 // itself.  A request has some tens to some hundreds of rows there, so that many items have no second row tile; its warps then take every second
 // tile of the cache for the first one's rows, with a maximum, a sum and an O of their own, and the two are added up at the item's end (both read the
-// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 64 thousand tokens of 4 heads: 48 us; a team's step takes 2.8 thousand
-// cycles there, 0.9 of which it waits for scores, whose keys' conversion takes 3.4 for every second tile.  Tried beside it, in the same case: the
+// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 64 thousand tokens of 4 heads: 44 us, 10 of which are one CTA's way to its
+// first product and from its last one to the result.  Over a long cache a tile takes 1.9 thousand cycles with 25 rows as with 125, and 2.7 with two
+// row tiles: for few rows the keys bound it, whose warps' way from one of their tiles to the next (every second one) is 3.7 thousand cycles: 0.5 for
+// the bytes, 1.7 to make them halves, 1.1 to find the next, each instruction behind some 13 cycles of others.  Tried beside it: the
 // products turned around (tokens as their 128 rows, query rows as 32, 64 or 128 columns, a softmax thread per token), which takes a tile's products as
 // long as there are rows: 90 us, since each thread then keeps a sum for every row and four warps have to agree on every reference; keys and values
-// from memory through registers to their place, without the bytes in shared memory: 58, with 24 words spilled.
+// from memory through registers to their place, without the bytes in shared memory, and four threads that issue products: 50; the bytes of two tiles
+// on their way, with three stages of halves instead of four: 46, but a fifteenth less where a request has 16 rows.
 template <int D, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_constant__ PagedAttnArgs a) {
     using S = Shape<D>;
@@ -360,6 +378,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    auto allocate = [&]() {
+        if (warp != kMmaWarp) return;
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(kTmemAll) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        fence_before();
+    };
+    if constexpr (TREE) allocate();
     pdl_wait_release();
     int n = planned(a.b.header, a.sizes, a.status).requests;
     if constexpr (TREE) {
@@ -377,18 +402,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         if (lane == 0) s_sum[warp] = mine;
     }
     __syncthreads();
-    long long total = 0;
+    static_assert(kWarps == 32, "a lane for each warp's units");
+    long long total = 0, upto = 0;   // (TREE) units of the warps up to the lane's
+    if constexpr (TREE) {
+        upto = s_sum[lane];
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) total += s_sum[k];
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) total += s_sum[k];
+    }
     const long long ctas = min(static_cast<long long>(gridDim.x), total), c = blockIdx.x;
     if (tid == 0) a.joins[c].last = 0;
-    if (c >= ctas) return;
-    if (warp == kMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(kTmemAll) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-        fence_before();
+    if (c >= ctas) {
+        if (TREE && warp == kMmaWarp) {
+            fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(kTmemAll) : "memory");
+        }
+        return;
     }
-    __syncthreads();
+    if constexpr (!TREE) allocate();
+    __syncthreads();   // (TREE: every warp has read the sums, in whose place the second team's will be)
     fence_after();
     const uint32_t tmem = s_tmem;
     const uint32_t base = smem_addr(s_mem);
@@ -585,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         const float inv = unit / l;
                         __half* const dst = a.out + token * a.out_stride + static_cast<long>(hq) * D;
 #pragma unroll 1
-                        for (int q = 0; q < D / 32; ++q) {
+                        for (int q = 0; q < (TREE && idle ? 0 : D / 32); ++q) {
                             tmem_ld(t_o + 32 * q, x);
                             tmem_ld_wait(x);
                             if constexpr (TREE) {
@@ -606,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         float* const part = a.partial + (2 * c + (begins ? 1 : 0)) * static_cast<long>(S::kPart);
                         const int pr = t * kRows + r_in;
 #pragma unroll 1
-                        for (int q = 0; q < D / 32; ++q) {
+                        for (int q = 0; q < (TREE && idle ? 0 : D / 32); ++q) {
                             tmem_ld(t_o + 32 * q, x);
                             tmem_ld_wait(x);
                             if constexpr (TREE) {
@@ -738,11 +776,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             }
         }
         if (warp == kScheduleWarp) {
-            const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
+            const long long u0 = quotient<TREE>(total * c, ctas), u1 = quotient<TREE>(total * (c + 1), ctas);
             Walker<TREE> at;
             long long front = 0;
             int w = 0;
-            while (w + 1 < kWarps && front + s_sum[w] <= u0) front += s_sum[w++];
+            if constexpr (TREE) {
+                w = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, upto > u0))) - 1;   // (u0 is below the total)
+                if (w > 0) front = __shfl_sync(0xffffffffu, upto, w - 1);
+            } else {
+                while (w + 1 < kWarps && front + s_sum[w] <= u0) front += s_sum[w++];
+            }
             at.place(a, w * per, n, u0 - front, u1 - u0, lane);
             bool more = at.left > at.before;
             do {
@@ -752,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     // the CTA that holds the item's last unit: the largest c' with total * c' / ctas <= that unit
                     const long long last_unit = u1 - at.left + at.before + (at.hi - at.tile) - 1;
                     s_seg[seg_n % kSegments] = {at.r.row, at.r.start, at.r.first(), at.r.held, at.r.rows, at.pair * kPairRows, at.head, at.tile, tiles, at.tile == at.lo,
-                                                at.tile + tiles == at.hi, static_cast<int>(((last_unit + 1) * ctas - 1) / total)};
+                                                at.tile + tiles == at.hi, static_cast<int>(quotient<TREE>((last_unit + 1) * ctas - 1, total))};
                     bar_arrive(bar(s_bar.seg_full[seg_n % kSegments]));
                 }
                 __syncwarp();
