@@ -932,8 +932,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             publish_smem();
             __syncwarp();
             if (lane == 0) bar_arrive(keys ? bar(s_bar.k_full[stage]) : bar(s_bar.v_full[stage]));
-            step(now);
-            if (now.tiles > 0) step(now);
+            if (TREE && now.j + 2 < now.tiles) {   // (in the same segment, as nearly always)
+                now.n += 2;
+                now.j += 2;
+            } else {
+                step(now);
+                if (now.tiles > 0) step(now);
+            }
             if (now.tiles > 0) fetch(now);
             for (; left < now.seg; ++left)
                 if (lane == 0) bar_arrive(bar(s_bar.seg_empty[left % kSegments]));
