@@ -144,8 +144,9 @@ __device__ __forceinline__ void store_head(__half* p, const uint4& v) {
 template <bool WIDE>
 __global__ void __launch_bounds__(512) qk_norm_rope_kernel(const __grid_constant__ QkNormArgs a) {
     ops_dependency_sync();
-    extern __shared__ __align__(16) float2 s_turn[];   // [rows of the CTA][dim / 2] cosine, sine
-    const int half = a.dim >> 1, all = (a.heads[0] + a.heads[1]) * a.lanes, rows_cta = a.beside * a.rows_each;
+    // [rows of the CTA][4][dim / 16][2] cosine, sine: two of a thread's pairs next to those of the next thread, which reads them beside it
+    extern __shared__ __align__(16) float2 s_turn[];
+    const int half = a.dim >> 1, chunks = a.dim >> 4, all = (a.heads[0] + a.heads[1]) * a.lanes, rows_cta = a.beside * a.rows_each;
     const long row0 = static_cast<long>(blockIdx.x) * rows_cta;
     const int rows = static_cast<int>(min(static_cast<long>(rows_cta), a.rows - row0));
     const int mine = a.beside > 1 ? static_cast<int>(threadIdx.x) / a.width : 0, place = static_cast<int>(threadIdx.x) - mine * a.width;
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(512) qk_norm_rope_kernel(const __grid_constant
                 const float angle = static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f;   // half turns, -1 .. 1
                 float s, c;
                 sincospif(angle, &s, &c);
-                s_turn[k] = make_float2(c, s);
+                s_turn[r * half + ((p >> 1 & 3) * chunks + (p >> 3)) * 2 + (p & 1)] = make_float2(c, s);
             }
             __syncthreads();
         }
@@ -196,10 +197,10 @@ __global__ void __launch_bounds__(512) qk_norm_rope_kernel(const __grid_constant
             for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (!live || r >= rows) continue;
             const float scale = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
-            const float4* const turn = reinterpret_cast<const float4*>(s_turn + r * half + t);
+            const float4* const turn = reinterpret_cast<const float4*>(s_turn + r * half) + (t >> 3);
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const float4 two = turn[j >> 1];
+                const float4 two = turn[(j >> 1) * chunks];
                 const float p0 = u[j] * scale * g[j], q0 = v[j] * scale * k[j], p1 = u[j + 1] * scale * g[j + 1], q1 = v[j + 1] * scale * k[j + 1];
                 u[j] = p0 * two.x - q0 * two.y;
                 v[j] = q0 * two.x + p0 * two.y;
