@@ -102,8 +102,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(__half* __restr
 // in several rows, so that it keeps the weights and finds its place once; `lanes` threads, the next power of two above D / 16, share a head and its sum
 // of squares.  It is bound by memory, 16 bytes in and out for eight elements (few rows: by latency, 2.6 us): a row's values are asked for while the one
 // before is at work, the first one's in front of the sines and cosines, which D / 2 threads take for all heads of a row.  8192 rows of 40 + 8 heads of
-// 128: 44.6 us, 4.5 TB/s, 69 % of a plain copy's rate (52 with a row to a CTA, whose threads find head and pair anew for each 64 bytes; 44.8 with three
-// CTAs to an SM instead of two, in 56 registers): some 200 instructions for 64 bytes are what is left beside memory.
+// 128: 36.5 us, 5.5 TB/s, 84 % of a plain copy's rate (52 with a row to a CTA, whose threads find head and pair anew for each 64 bytes; 44.6 with sines
+// and cosines in the pairs' order, where four threads of eight read the same banks; 41.5 in 75 registers, of which two CTAs of 384 threads fill an SM
+// instead of three, though heads of 64, 16 + 4 of them, take 10.4 with those and 11.3 with these).
 constexpr int kHeadHalfMax = 256;
 struct QkNormArgs {
     const __half* x[2];       // queries, keys
@@ -142,7 +143,7 @@ __device__ __forceinline__ void store_head(__half* p, const uint4& v) {
     }
 }
 template <bool WIDE>
-__global__ void __launch_bounds__(512) qk_norm_rope_kernel(const __grid_constant__ QkNormArgs a) {
+__global__ void __maxnreg__(56) qk_norm_rope_kernel(const __grid_constant__ QkNormArgs a) {
     ops_dependency_sync();
     // [rows of the CTA][4][dim / 16][2] cosine, sine: two of a thread's pairs next to those of the next thread, which reads them beside it
     extern __shared__ __align__(16) float2 s_turn[];
