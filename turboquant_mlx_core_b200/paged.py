@@ -335,26 +335,34 @@ def verify_drafts(starts, parents, tokens, target, draft, uniforms, path, kept, 
     `PagedKVCache.keep` takes, and the tokens that follow."""
     _load_torch()
     on = _device_of(starts, "starts")
-    if len(path.shape) != 2 or _number(starts, "starts") != path.shape[0] + 1:
-        raise ValueError("verify_drafts: path must be [n, width], starts [n + 1]")
-    (n, width), rows = path.shape, _number(tokens, "tokens")
-    at = []
-    for x, what in ((target, "target"), (draft, "draft")):
-        if x is None:
-            at += [None, 0]
-            continue
-        if x.shape != target.shape or len(x.shape) != 2 or x.shape[0] != rows or (x.shape[1] > 1 and x.stride(1) != 1):
-            raise ValueError(f"{what} must be [{rows}, vocab] with contiguous rows")
-        if x.dtype is not target.dtype:
-            raise ValueError("target and draft must have the same type")
-        if _device_of(x, what) != on:
-            raise ValueError(f"{what} is on another device than starts")
-        at += [x.data_ptr(), x.stride(0) if rows > 1 else max(x.stride(0), x.shape[1])]
-    if uniforms.dtype is not _float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous():
+    try:
+        n, width = path.shape
+        rows, vocab = target.shape
+        step, one = target.stride()
+    except ValueError:
+        raise ValueError("path must be [n, width], target [rows, vocab]") from None
+    if _device_of(target, "target") != on:
+        raise ValueError("target is on another device than starts")
+    dp, drafted = None, 0
+    if draft is not None:
+        if draft.shape != target.shape or draft.dtype is not target.dtype:
+            raise ValueError("target and draft must have the same shape and type")
+        if _device_of(draft, "draft") != on:
+            raise ValueError("draft is on another device than starts")
+        drafted, other = draft.stride()
+        if other != 1:
+            one = other
+        dp = draft.data_ptr()
+    if one != 1 and vocab > 1:
+        raise ValueError("rows of target and draft must be contiguous")
+    if rows <= 1:      # (a stride that is not used may be anything)
+        step, drafted = max(step, vocab), max(drafted, vocab)
+    if uniforms.dtype is not _float32 or uniforms.numel() != rows or not uniforms.is_contiguous():
         raise ValueError(f"uniforms must be contiguous float32 [{rows}]")
     if _device_of(uniforms, "uniforms") != on:
         raise ValueError("uniforms are on another device than starts")
-    if _lib.load().tq_verify_drafts(_ints(starts, "starts", n + 1, on), _ints(parents, "parents", rows, on), _ints(tokens, "tokens", rows, on), n, rows, at[0], at[2],
-                                    _tag(target, "verify_drafts"), _fits(target.shape[1], "vocab"), at[1], at[3], uniforms.data_ptr(), _ints(path, "path", n * width, on),
-                                    width, _ints(kept, "kept", n, on), _ints(next, "next", n, on), None if stream is None else _stream_ptr(stream)):
+    if _lib.load().tq_verify_drafts(_ints(starts, "starts", n + 1, on), _ints(parents, "parents", rows, on), _ints(tokens, "tokens", rows, on), n, rows, target.data_ptr(),
+                                    dp, TQ_F32 if target.dtype is _float32 else _tag(target, "verify_drafts"), _fits(vocab, "vocab"), step, drafted, uniforms.data_ptr(),
+                                    _ints(path, "path", n * width, on), width, _ints(kept, "kept", n, on), _ints(next, "next", n, on),
+                                    None if stream is None else _stream_ptr(stream)):
         check(-1, "verify_drafts")
