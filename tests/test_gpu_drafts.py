@@ -286,3 +286,21 @@ def test_results_where_arguments_are(tq):
     for change in ({"next": drafted[3:5]}, {"kept": starts[1:]}, {"next": out["kept"]}, {"kept": out["path"].view(-1)[6:]}, {"path": uniforms.view(torch.int32)[:8].view(2, 4)}):
         with pytest.raises(tq.TQError, match="must not be where"):
             tq.verify_drafts(starts, ints(np.concatenate(parents)), drafted, on_device(target), on_device(draft), uniforms, **{**out, **change})
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_as_many_requests_as_there_may_be(tq, drawn):
+    """65536 requests of one to three nodes: more clusters than the device holds at once, in any order."""
+    rng = np.random.default_rng(13)
+    distinct = 512
+    counts = rng.integers(1, 4, distinct).tolist()
+    parents, tokens, target, draft, u = batch(rng, counts, 9, 2, drawn)
+    starts, times = np.concatenate([[0], np.cumsum(counts)]), 65536 // distinct
+    rows, out = int(starts[-1]), outputs(65536, 3)
+    many = ints(np.concatenate([starts[:-1] + k * rows for k in range(times)] + [[times * rows]]))
+    again = lambda x: None if x is None else torch.from_numpy(np.concatenate([x] * times)).cuda()      # noqa: E731
+    tq.verify_drafts(many, again(np.concatenate([np.asarray(p, np.int32) for p in parents])), again(tokens), again(target), again(draft), again(u), **out)
+    torch.cuda.synchronize()
+    want = [drafts_model.verify(parents[i], tokens[s:e], target[s:e], None if draft is None else draft[s:e], u[s:e], 3) for i, (s, e) in enumerate(zip(starts, starts[1:]))]
+    assert out["kept"].tolist() == [len(p) for p, _ in want] * times and out["next"].tolist() == [t for _, t in want] * times
+    assert out["path"].tolist() == [p + [-1] * (3 - len(p)) for p, _ in want] * times

@@ -301,3 +301,27 @@ def test_captured_and_replayed_on_new_trees(tq):
         compare(out, lse, tree_attention_model.attention(b.m, x, b.parents))
     b.c.check_status()
     b.c.close()
+
+
+def test_two_caches_on_two_streams(tq):
+    """Calls of two caches at once, several of each behind one another: each has the result that it has alone."""
+    rng = np.random.default_rng(12)
+    batches = [Batch(tq, rng, 2, 128, 64, [700, 130, 5], [12, 40, 3], 3), Batch(tq, rng, 4, 64, 16, [90] * 9, [7] * 9, 2)]
+    qs = [torch.from_numpy(queries(rng, b.tokens, g, b.m.dim)).cuda() for b, g in zip(batches, (8, 4))]
+    alone = [b.run(q) for b, q in zip(batches, qs)]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        outs = []
+        for b, q, stream in zip(batches, qs, streams):
+            with torch.cuda.stream(stream):
+                out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device="cuda")
+                for _ in range(3):
+                    b.c.tree_attention(0, q, out=out, lse=lse, stream=stream)
+                outs.append((out, lse))
+        torch.cuda.synchronize()
+        for (out, lse), (want, sums) in zip(outs, alone):
+            assert torch.equal(out, want) and torch.equal(lse, sums)
+    for b in batches:
+        b.c.check_status()
+        b.c.close()

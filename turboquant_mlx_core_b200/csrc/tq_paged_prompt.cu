@@ -384,6 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         fence_before();
     };
+    // (in front of the wait for the kernel before: nobody beside this CTA can be in want of tensor memory meanwhile, since its threads have all of the
+    // SM's registers)
+    static_assert(kThreads * 64 == 65536);
     if constexpr (TREE) allocate();
     pdl_wait_release();
     int n = planned(a.b.header, a.sizes, a.status).requests;
