@@ -610,8 +610,9 @@ int tq_paged_truncate(tq_paged_cache_t cache, const int* rows, const int* length
 int tq_paged_tree(tq_paged_cache_t cache, const int* parents, int tokens, int* positions, void* stream);
 /** Of request i's new tokens the kept[i] ones path[i, 0 .. ] stay, ascending (as tq_verify_drafts gives them), all of them where kept[i] is below
  *  0.  In all layers they move up to the places of the first new ones, and the pages behind become free.  A token that stays in its page keeps
- *  its numbers; one that joins another page joins it as an append of its values would, and where the page's scale grows all that the page holds is
- *  rounded once more.  path [n, width], kept [n] and lengths [n] (may be NULL; the tokens that each request holds then) are device memory, n is
+ *  its numbers; one that joins another page joins it as an append of its values behind the page's tokens would, those that do not stay among them: the
+ *  page's scale, which they may have raised, grows where it must and all that the page holds is rounded once more then.  A page that is not a
+ *  number (an infinity or a NaN came to it) and of whose tokens none stays is as if it were new.  path [n, width], kept [n] and lengths [n] (may be NULL; the tokens that each request holds then) are device memory, n is
  *  the plan's; lengths must not be where the other two are.  A path that is none changes nothing (tq_paged_status tells).  Ends the plan in force. */
 int tq_paged_keep(tq_paged_cache_t cache, const int* path, int width, const int* kept, int n, int* lengths, void* stream);
 /** Keys and values [tokens, heads, head_dim] of the planned tokens (TQ_F32 or TQ_F16), token t at t * stride elements (heads * head_dim

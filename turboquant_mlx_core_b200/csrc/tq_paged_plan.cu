@@ -683,7 +683,11 @@ __global__ void __launch_bounds__(128) paged_keep_kernel(PagedKeepArgs a) {
             }
             if (near < upto) {   // from others
                 unsigned int* const scale_at = scale_of(page);
-                const unsigned int held = *scale_at;
+                // A page that is not a number, and of whose tokens none stays, is those that join it, as for an append at its first place: what made it so were
+                // drafts that nobody keeps.  (A scale that is a number stays, whoever made it so large.)
+                const unsigned int stored = *scale_at;
+                const bool empty = stored >= 0x7f800000u && near == k && (first + k) % P == 0;
+                const unsigned int held = empty ? 0u : stored;
                 unsigned int top = 0u;
                 for (int base = near; base < upto; base += kTokens) {
                     const int t = base + r;
@@ -703,7 +707,7 @@ __global__ void __launch_bounds__(128) paged_keep_kernel(PagedKeepArgs a) {
                 top = __reduce_max_sync(0xffffffffu, top);
                 const unsigned int scale = max(scale_bits(top), held);   // (as bits: NaN is above the finite ones, and stays)
                 const bool finite = scale < 0x7f800000u;
-                if (finite && scale != held) {
+                if (finite && scale != held && !empty) {
                     const float ratio = scale_ratio(held, scale);
                     for (int t = r; t < P; t += kTokens) *chunk(codes, t) = rescaled16(*chunk(codes, t), ratio);
                 }
