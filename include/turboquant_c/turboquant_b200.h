@@ -597,7 +597,8 @@ void tq_paged_cache_free(tq_paged_cache_t cache);
  *    positions [tokens]  its position in the request (as tq_rope_f16 takes them), 0 behind the last
  *    tables    [n, tables_width]  the requests' pages, -1 behind the last (and cut to the width)
  *  A batch that does not fit (a bad row or count, a row of the tables or the free pages used up) changes nothing: its starts are 0,
- *  its slots -1, the step's appends and attentions do nothing, and tq_paged_status tells. */
+ *  its slots -1, its lengths and tables those that the requests have (none in a row outside the tables), the step's appends and attentions do
+ *  nothing, and tq_paged_status tells. */
 int tq_paged_plan(tq_paged_cache_t cache, const int* rows, const int* counts, int n, int tokens, int max_count, int* starts, int* lengths,
                   int* slots, int* positions, int* tables, int tables_width, void* stream);
 /** The request in row rows[i] keeps its first lengths[i] tokens (0: it is gone); its other pages become free, to be taken in the same order
@@ -612,8 +613,9 @@ int tq_paged_tree(tq_paged_cache_t cache, const int* parents, int tokens, int* p
  *  0.  In all layers they move up to the places of the first new ones, and the pages behind become free.  A token that stays in its page keeps
  *  its numbers; one that joins another page joins it as an append of its values behind the page's tokens would, those that do not stay among them: the
  *  page's scale, which they may have raised, grows where it must and all that the page holds is rounded once more then.  A page that is not a
- *  number (an infinity or a NaN came to it) and of whose tokens none stays is as if it were new.  path [n, width], kept [n] and lengths [n] (may be NULL; the tokens that each request holds then) are device memory, n is
- *  the plan's; lengths must not be where the other two are.  A path that is none changes nothing (tq_paged_status tells).  Ends the plan in force. */
+ *  number (an infinity or a NaN came to it) and of whose tokens none stays is as if it were new.  path [n, width], kept [n] and lengths [n] (may be
+ *  NULL; the tokens that each request holds then, behind a plan that was refused too) are device memory, n is the plan's; lengths must not be
+ *  where the other two are.  A path that is none changes nothing (tq_paged_status tells).  Ends the plan in force. */
 int tq_paged_keep(tq_paged_cache_t cache, const int* path, int width, const int* kept, int n, int* lengths, void* stream);
 /** Keys and values [tokens, heads, head_dim] of the planned tokens (TQ_F32 or TQ_F16), token t at t * stride elements (heads * head_dim
  *  or more: a slice of a fused projection's result), into a layer.  `tokens` is the plan's; rows behind the last request's are not read.

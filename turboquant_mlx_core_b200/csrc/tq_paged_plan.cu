@@ -114,15 +114,18 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         row[k] = a.rows ? a.rows[i0 + k] : i0 + k;
         count[k] = a.counts[i0 + k];
         unsigned int bad = kPagedOk;
-        if (row[k] < 0 || row[k] >= a.b.max_requests || seen_before(s_seen, row[k])) bad = kPagedBadRow;
-        else if (count[k] < 0 || count[k] > a.max_count) bad = kPagedBadCount;
-        else {
-            old[k] = a.b.lengths[row[k]];
-            if (static_cast<long long>(old[k]) + count[k] > static_cast<long long>(a.b.max_pages) * P) bad = kPagedLongRequest;
+        if (row[k] < 0 || row[k] >= a.b.max_requests) {
+            bad = kPagedBadRow;
+            row[k] = 0;   // (nothing below goes by what it names)
+        } else {
+            old[k] = a.b.lengths[row[k]];   // (of a batch that is refused, too: its lengths are told)
+            if (seen_before(s_seen, row[k])) bad = kPagedBadRow;
+            else if (count[k] < 0 || count[k] > a.max_count) bad = kPagedBadCount;
+            else if (static_cast<long long>(old[k]) + count[k] > static_cast<long long>(a.b.max_pages) * P) bad = kPagedLongRequest;
         }
         if (bad != kPagedOk) {
             atomicMax(&s_error, bad);
-            row[k] = old[k] = count[k] = 0;   // (nothing below goes by what it names)
+            count[k] = 0;
             continue;
         }
         const int now = old[k] + count[k];
