@@ -75,11 +75,11 @@ int tq_verify_drafts(const int* starts, const int* parents, const int* tokens, i
             TQ_REQUIRE(rows == 0 || is_device_pointer(p), "verify drafts: arguments must be device pointers");
         TQ_REQUIRE(rows == 0 || !draft || is_device_pointer(draft), "verify drafts: arguments must be device pointers");
         // (the CTAs of a request read what they decide by in their own time, and must all see the same)
-        const struct { const void* p; size_t bytes; } all[] = {{path, 4ul * n * width}, {kept, 4ul * n}, {next, 4ul * n}, {starts, 4ul * n + 4}, {parents, 4ul * rows},
-                                                               {tokens, 4ul * rows}, {uniforms, 4ul * rows}};
+        const size_t es = dtype == TQ_F16 ? 2 : 4;
+        const ByteRows all[] = {{path, 4ul * n * width}, {kept, 4ul * n}, {next, 4ul * n}, {starts, 4ul * n + 4}, {parents, 4ul * rows}, {tokens, 4ul * rows},
+                                {uniforms, 4ul * rows}, {target, vocab * es, rows, target_stride * es}, {draft, vocab * es, draft ? rows : 0, draft_stride * es}};
         for (int i = 0; i < 3; ++i)
-            for (int j = i + 1; j < 7; ++j)
-                TQ_REQUIRE(ranges_apart(all[i].p, all[i].bytes, all[j].p, all[j].bytes), "verify drafts: results must not be where an argument or another result is");
+            for (int j = i + 1; j < 9; ++j) TQ_REQUIRE(rows_apart(all[i], all[j]), "verify drafts: results must not be where an argument or another result is");
         const OnDevice on(starts);
         launch_verify_drafts({starts, parents, tokens, target, draft, uniforms, target_stride, draft ? draft_stride : 0, rows, vocab, width, 0, path, kept, next}, n,
                              dtype == TQ_F16, static_cast<cudaStream_t>(stream));

@@ -61,6 +61,24 @@ inline bool ranges_apart(const void* a, size_t a_bytes, const void* b, size_t b_
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return !a || !b || x + a_bytes <= y || y + b_bytes <= x;
 }
+// Rows of `width` bytes, `stride` bytes apart.
+struct ByteRows {
+    const void* p;
+    size_t width;
+    long rows = 1;
+    size_t stride = 0;
+};
+// True when two of them have no byte in common; what lies between rows is no part of them.  Several rows of different strides count as in each
+// other's way where their ranges meet.
+inline bool rows_apart(const ByteRows& a, const ByteRows& b) {
+    if (a.rows <= 0 || b.rows <= 0) return true;
+    if (ranges_apart(a.p, (a.rows - 1) * a.stride + a.width, b.p, (b.rows - 1) * b.stride + b.width)) return true;
+    if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.stride != b.stride)) return false;
+    const size_t stride = a.rows > 1 ? a.stride : b.stride;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    const size_t behind = y >= x ? (y - x) % stride : (stride - (x - y) % stride) % stride;   // of a's rows b's begin
+    return behind >= a.width && behind + b.width <= stride;
+}
 
 // For page-locked host memory (cudaHostAlloc / cudaHostRegister, mapped as usual under unified
 // addressing) returns the address a kernel can use for it, else NULL.
