@@ -31,3 +31,41 @@ def test_results_of_a_verification_over_the_rows(tq, dtype):
         tq.verify_drafts(*args, *rows, uniforms, **out)
         assert out["next"].tolist() == [t for _, t in want] and out["path"].tolist() == [p + [-1] * (2 - len(p)) for p, _ in want]
         assert torch.equal(rows[which].cpu(), torch.from_numpy((target, draft)[which]))
+
+
+def test_results_of_norms_over_their_arguments(tq):
+    rows, heads, kv, dim = 33, 4, 2, 64
+    step = (heads + 2 * kv) * dim
+    block = torch.randn((rows + 1, step), device="cuda").half()
+    flat, before = block.view(-1), block.clone()
+    slot = lambda at, n, stride=step: flat[at:].as_strided((rows, n, dim), (stride, dim, 1))      # noqa: E731
+    q, k = slot(0, heads), slot(heads * dim, kv)
+    w, positions = torch.ones((2, dim), device="cuda").half(), torch.arange(rows, dtype=torch.int32, device="cuda")
+    apart = lambda n: torch.empty((rows, n, dim), dtype=torch.float16, device="cuda")      # noqa: E731
+    many = torch.zeros(rows * heads * dim + 8, dtype=torch.float16, device="cuda")
+    inside = many.view(torch.int32)[3:3 + rows]
+    cases = [((slot(0, heads, heads * dim), apart(kv)), {}), ((slot(step, heads), apart(kv)), {}),       # packed in place; a row further
+             ((slot(dim, heads), apart(kv)), {}), ((slot(heads * dim, heads), apart(kv)), {}),           # a head further; over the keys
+             ((apart(heads), slot(0, kv)), {}), ((apart(heads), slot(heads * dim - dim, kv)), {}),       # the keys' over the queries, wholly and by a head
+             ((slot((heads + kv) * dim - dim, kv + 1), apart(kv)), {"queries": apart(kv + 1)}),
+             ((slot(0, heads), slot(2 * dim, kv)), {}),
+             ((many[:rows * heads * dim].view(rows, heads, dim), apart(kv)), {"positions": inside}),
+             ((many[:rows * heads * dim].view(rows, heads, dim), apart(kv)), {"query_weight": many[100 * 8:][:dim]}),
+             ((apart(heads), many[:rows * kv * dim].view(rows, kv, dim)), {"key_weight": many[:dim]}),
+             ((many[:rows * heads * dim].view(rows, heads, dim), many[8:8 + rows * kv * dim].view(rows, kv, dim)), {})]
+    for out, change in cases:
+        args = {"queries": q, "keys": k, "query_weight": w[0], "key_weight": w[1], "positions": positions, **change}
+        with pytest.raises(tq.TQError, match="must (not )?be"):
+            tq.qk_norm_rope(**args, out=out)
+    assert torch.equal(block, before)
+    want = tq.qk_norm_rope(q, k, *w, positions, out=(apart(heads), apart(kv)))
+    # another slot of the same rows, then in place
+    tq.qk_norm_rope(q, k, *w, positions, out=(apart(heads), slot((heads + kv) * dim, kv)))
+    assert torch.equal(slot((heads + kv) * dim, kv), want[1])
+    tq.qk_norm_rope(q, k, *w, positions)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    # one row has no stride
+    q1, k1 = slot(0, heads)[:1].clone(), slot(heads * dim, kv)[:1].clone()
+    want = tq.qk_norm_rope(q1, k1, *w, positions[:1], out=(torch.empty_like(q1), torch.empty_like(k1)))
+    tq.qk_norm_rope(q1, k1, *w, positions[:1], out=(q1.as_strided((1, heads, dim), (5 * step, dim, 1)), k1))
+    assert torch.equal(q1, want[0]) and torch.equal(k1, want[1])

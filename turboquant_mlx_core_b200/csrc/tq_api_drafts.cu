@@ -51,6 +51,15 @@ int tq_qk_norm_rope_f16(const void* q_fp16, const void* k_fp16, const void* q_we
         for (const void* p : {q_fp16, k_fp16, q_weight_fp16, k_weight_fp16, static_cast<const void*>(positions), static_cast<const void*>(q_out_fp16),
                               static_cast<const void*>(k_out_fp16)})
             TQ_REQUIRE(is_device_pointer(p), "qk norm: arguments must be device pointers");
+        // (in place each thread writes what it alone has read; anywhere else over an argument another CTA may not have read it yet)
+        const ByteRows in[] = {{q_fp16, 2ul * q_row, rows, 2ul * q_stride}, {k_fp16, 2ul * k_row, rows, 2ul * k_stride}, {q_weight_fp16, 2ul * head_dim},
+                               {k_weight_fp16, 2ul * head_dim}, {positions, 4ul * rows}};
+        const ByteRows out[] = {{q_out_fp16, 2ul * q_row, rows, 2ul * q_out_stride}, {k_out_fp16, 2ul * k_row, rows, 2ul * k_out_stride}};
+        for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < 5; ++j)
+                TQ_REQUIRE((i == j && out[i].p == in[j].p && (rows == 1 || out[i].stride == in[j].stride)) || rows_apart(out[i], in[j]),
+                           "qk norm: results must be where their rows are, with the same stride, or not where an argument is");
+        TQ_REQUIRE(rows_apart(out[0], out[1]), "qk norm: the two results must not be in the same place");
         const OnDevice on(q_fp16);
         const auto half = [](const void* p) { return static_cast<const __half*>(p); };
         launch_qk_norm_rope_f16(half(q_fp16), half(k_fp16), half(q_weight_fp16), half(k_weight_fp16), positions, rows, q_heads, kv_heads, head_dim, q_stride,

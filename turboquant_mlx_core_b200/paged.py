@@ -298,8 +298,8 @@ def _device_of(x, what):
 
 def qk_norm_rope(queries, keys, query_weight, key_weight, positions, theta: float = 10000.0, eps: float = 1e-6, out=None, stream=None):
     """The norm of each head of queries and keys, fp16 [tokens, heads, head_dim], and its rotation by `positions` (int32 [tokens]; what `plan` and `tree`
-    give) in one pass; a token's heads are contiguous, tokens may be apart.  The weights are fp16 [head_dim].  out: a pair of tensors, None: in
-    place.  Returns the pair."""
+    give) in one pass; a token's heads are contiguous, tokens may be apart.  The weights are fp16 [head_dim].  out: a pair of tensors that share no
+    memory with the arguments, None: in place.  Returns the pair."""
     _load_torch()
     on = _device_of(queries, "queries")
     if len(queries.shape) != 3:
