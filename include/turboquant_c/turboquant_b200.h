@@ -607,7 +607,7 @@ int tq_paged_plan(tq_paged_cache_t cache, const int* rows, const int* counts, in
 int tq_paged_truncate(tq_paged_cache_t cache, const int* rows, const int* lengths, int n, void* stream);
 /** The planned tokens as trees of drafts: parents [tokens] (device memory) is each token's parent, counted from its request's first new token and in
  *  front of it, or -1: none; NULL: the token in front.  positions [tokens] (may be NULL): what the request held before and the token's depth, 0
- *  behind the last.  A request whose new tokens are a chain may have any number of them, another one 256.  A request whose parents are no tree has
+ *  behind the last; at the parents' address or apart from them.  A request whose new tokens are a chain may have any number of them, another one 256.  A request whose parents are no tree has
  *  no attention (tq_paged_status tells); its positions are 0.  In force until the plan ends. */
 int tq_paged_tree(tq_paged_cache_t cache, const int* parents, int tokens, int* positions, void* stream);
 /** Of request i's new tokens the kept[i] ones path[i, 0 .. ] stay, ascending (as tq_verify_drafts gives them), all of them where kept[i] is below

@@ -69,3 +69,22 @@ def test_results_of_norms_over_their_arguments(tq):
     want = tq.qk_norm_rope(q1, k1, *w, positions[:1], out=(torch.empty_like(q1), torch.empty_like(k1)))
     tq.qk_norm_rope(q1, k1, *w, positions[:1], out=(q1.as_strided((1, heads, dim), (5 * step, dim, 1)), k1))
     assert torch.equal(q1, want[0]) and torch.equal(k1, want[1])
+
+
+def test_positions_over_parents(tq):
+    """At the same address: in their place.  Shifted: refused, since a request's would lie over another one's parents."""
+    c = tq.PagedKVCache(1, 1, 64, 40, 16, 20, 4, 256)
+    c.plan(np.array([3, 0, 9], np.int32))
+    c.plan(np.array([5] * 20, np.int32))
+    block = ints([0] * 4 + [-1, 0, 0, 1, 3] * 20 + [0] * 4)
+    for at in (0, 1, 3, 5, 8):
+        with pytest.raises(tq.TQError, match="must not be where"):
+            c.tree(block[4:104], positions=block[at:at + 100])
+    positions = torch.zeros(100, dtype=torch.int32, device="cuda")
+    c.tree(block[4:104], positions=positions)
+    c.tree(block[4:104], positions=block[4:104])
+    want = [held + d for held in [3, 0, 9] + [0] * 17 for d in (0, 1, 1, 2, 3)]
+    assert positions.tolist() == want and block.tolist() == [0] * 4 + want + [0] * 4
+    torch.cuda.synchronize()
+    c.check_status()
+    c.close()

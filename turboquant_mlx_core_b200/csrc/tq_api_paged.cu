@@ -119,6 +119,9 @@ public:
         TQ_REQUIRE(tokens == plan_.tokens, "paged tree: the plan is for " + std::to_string(plan_.tokens) + " tokens");
         TQ_REQUIRE(!parents || tokens == 0 || tq::is_device_pointer(parents), "paged tree: parents must be a device pointer");
         TQ_REQUIRE(!positions || tokens == 0 || tq::is_device_pointer(positions), "paged tree: positions must be a device pointer");
+        // (a request's CTA reads all of its parents before it writes its positions, but others' it does not know)
+        TQ_REQUIRE(positions == parents || tq::ranges_apart(positions, 4ul * tokens, parents, 4ul * tokens),
+                   "paged tree: positions must not be where the parents are, but for the same address");
         begin(st);
         tq::launch_paged_tree({b_, parents, positions, plan_, d_status_}, st);
         tree_ = true;
