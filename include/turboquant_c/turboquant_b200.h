@@ -630,7 +630,8 @@ int tq_paged_read(tq_paged_cache_t cache, int layer, const int* pages, int n, vo
  *  max(0, p - window + 1) .. p, all up to p with window 0.  q_heads is a multiple of the KV heads, whose groups are
  *  contiguous.  scale 0: 1 / sqrt(head_dim).  out fp16 of the queries' shape, strides in elements from token to token; lse
  *  (may be NULL): fp32 [tokens, q_heads], the log of each softmax denominator, with which parts merge
- *  (tq_exchange_merge_attention).  Rows behind the last request's are left as they are.  Results do not depend on the order in which
+ *  (tq_exchange_merge_attention).  Results may be where the queries are, with the same stride, and not otherwise over them or one another.  Rows
+ *  behind the last request's are left as they are.  Results do not depend on the order in which
  *  CTAs run.
  *
  *  Scores, softmax and sums are fp32 (a score beyond its range makes its row NaN); the weights are rounded to halves for their product

@@ -88,3 +88,36 @@ def test_positions_over_parents(tq):
     torch.cuda.synchronize()
     c.check_status()
     c.close()
+
+
+@pytest.mark.parametrize("counts", [[2, 1, 4], [40, 3, 70]])
+def test_results_of_attention_over_the_queries(tq, counts):
+    """In place, as chains through both calls: few rows, many, and both in a batch over a context that several CTAs share."""
+    c = tq.PagedKVCache(1, 2, 64, 120, 64, 3, 60, 4096)
+    x = torch.randn((3500, 2, 64), device="cuda").half()
+    c.plan(np.array([3000, 0, 500], np.int32))
+    c.append(0, x, x)
+    tokens, heads = sum(counts), 6
+    c.plan(np.array(counts, np.int32))
+    c.tree()
+    c.append(0, x[:tokens], x[:tokens])
+    step = heads * 64 + 2 * 64
+    block = torch.randn((tokens + 1) * step, device="cuda").half()
+    slot = lambda at=0, stride=step: block[at:].as_strided((tokens, heads, 64), (stride, 64, 1))      # noqa: E731
+    before, numbers = block.clone(), block.view(torch.float32)
+    for call in (c.attention, c.tree_attention):
+        for out in (slot(stride=heads * 64), slot(step), slot(64), slot(2 * 64)):
+            with pytest.raises(tq.TQError, match="must be where"):
+                call(0, slot(), out=out)
+        apart = torch.empty((tokens, heads, 64), dtype=torch.float16, device="cuda")
+        for out, lse in ((apart, numbers[:tokens * heads]), (apart, apart.view(-1).view(torch.float32)[:tokens * heads])):
+            with pytest.raises(tq.TQError, match="lse must not be"):
+                call(0, slot(), out=out, lse=lse.view(tokens, heads))
+        assert torch.equal(block, before)
+        call(0, slot(), out=apart)
+        call(0, slot(), out=slot())
+        assert torch.equal(slot(), apart)
+        block.copy_(before)
+    torch.cuda.synchronize()
+    c.check_status()
+    c.close()

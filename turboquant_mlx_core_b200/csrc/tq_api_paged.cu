@@ -197,6 +197,12 @@ public:
                    "paged attention: queries and results must be device pointers");
         const long row = static_cast<long>(q_heads) * dim_;
         TQ_REQUIRE(q_stride >= row && out_stride >= row, "paged attention: a token's stride is shorter than its heads");
+        // (in place the rows of a request and head are written by the CTA that has read them, or by the kernel behind; anywhere else over the queries they
+        // may be another's that has not)
+        const tq::ByteRows from{q, 2ul * row, tokens, 2ul * q_stride}, to{out, 2ul * row, tokens, 2ul * out_stride}, logs{lse, 4ul * tokens * q_heads, lse ? 1 : 0};
+        TQ_REQUIRE((out == q && (tokens == 1 || out_stride == q_stride)) || tq::rows_apart(to, from),
+                   "paged attention: results must be where the queries are, with the same stride, or not where they are");
+        TQ_REQUIRE(tq::rows_apart(logs, from) && tq::rows_apart(logs, to), "paged attention: lse must not be where queries or results are");
         begin(st);
         tq::PagedAttnArgs a{};
         a.b = b_;
