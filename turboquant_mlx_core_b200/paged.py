@@ -90,6 +90,8 @@ def _rows(x, heads, dim, what, device):
         d = None
     if d != dim or (heads and n != heads):
         raise ValueError(f"{what} must be [tokens, {heads or 'heads'}, {dim}]")
+    if (tokens | n | d) > 0x7fffffff:
+        raise ValueError(f"the sizes of {what} must fit in 32 bits")
     if one != 1 or (head != dim and n > 1):
         raise ValueError(f"the heads of a token of {what} must be contiguous")
     return x.data_ptr(), tokens, n, step if tokens > 1 else max(n * dim, step)
@@ -98,7 +100,7 @@ def _rows(x, heads, dim, what, device):
 def _number(x, what):
     if len(x.shape) != 1:
         raise ValueError(f"{what} must have one dimension")
-    return x.shape[0]
+    return _fits(x.shape[0], f"the size of {what}")
 
 
 def _tag(x, what):
@@ -190,6 +192,8 @@ class PagedKVCache:
         if len(path.shape) != 2:
             raise ValueError("keep: path must be [n, width]")
         n, width = path.shape
+        if (n | width) > 0x7fffffff:
+            raise ValueError("the sizes of path must fit in 32 bits")
         on = self._device
         if self._L.tq_paged_keep(self._h, _ints(path, "path", n * width, on), width, _ints(kept, "kept", n, on), n, _ints(lengths, "lengths", n, on),
                                  None if stream is None else _stream_ptr(stream)):
@@ -341,6 +345,8 @@ def verify_drafts(starts, parents, tokens, target, draft, uniforms, path, kept, 
         step, one = target.stride()
     except ValueError:
         raise ValueError("path must be [n, width], target [rows, vocab]") from None
+    if (n | width | rows | vocab) > 0x7fffffff:
+        raise ValueError("the sizes of path and target must fit in 32 bits")
     if _device_of(target, "target") != on:
         raise ValueError("target is on another device than starts")
     dp, drafted = None, 0
@@ -362,7 +368,7 @@ def verify_drafts(starts, parents, tokens, target, draft, uniforms, path, kept, 
     if _device_of(uniforms, "uniforms") != on:
         raise ValueError("uniforms are on another device than starts")
     if _lib.load().tq_verify_drafts(_ints(starts, "starts", n + 1, on), _ints(parents, "parents", rows, on), _ints(tokens, "tokens", rows, on), n, rows, target.data_ptr(),
-                                    dp, TQ_F32 if target.dtype is _float32 else _tag(target, "verify_drafts"), _fits(vocab, "vocab"), step, drafted, uniforms.data_ptr(),
+                                    dp, TQ_F32 if target.dtype is _float32 else _tag(target, "verify_drafts"), vocab, step, drafted, uniforms.data_ptr(),
                                     _ints(path, "path", n * width, on), width, _ints(kept, "kept", n, on), _ints(next, "next", n, on),
                                     None if stream is None else _stream_ptr(stream)):
         check(-1, "verify_drafts")
