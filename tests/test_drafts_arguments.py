@@ -62,3 +62,13 @@ def test_sizes_that_do_not_fit(cache, monkeypatch, wide):  # noqa: F811
     rope()
     cache.tree_attention(0, Sized(3, 2, 64, **half), out=Sized(3, 2, 64, **half))
     assert [c[0] for c in cache._L.calls] == ["tq_paged_tree", "tq_paged_keep", "tq_verify_drafts", "tq_qk_norm_rope_f16", "tq_paged_tree_attention"]
+
+
+@pytest.mark.parametrize("name", ["attention", "tree_attention"])
+def test_errors_name_their_call(cache, monkeypatch, name):  # noqa: F811
+    monkeypatch.setattr(cache._L, f"tq_paged_{name}", lambda *a: -1, raising=False)
+    x = Sized(3, 2, 64, dtype=torch.float16)
+    with pytest.raises(tq.TQError, match=rf"PagedKVCache\.{name}\b"):
+        getattr(cache, name)(0, x, out=x)
+    with pytest.raises(TypeError, match=rf"^{name}: queries"):
+        getattr(cache, name)(0, Sized(3, 2, 64, dtype=torch.float32))

@@ -222,16 +222,16 @@ class PagedKVCache:
     def attention(self, layer: int, queries, window: int = 0, scale: float = 0.0, out=None, lse=None, stream=None):
         """Causal attention of the planned tokens' queries, fp16 [tokens, q_heads, head_dim], over their requests; returns out.  A `window` of w
         lets a token see itself and the w - 1 before it.  lse: fp32 [tokens, q_heads], filled with the log of the softmax denominators."""
-        return self._attend(self._L.tq_paged_attention, layer, queries, window, scale, out, lse, stream)
+        return self._attend(self._L.tq_paged_attention, "attention", layer, queries, window, scale, out, lse, stream)
 
     def tree_attention(self, layer: int, queries, window: int = 0, scale: float = 0.0, out=None, lse=None, stream=None):
         """The same for tokens that are trees of drafts (`tree`): a token sees those in front of its request's new ones, its ancestors and itself."""
-        return self._attend(self._L.tq_paged_tree_attention, layer, queries, window, scale, out, lse, stream)
+        return self._attend(self._L.tq_paged_tree_attention, "tree_attention", layer, queries, window, scale, out, lse, stream)
 
-    def _attend(self, call, layer, queries, window, scale, out, lse, stream):
+    def _attend(self, call, name, layer, queries, window, scale, out, lse, stream):
         qp, tokens, q_heads, qs = _rows(queries, 0, self.head_dim, "queries", self._device)
         if queries.dtype is not _float16:
-            raise TypeError("attention: queries must be float16")
+            raise TypeError(f"{name}: queries must be float16")
         if out is None:
             out = _zeros_like(queries, stream)
         op, more, _, os_ = _rows(out, q_heads, self.head_dim, "out", self._device)
@@ -248,7 +248,7 @@ class PagedKVCache:
             _fits(layer, "layer")
             _fits(window, "window")
         if call(self._h, layer, qp, tokens, q_heads, qs, window, scale, op, os_, lp, None if stream is None else _stream_ptr(stream)):
-            check(-1, "PagedKVCache.attention")
+            check(-1, f"PagedKVCache.{name}")
         return out
 
     def read_pages(self, layer: int, pages, keys=None, values=None, stream=None):
