@@ -59,6 +59,15 @@ struct __align__(16) PagedNode {
     int pre, last, depth;
     int good;            // of a request whose parents make a tree
 };
+// Whether the node of a number is the one that begins at `pre`, or below it (span = last - pre).  In unsigned numbers, where a difference below 0 is a
+// large one; kNoNode with a span of 0 stands for what is no node: nothing is below it.
+constexpr int kNoNode = static_cast<int>(0x80000000u);
+__host__ __device__ constexpr bool node_below(int number, int pre, unsigned int span) {
+    return static_cast<unsigned int>(number) - static_cast<unsigned int>(pre) <= span;
+}
+// (a constant expression has no signed overflow)
+static_assert(node_below(5, 3, 2) && node_below(3, 3, 0) && !node_below(6, 3, 2) && !node_below(2, 3, 2) && !node_below(0, 3, 200));
+static_assert(!node_below(0, kNoNode, 0) && !node_below(255, kNoNode, 0) && !node_below(0x7fffffff, kNoNode, 0));
 // A run of new tokens in one page.
 struct PagedPiece {
     int token, count, page, offset;

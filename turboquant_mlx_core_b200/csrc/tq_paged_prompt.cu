@@ -264,7 +264,7 @@ __device__ __noinline__ uint64_t seen_nodes(const PagedAttnArgs& a, const Segmen
     for (int h = 0; h < 2; ++h) {
         const int token = tb + 32 * h + lane;
         const bool there = token >= at.first && token < at.held;
-        int lo = static_cast<int>(0x80000000u), place = 0;   // (no number is in there)
+        int lo = kNoNode, place = 0;
         unsigned int span = 0;
         if (there) {
             const PagedNode node = a.b.nodes[at.start + token - at.first];
@@ -281,7 +281,7 @@ __device__ __noinline__ uint64_t seen_nodes(const PagedAttnArgs& a, const Segmen
             for (int k = 0; k < 4; ++k) {
                 const int e = e0 + k, lo_e = __shfl_sync(0xffffffffu, lo, e), place_e = __shfl_sync(0xffffffffu, place, e);
                 const unsigned int span_e = __shfl_sync(0xffffffffu, span, e);
-                if (static_cast<unsigned int>(number - lo_e) <= span_e && (a.window <= 0 || place_e > pos - a.window)) bits |= 1u << e;
+                if (node_below(number, lo_e, span_e) && (a.window <= 0 || place_e > pos - a.window)) bits |= 1u << e;
             }
         }
         seen |= static_cast<uint64_t>(bits) << (32 * h);
