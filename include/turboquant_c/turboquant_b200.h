@@ -384,9 +384,9 @@ int tq_rope_qk_f16(void* q_fp16, void* k_fp16, const int* positions, long rows, 
 int tq_swiglu_f16(const void* gate_up_fp16, void* act_fp16, long rows, int intermediate, void* stream);
 /** The norm of each query and key head and its rotation in one pass, fp16: y = x * rsqrt(mean(x^2) + eps) * weight over a head's head_dim
  *  elements, then y_i and y_{i + head_dim/2} turned by positions[row] * theta^(-2i/head_dim).  fp32 arithmetic with one rounding at the end;
- *  angles as fractions of a turn in 64 bits, right at any position.  Row r's heads are contiguous, at r * stride elements (heads * head_dim or
- *  more: a slice of a fused projection's result).  Results may go to where their rows are, with the same stride, and not otherwise over an argument or
- *  one another.  head_dim a multiple of 16, up to 512; weights [head_dim].
+ *  angles are fractions of a turn in 64 bits, off by |position| * 2^-51 turns at most.  Row r's heads are contiguous, at r * stride elements
+ *  (heads * head_dim or more: a slice of a fused projection's result).  Results may go to where their rows are, with the same stride, and not
+ *  otherwise over an argument or one another.  head_dim a multiple of 16, up to 512; weights [head_dim].
  *  All pointers are device pointers of one device, whichever is current.  Fastest where pointers and strides are multiples of 16 bytes. */
 int tq_qk_norm_rope_f16(const void* q_fp16, const void* k_fp16, const void* q_weight_fp16, const void* k_weight_fp16, const int* positions, long rows,
                         int q_heads, int kv_heads, int head_dim, long q_stride, long k_stride, float eps, float theta, void* q_out_fp16, void* k_out_fp16,

@@ -95,8 +95,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(__half* __restr
 //   y = x rsqrt(mean(x^2) + eps) w,  (y_i, y_{i + D/2}) turned by position * theta^(-2 i / D)
 //
 // fp32 from the sum of squares to the rotation, one rounding at the end.  The angle is a fraction of a turn: position times the frequency in units
-// of 2^-64 turns, of which a 64-bit product keeps the fraction, 2^-34 off at most whatever the position (in fp32 it is a hundredth off at
-// position 131072).
+// of 2^-64 turns, of which a 64-bit product keeps the fraction without a rounding.  The frequencies come from 64-bit floats: 25 of their roundings, of
+// 2^-53 of a frequency each, are 2^-51 turns at most (against 60 digits, theta 10 to 5e8 and heads of 16 to 512: 2^-54), so that the fraction is off
+// by that times the position: 2^-30 turns at position 2^24, 2^-23 at 2^31, beside the 2^-26 of its rounding to 24 bits (a product in fp32 is a
+// hundredth of a radian off at position 131072).
 //
 // A thread takes eight pairs of a head, 16 bytes from either half, so that the rotation stays in its registers, and the same pairs of the same head
 // in several rows, so that it keeps the weights and finds its place once; `lanes` threads, the next power of two above D / 16, share a head and its sum
@@ -332,7 +334,7 @@ void launch_qk_norm_rope_f16(const __half* q, const __half* k, const __half* q_w
     a.lanes = 1;
     while (a.lanes * 16 < dim) a.lanes *= 2;
     constexpr double kTwoPi = 6.283185307179586476925286766559;
-    // (a power for every eighth, the others eight products of it at most: 2^-50 off, where a power each took two thirds of the call)
+    // (a power for every eighth, the others up to seven products of it, 25 2^-53 off in all, where a power each took two thirds of the call)
     const double ratio = std::pow(static_cast<double>(theta), -2.0 / dim);
     for (int i = 0; i < dim / 2; i += 8) {
         double turn = std::pow(static_cast<double>(theta), -2.0 * i / dim) / kTwoPi * 18446744073709551616.0;
