@@ -643,7 +643,8 @@ int tq_paged_attention(tq_paged_cache_t cache, int layer, const void* queries_fp
 /** The same for planned tokens that are trees (tq_paged_tree): a token sees those in front of its request's new ones, its ancestors and itself, with
  *  a window those of them whose positions are above its own less the window.  Rows of a request whose parents make no tree are left as they
  *  are.  Weights are rounded to halves: 2^-11 of each at most, and of small ones 2^-32 of the row's largest weight, times the largest scale among
- *  the values that the row sees. */
+ *  the values that the row sees.  Chains may be among the trees, but tq_paged_attention has kernels that are faster for them: for up to 16 query rows
+ *  of a request (half the time over long contexts) and for prompts and chunks (a fifth); so a prompt is better planned apart from drafts. */
 int tq_paged_tree_attention(tq_paged_cache_t cache, int layer, const void* queries_fp16, int tokens, int q_heads, long q_stride, int window,
                             float scale, void* out_fp16, long out_stride, float* lse, void* stream);
 /** Non-zero, once, when a call that has finished found its batch impossible or another plan on the device than the one that it was made for, or a wait

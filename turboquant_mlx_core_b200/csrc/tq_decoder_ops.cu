@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(__half* __restr
 //
 // A thread takes eight pairs of a head, 16 bytes from either half, so that the rotation stays in its registers, and the same pairs of the same head
 // in several rows, so that it keeps the weights and finds its place once; `lanes` threads, the next power of two above D / 16, share a head and its sum
-// of squares.  It is bound by memory, 16 bytes in and out for eight elements (few rows: by latency, 2.6 us): a row's values are asked for while the one
+// of squares.  It is bound by memory, 16 bytes in and out for eight elements (few rows: by latency, 2.4 us replayed in a graph, as all times here): a row's values are asked for while the one
 // before is at work, the first one's in front of the sines and cosines, which D / 2 threads take for all heads of a row.  8192 rows of 40 + 8 heads of
 // 128: 36.5 us, 5.5 TB/s, 84 % of a plain copy's rate (52 with a row to a CTA, whose threads find head and pair anew for each 64 bytes; 44.6 with sines
 // and cosines in the pairs' order, where four threads of eight read the same banks; 41.5 in 75 registers, of which two CTAs of 384 threads fill an SM

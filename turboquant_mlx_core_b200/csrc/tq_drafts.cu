@@ -15,9 +15,9 @@
 // order.  The warp in whose part the sum passes u0 Z goes over it once more.  Sums, products and comparisons are in 64 bits: a token is a whole
 // number, and a comparison of sums in 32 bits would go wrong next to a border, of which there are as many as tokens.
 //
-// What bounds it: latency.  Few requests: three loads behind one another, a pass, the cluster's barriers, the last part once more, 10 us for one.  Many: the
-// request that takes most passes, each of them some rounds of loads, sums in 64 bits and a barrier of the cluster: 64 requests of 16 nodes in 39 us, 3
-// TB/s of rows out of memory and L2 cache, with a third of the issue slots and a sixth of the conversions' rate in use.
+// What bounds it: latency.  Few requests: three loads behind one another, a pass, the cluster's barriers, the last part once more, 10 us for one (as all
+// times here, replayed in a graph).  Many: the request that takes most passes, each of them some rounds of loads, sums in 64 bits and a barrier of the
+// cluster: 64 requests of 16 nodes in 39 us, 3 TB/s of rows out of memory and L2 cache, with a third of the issue slots and a sixth of the conversions' rate in use.
 
 #include <cooperative_groups.h>
 

@@ -65,7 +65,10 @@ constexpr int kItemUnits = 4;        // what an item's beginning and end cost, i
 constexpr int kStages = 4;           // of keys and of values, as halves
 constexpr int kRefs = 8;             // tiles whose scales are kept
 // Weights are held times 2^7, and at most 2^15: halves that are normal numbers down to 2^-21 of the reference, and 2^-32 of it off below: of 131072
-// tokens' values 2^-15 of the largest one at the very worst, 1/16 of the result's rounding.
+// tokens' values 2^-15 of the largest one at the very worst, 1/16 of the result's rounding.  Their sums are of the numbers before that rounding, so that
+// a row with one large weight is off by that one's, 2^-11 at most: trees whose rows' largest weights are 0.4 at their median are 2.2e-4 to 2.4e-4 of
+// their norm off, 2.05e-4 of which is the results' own rounding.  (With sums of the halves, simulated, 2.2e-4, for 64 conversions more to a row and
+// tile.)
 constexpr float kOffset = 7.f, kSlack = 8.f;
 // Of a tile's values against the largest so far: a weight times 2^-60 is 0 as a half, and their sum, which is taken of these, far from it
 constexpr int kLeastLower = -60;
@@ -93,7 +96,9 @@ struct Request {
     // tiles of the cache that the rows of a pair see
     template <bool TREE>
     __device__ __forceinline__ void tiles(const PagedAttnArgs& a, int pair, int& lo, int& hi) const {
-        if constexpr (TREE) {   // (any row may see any place)
+        // Any row may see any place.  Requests that are chains go the same way, past tiles that a causal row tile leaves out and with a look at the nodes in
+        // each tile of new tokens: 4096 from an empty cache 887 us, under any window (the plain kernel: 182, and 83 with a window of 512).
+        if constexpr (TREE) {
             lo = a.window > 0 ? max(0, first() - a.window + 1) / kTokens : 0;
             hi = (held - 1) / kTokens + 1;
             return;
@@ -326,8 +331,8 @@ __device__ __forceinline__ void add_second(uint32_t (&x)[32], uint32_t taddr, fl
 // TREE: trees of drafts (paged_tree_kernel in tq_paged_plan.cu numbers the nodes): a row sees the tokens in front of the new ones, its ancestors and
 // itself.  A request has some tens to some hundreds of rows there, so that many items have no second row tile; its warps then take every second
 // tile of the cache for the first one's rows, with a maximum, a sum and an O of their own, and the two are added up at the item's end (both read the
-// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 61 thousand tokens of 4 heads: 44 us, 10 of which are one CTA's way to its
-// first product and from its last one to the result.  Over a long cache a tile takes 1.9 thousand cycles with 25 rows as with 125, and 2.7 with two
+// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 61 thousand tokens of 4 heads: 44 us (as all times here, replayed in a
+// graph), 10 of which are one CTA's way to its first product and from its last one to the result.  Over a long cache a tile takes 1.9 thousand cycles with 25 rows as with 125, and 2.7 with two
 // row tiles: for few rows the keys bound it, whose warps' way from one of their tiles to the next (every second one) is 3.7 thousand cycles: 0.5 for
 // the bytes, 1.7 to make them halves, 1.1 to find the next, each instruction behind some 13 cycles of others.  Tried beside it: the
 // products turned around (tokens as their 128 rows, query rows as 32, 64 or 128 columns, a softmax thread per token), which takes a tile's products as
