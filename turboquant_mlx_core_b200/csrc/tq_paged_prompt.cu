@@ -331,9 +331,9 @@ __device__ __forceinline__ void add_second(uint32_t (&x)[32], uint32_t taddr, fl
 // TREE: trees of drafts (paged_tree_kernel in tq_paged_plan.cu numbers the nodes): a row sees the tokens in front of the new ones, its ancestors and
 // itself.  A request has some tens to some hundreds of rows there, so that many items have no second row tile; its warps then take every second
 // tile of the cache for the first one's rows, with a maximum, a sum and an O of their own, and the two are added up at the item's end (both read the
-// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 61 thousand tokens of 4 heads: 44 us (as all times here, replayed in a
-// graph), 10 of which are one CTA's way to its first product and from its last one to the result.  Over a long cache a tile takes 1.9 thousand cycles with 25 rows as with 125, and 2.7 with two
-// row tiles: for few rows the keys bound it, whose warps' way from one of their tiles to the next (every second one) is 3.7 thousand cycles: 0.5 for
+// same lanes of tensor memory).  16 requests of 8 to 16 nodes, 7 rows each, over 61 thousand tokens of 4 heads: 44 us replayed in a
+// graph, 10 of which are one CTA's way to its first product and from its last one to the result.  Over a long cache a tile takes 1.9 thousand cycles
+// with 25 rows as with 125, and 2.7 with two row tiles: for few rows the keys bound it, whose warps' way from one of their tiles to the next (every second one) is 3.7 thousand cycles: 0.5 for
 // the bytes, 1.7 to make them halves, 1.1 to find the next, each instruction behind some 13 cycles of others.  Tried beside it: the
 // products turned around (tokens as their 128 rows, query rows as 32, 64 or 128 columns, a softmax thread per token), which takes a tile's products as
 // long as there are rows: 90 us, since each thread then keeps a sum for every row and four warps have to agree on every reference; keys and values
