@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(kTreeThreads) paged_tree_kernel(PagedTreeArgs 
     const int tid = threadIdx.x, requests = paged_device::planned(a.b.header, a.sizes, a.status).requests;
     if (blockIdx.x == 0) {
         if (tid == 0 && requests > 0) a.b.header->state = kPagedTree;
-        if (a.positions && requests == 0)
+        // (a plan of no requests, or one that was refused: all rows are behind the last; under a plan of other sizes nothing is done)
+        const PagedSizes sizes = const_cast<const PagedHeader*>(a.b.header)->sizes;
+        if (a.positions && requests == 0 && sizes.n == a.sizes.n && sizes.tokens == a.sizes.tokens && sizes.most == a.sizes.most)
             for (int t = tid; t < a.sizes.tokens; t += kTreeThreads) a.positions[t] = 0;
     }
     for (int i = blockIdx.x; i < requests; i += gridDim.x) {
