@@ -92,3 +92,24 @@ def test_large_drafts_that_do_not_stay(tq, page):
     p.compare(20)
     assert p.m[0].exps[0][p.m[0].tables[0][1], 0] == 9
     p.c.close()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_keys_and_values_each_for_themselves(tq, which):
+    """Of fp32 tensors, where either may be out of a half's range."""
+    rng = np.random.default_rng(which)
+    p = Pair(tq, 2, 64, 16, 2, 30)
+    p.step(rng, [16, 3], [0, 1])
+    for m in p.m:
+        m.plan([40, 40], [0, 1])
+    p.c.plan(np.array([40, 40], np.int32), rows=ints([0, 1]))
+    kv = [rng.standard_normal((80, 2, 64)).astype(np.float32) for _ in range(2)]
+    kv[which][2, 0, 1], kv[which][41 + 13, 1, 63], kv[1 - which][9, 1, 0] = np.inf, np.nan, 3e38
+    for i, x in enumerate(kv):
+        p.m[0].append(i, x)
+    p.c.append(0, *(torch.from_numpy(x).cuda() for x in kv))
+    kept(p, [[17, 20, 39], [*range(13), 29, 30]], [0, 1])
+    p.compare(30)
+    exps = [p.m[0].exps[i][p.m[0].tables[r][1]].tolist() for r in (0, 1) for i in (which, 1 - which)]
+    assert None not in exps[0] + exps[1] + exps[2] + exps[3] and exps[1][1] > 100 > exps[0][0]
+    p.c.close()
